@@ -11,6 +11,8 @@ from .build import EXT_PATH, LIB_PATH
 _lib = None
 _ext = None
 
+_P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+
 _C_SIGNATURES = {
     "gdsq_version": (ctypes.c_int, []),
     "gdsq_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -70,6 +72,13 @@ _C_SIGNATURES = {
                                          [ctypes.c_int] * 9 + [ctypes.c_void_p, ctypes.c_void_p]),
     "gdsq_moe_router": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
                                        ctypes.c_void_p, ctypes.c_int] + [ctypes.c_void_p] * 6),
+    "gdsq_build_tables": (ctypes.c_int, [_P, _P, _I, _P, _I, _P, _I, _P, _I, _I] + [_P] * 6),
+    "gdsq_append_kv8": (ctypes.c_int, [_I] + [_P, _L, _L] * 3 + [_P, _P, _I, _P, _P] + [_I] * 5 + [_P] * 4 +
+                        [_I, _I, _P]),
+    "gdsq_attend_kv8_workspace": (ctypes.c_size_t, [_I] * 5),
+    "gdsq_attend_kv8": (ctypes.c_int, [_P, _I, _L, _L, _P, _P, _I, _P, _P, _I, _I, _P, _I, _P, _P] + [_I] * 7 +
+                        [ctypes.c_float, _P, _P, ctypes.c_size_t, _P]),
+    "gdsq_sample": (ctypes.c_int, [_I, _P, _L, _I, _I] + [_P] * 8),
     "gdsq_silu_mul_f16": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong,
                                          ctypes.c_void_p]),
     "gdsq_argmax_f16": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,

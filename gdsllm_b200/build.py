@@ -1,7 +1,8 @@
 """Builds the native parts of gdsllm_b200 in-tree.
 
 * ``_build/libgdsq.so``        every CUDA kernel plus the C ABI of include/gdsq.h,
-                               compiled by nvcc for sm_100a only.
+                               compiled by nvcc for sm_100a only, one object per
+                               ``csrc/*.cu`` (compiled side by side).
 * ``_build/gds_io_ext*.so``    the torch binding that mirrors the reference's
                                ``gdsllm.runtime.gds_io_ext`` module, linked
                                against libgdsq.so.
@@ -12,9 +13,11 @@ Both are rebuilt only when a source is newer than the product.  Run
 from __future__ import annotations
 
 import os
+import re
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -28,9 +31,8 @@ ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + [
     "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC,-fvisibility=hidden",
-    "-Xlinker", "--exclude-libs,ALL",
-    "-Xlinker", "-soname=libgdsq.so",
 ]
+LINK_FLAGS = ["-Xlinker", "--exclude-libs,ALL", "-Xlinker", "-soname=libgdsq.so"]
 
 LIB_PATH = BUILD / "libgdsq.so"
 EXT_PATH = BUILD / ("gds_io_ext" + sysconfig.get_config_var("EXT_SUFFIX"))
@@ -49,13 +51,36 @@ def _run(cmd, verbose):
     subprocess.run([str(c) for c in cmd], check=True)
 
 
+def _sources(path: Path, seen=None):
+    """`path` and the headers of this repository that it includes."""
+    seen = set() if seen is None else seen
+    if path in seen:
+        return seen
+    seen.add(path)
+    for name in re.findall(r'^#include "([^"]+)"', path.read_text(), re.M):
+        for folder in (path.parent, CSRC, INCLUDE):
+            if (folder / name).exists():
+                _sources(folder / name, seen)
+                break
+    return seen
+
+
 def build_lib(force: bool = False, verbose: bool = True) -> Path:
-    sources = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
-    if force or _newer(LIB_PATH, sources):
-        BUILD.mkdir(parents=True, exist_ok=True)
+    BUILD.mkdir(parents=True, exist_ok=True)
+    units = [(src, BUILD / (src.stem + ".o")) for src in sorted(CSRC.glob("*.cu"))]
+    stale = [(src, obj) for src, obj in units if force or _newer(obj, _sources(src))]
+
+    def compile_unit(unit):
+        src, obj = unit
+        tmp = obj.with_suffix(".o.tmp")
+        _run([NVCC, *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, "-c", "-o", tmp, src], verbose)
+        os.replace(tmp, obj)
+
+    with ThreadPoolExecutor(max_workers=4) as pool:
+        list(pool.map(compile_unit, stale))
+    if stale or _newer(LIB_PATH, [obj for _, obj in units]):
         tmp = LIB_PATH.with_suffix(".so.tmp")
-        _run([NVCC, *NVCC_FLAGS, "-I", INCLUDE, "-I", CSRC, "-shared", "-o", tmp,
-              CSRC / "gdsq.cu"], verbose)
+        _run([NVCC, *ARCH_FLAGS, *LINK_FLAGS, "-shared", "-o", tmp, *[obj for _, obj in units]], verbose)
         os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

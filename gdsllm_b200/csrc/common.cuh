@@ -13,7 +13,7 @@
 
 namespace gdsq {
 
-// Kernel-side error word (one per device, in the module's static memory).
+// Kernel-side error word (one per device and translation unit, in the module's static memory).
 // Kernels OR a bit in and return instead of trapping; the host reads it with
 // gdsq_device_error().  Bits:
 enum : int {
@@ -21,7 +21,7 @@ enum : int {
   kDevErrBadArgument = 2,      // a launch saw inconsistent arguments
   kDevErrBadIndex = 4,         // an index read from device memory was out of range
 };
-__device__ int g_device_error;
+static __device__ int g_device_error;
 
 // Upper bound for any wait on an async copy, in nanoseconds of %globaltimer.
 // A weight tile takes microseconds to arrive; one second means "never".

@@ -1,7 +1,9 @@
 // gdsq: C-ABI entry points (include/gdsq.h) and host-side dispatch.
 //
-// One translation unit holds every kernel so that they can share the
-// device-side error word without relocatable device code.
+// This translation unit holds the GEMV, MoE, exchange and decode-step kernels,
+// which share its device-side error word without relocatable device code; the
+// units of the batched-serving kernels have words of their own, and
+// gdsq_device_error reads them all.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
@@ -17,6 +19,7 @@
 #include <unordered_map>
 
 #include "gdsq.h"
+#include "host.h"
 #include "common.cuh"
 #include "dequant.cuh"
 #include "gemv.cuh"
@@ -26,11 +29,11 @@
 #include "decode.cuh"
 
 namespace gdsq {
-namespace {
+
+// ---- host.h -------------------------------------------------------------------
 
 thread_local std::string t_last_error;
 int g_pdl_enabled = 0;
-std::atomic<unsigned long long> g_peer_wait_ns{kPeerWaitDefaultNs};
 
 int fail(int status, const char* fmt, ...) {
   char buf[512];
@@ -47,16 +50,12 @@ int cuda_fail(cudaError_t e, const char* what) {
   return fail(GDSQ_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
-struct DeviceInfo {
-  bool ready = false;
-  int ordinal = 0;
-  int sms = 0;
-  int smem_optin = 0;
-};
-
-constexpr int kMaxDevices = 64;
+namespace {
 DeviceInfo g_devices[kMaxDevices];
 std::mutex g_device_mutex;
+std::unordered_map<const void*, int> g_smem_set[kMaxDevices];
+PFN_cuTensorMapEncodeTiled_v12000 g_encode_tiled = nullptr;
+}  // namespace
 
 // Cached per-device attributes (the reference queried device 0 on every
 // launch, gdsllm/runtime/fused_gemv.cu:117-118).
@@ -81,51 +80,15 @@ int device_info(const DeviceInfo** out) {
   return GDSQ_OK;
 }
 
-bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
-
-template <typename... KArgs, typename... Args>
-cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                   cudaStream_t stream, bool pdl, Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  cfg.attrs = attr;
-  cfg.numAttrs = 0;
-  if (pdl) {
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 1;
-  }
-  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-}
-
-// Raises a kernel's dynamic shared-memory limit when a launch needs more than
-// was last set for that (kernel, device).
-std::unordered_map<const void*, int> g_smem_set[kMaxDevices];
-
-template <typename K>
-cudaError_t ensure_smem(K kernel, int bytes, int device) {
+cudaError_t ensure_smem_limit(const void* kernel, int bytes, int device) {
   if (bytes <= 48 * 1024) return cudaSuccess;
-  const void* key = reinterpret_cast<const void*>(kernel);
   std::lock_guard<std::mutex> lock(g_device_mutex);
-  auto it = g_smem_set[device].find(key);
+  auto it = g_smem_set[device].find(kernel);
   if (it != g_smem_set[device].end() && it->second >= bytes) return cudaSuccess;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess) g_smem_set[device][key] = bytes;
+  if (e == cudaSuccess) g_smem_set[device][kernel] = bytes;
   return e;
 }
-
-// ---------------------------------------------------------------------------
-// Weight tensor maps for the TMA loads of the fast GEMV.  A packed weight
-// matrix is described as a 2-D tensor of 8-byte elements: [N rows][row_bytes
-// / 8], row pitch row_bytes; one box is 32 rows x one 256-column chunk.
-// Encoded maps are cached per (pointer, shape, format, device), so repeated
-// calls on resident weights (a decode loop) pay only a hash lookup.
-
-PFN_cuTensorMapEncodeTiled_v12000 g_encode_tiled = nullptr;
 
 int get_encoder(PFN_cuTensorMapEncodeTiled_v12000* out) {
   static std::once_flag once;
@@ -141,6 +104,17 @@ int get_encoder(PFN_cuTensorMapEncodeTiled_v12000* out) {
   *out = g_encode_tiled;
   return GDSQ_OK;
 }
+
+namespace {
+
+std::atomic<unsigned long long> g_peer_wait_ns{kPeerWaitDefaultNs};
+
+// ---------------------------------------------------------------------------
+// Weight tensor maps for the TMA loads of the fast GEMV.  A packed weight
+// matrix is described as a 2-D tensor of 8-byte elements: [N rows][row_bytes
+// / 8], row pitch row_bytes; one box is 32 rows x one 256-column chunk.
+// Encoded maps are cached per (pointer, shape, format, device), so repeated
+// calls on resident weights (a decode loop) pay only a hash lookup.
 
 struct MapKey {
   uintptr_t ptr;
@@ -1186,6 +1160,8 @@ int gdsq_device_error(int device, int clear, int* out_bits) {
     const int zero = 0;
     e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
   }
+  if (e == cudaSuccess) e = serve_error_bits(clear != 0, &bits);
+  if (e == cudaSuccess) e = attend_error_bits(clear != 0, &bits);
   cudaSetDevice(prev);
   if (e != cudaSuccess) return cuda_fail(e, "reading the device error word");
   *out_bits = bits;

@@ -241,6 +241,7 @@ GDSQ_API int gdsq_allreduce_sum_f16(const void* in, void* out, int n, const void
 
 #define GDSQ_ELEM_F16 0
 #define GDSQ_ELEM_F32 1
+#define GDSQ_ELEM_BF16 3
 #define GDSQ_ELEM_F32_TO_F16 2 /* fp32 in; out fp16 of the sum clamped to +-65504 (qwen_moe.py:514) */
 
 /* out[i] = sum over ranks r (in rank order, fp32) of in_r[i], fp16 or fp32
@@ -356,6 +357,92 @@ GDSQ_API int gdsq_silu_mul_f16(const void* gate, const void* up, void* out, long
 /* *token = the first index of the largest of n fp16 logits (torch.argmax);
  * then *pos += 1 when pos is not NULL. */
 GDSQ_API int gdsq_argmax_f16(const void* logits, int n, long long* token, long long* pos, void* stream);
+
+/* ---- Batched serving over a paged 8-bit KV cache ------------------------ */
+
+/* No reference counterpart: the reference serves one request at a time over
+ * an fp16 cache (kv_cache.py:35-67) and samples on the host (engine.py:47-95).
+ *
+ * The cache of one layer is two arrays of 8-bit codes [num_blocks]
+ * [num_kv_heads][block_size][head_dim] (K and V, 128-byte aligned), each with
+ * fp32 scales [num_blocks][num_kv_heads]; a value is code * scale.  A request
+ * owns the blocks its row of the block table names; token position p sits in
+ * slot table[p / block_size] * block_size + p % block_size.
+ * block_size 16, 32, 64 or 128; head_dim 64, 128 or 256. */
+#define GDSQ_CACHE_INT8 0 /* codes -127..127 */
+#define GDSQ_CACHE_E4M3 1 /* 8-bit floating point, largest 448 */
+
+/* One step's bookkeeping from the request lengths: request r holds
+ * context_lens[r] tokens and gets new_lens[r] more.  Fills the block table's
+ * new entries from the queue of free blocks (free_blocks[*free_head...], in
+ * request order), seq_lens[r] = context + new, query_starts [requests + 1] =
+ * the running sum of new_lens, and for each of the num_tokens new tokens its
+ * position and slot; tokens past the last request get position 0, slot -1.
+ * *free_head_out = *free_head + blocks taken (not the same address).  All
+ * arrays int32 except positions and slots (int64).  At most 16384 requests.
+ * A negative length, a row or queue that is too short or more new tokens than
+ * num_tokens sets device error bit 4; the entries it concerns become -1. */
+GDSQ_API int gdsq_build_tables(const int32_t* context_lens, const int32_t* new_lens, int num_requests,
+                               int32_t* block_table, int table_width, const int32_t* free_blocks, int num_free,
+                               const int32_t* free_head, int block_size, int num_tokens, int32_t* seq_lens,
+                               int32_t* query_starts, long long* positions, long long* slots,
+                               int32_t* free_head_out, void* stream);
+
+/* Writes k and v [num_tokens][num_kv_heads][head_dim] (elem_type GDSQ_ELEM_F16
+ * or GDSQ_ELEM_BF16, strides in elements, multiples of 8) into the cache slots
+ * `slots` (int64; -1 = skip; the tokens of one block are adjacent).  With
+ * freqs (fp32 cos/sin pairs [max_position][head_dim / 2]) k is rotated by its
+ * token's position first, and q [num_tokens][num_heads][head_dim], if given,
+ * into q_out (contiguous).  The scale of a block the new tokens begin is
+ * their largest magnitude / 127 (448); a block partly filled before keeps its
+ * scale while that suffices, else takes max(what they need, twice its scale)
+ * and its codes are rounded again.  A non-finite value is stored as 0 under a
+ * NaN scale, so that only queries that see its block turn NaN.  A slot or
+ * position out of range sets device error bit 4 and is not written. */
+GDSQ_API int gdsq_append_kv8(int elem_type, const void* q, long long q_token_stride, long long q_head_stride,
+                             const void* k, long long k_token_stride, long long k_head_stride, const void* v,
+                             long long v_token_stride, long long v_head_stride, void* q_out, const void* freqs,
+                             int max_position, const long long* positions, const long long* slots, int num_tokens,
+                             int num_heads, int num_kv_heads, int head_dim, int cache_type, void* k_cache,
+                             void* v_cache, float* k_scale, float* v_scale, int num_blocks, int block_size,
+                             void* stream);
+
+/* Attention of the new tokens q [num_tokens][num_heads][head_dim] (strides in
+ * elements, multiples of 8; 16-byte aligned) over the cache: the tokens
+ * query_starts[r] .. query_starts[r+1]-1 are the last new tokens of request
+ * r's seq_lens[r], and each sees the positions up to its own.  Query heads
+ * h*G..h*G+G-1 (G = num_heads / num_kv_heads) read KV head h.  out: contiguous,
+ * q's type; a query that sees nothing gives zeros.  max_query_len and
+ * max_seq_len bound the requests' new tokens and lengths (they size the
+ * launch; tokens past max_query_len of a request are left unwritten).
+ * workspace: workspace_bytes of device memory, zeroed before its first use
+ * and left zeroed where it has to be by every call; calls that may overlap
+ * need one each.  gdsq_attend_kv8_workspace says how much a call can use. A
+ * block table entry out of range sets device error bit 4 and reads block 0. */
+GDSQ_API size_t gdsq_attend_kv8_workspace(int num_requests, int max_query_len, int num_heads, int num_kv_heads,
+                                          int head_dim);
+GDSQ_API int gdsq_attend_kv8(const void* q, int elem_type, long long q_token_stride, long long q_head_stride,
+                             const void* k_cache, const void* v_cache, int cache_type, const float* k_scale,
+                             const float* v_scale, int num_blocks, int block_size, const int32_t* block_table,
+                             int table_width, const int32_t* seq_lens, const int32_t* query_starts,
+                             int num_requests, int num_tokens, int max_query_len, int max_seq_len, int num_heads,
+                             int num_kv_heads, int head_dim, float softmax_scale, void* out, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+#define GDSQ_SAMPLE_MAX_VOCAB 524288
+
+/* One token per row of logits [num_rows][vocab] (fp16, bf16 or fp32; rows
+ * row_stride elements apart) from one uniform number per row in [0, 1):
+ * temperature (<= 0: the largest logit), then top_k (<= 0: off), top_p of the
+ * top_k's weight, and min_p times the largest probability; each an array of
+ * num_rows or NULL (1, off, 1, 0).  Weights are whole numbers,
+ * floor(2^31 exp((l - max) / temperature)), so equal inputs give equal tokens
+ * whatever the launch.  Ties keep the lowest index; NaN counts as -inf; a row
+ * of nothing but -inf gives token -1 (and logprob -inf).  logprobs (fp32, may
+ * be NULL): the log of the token's share of the kept weight. */
+GDSQ_API int gdsq_sample(int elem_type, const void* logits, long long row_stride, int num_rows, int vocab,
+                         const float* uniforms, const float* temperature, const int32_t* top_k, const float* top_p,
+                         const float* min_p, long long* tokens, float* logprobs, void* stream);
 
 #ifdef __cplusplus
 }
