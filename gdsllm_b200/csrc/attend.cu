@@ -30,7 +30,9 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <cstring>
+#include <functional>
+#include <mutex>
+#include <unordered_map>
 
 #include "gdsq.h"
 #include "host.h"
@@ -110,9 +112,48 @@ struct Code<GDSQ_CACHE_E4M3> {
   }
 };
 
-__device__ __forceinline__ float load_q(const AttendArgs& p, long long i) {
-  return p.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.q)[i])
-                : __half2float(static_cast<const __half*>(p.q)[i]);
+__device__ __forceinline__ float2 unpack_q(bool bf16, uint32_t w) {
+  return bf16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w)) : __half22float2(u32_as_h2(w));
+}
+
+// N pairs of one q row, from element i (aligned to N pairs).
+template <int N>
+__device__ __forceinline__ void load_q(const AttendArgs& p, long long i, uint32_t (&w)[N]) {
+  const uint16_t* src = static_cast<const uint16_t*>(p.q) + i;
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(src);
+  } else if constexpr (N == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(src);
+    w[0] = x.x; w[1] = x.y;
+  } else {
+    const uint4 x = *reinterpret_cast<const uint4*>(src);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+  }
+}
+
+// The cache is read once where one tile of rows covers a request's queries.
+__device__ __forceinline__ uint64_t l2_policy_normal() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+
+// Four dims of one output row.
+__device__ __forceinline__ void store_out(const AttendArgs& p, int start, int h, int row, int d, const float (&num)[4],
+                                          float den) {
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  const long long at = (long long)(start + row / p.group) * p.out_token_stride +
+                       (long long)(h * p.group + row % p.group) * p.out_head_stride + d;
+  uint2 v;
+  if (p.bf16) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(num[0] * inv, num[1] * inv);
+    const __nv_bfloat162 b = __floats2bfloat162_rn(num[2] * inv, num[3] * inv);
+    v = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  } else {
+    v = make_uint2(h2_as_u32(__floats2half2_rn(num[0] * inv, num[1] * inv)),
+                   h2_as_u32(__floats2half2_rn(num[2] * inv, num[3] * inv)));
+  }
+  *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + at) = v;
 }
 
 // Per-page constants of the softmax: x = kscale factor, y = lv, z = 2^-lv.
@@ -126,297 +167,611 @@ __device__ __forceinline__ float3 page_constants(const AttendArgs& p, int page, 
   return make_float3(ks * p.scale, fine ? lv : __int_as_float(0x7fffffff), fine ? exp2f(-lv) : 1.f);
 }
 
-// Grid (row tiles, kv_heads, requests), 4 warps.  A CTA owns 16 * MT rows of
-// one (request, KV head); its warps take every fourth tile of 32 tokens and
-// their sums are joined in shared memory at the end.
+// ---------------------------------------------------------------------------
+// Few rows per (request, KV head): single tokens, drafts, short chunks.
+//
+// Bound by reading the cache, so the work is cut by cache tokens, evenly: an
+// item is (request, KV head, tile of 16 * MT rows), its steps are 128 tokens
+// each, and CTA c of C takes the steps [c S / C, (c + 1) S / C) of all items in
+// order.  An item that ends in the CTA it began in is written out; the others
+// leave partial sums, and the CTA that arrives last at an item's counter adds
+// them in CTA order.  So neither ragged lengths nor few requests leave SMs
+// idle, and the result does not depend on who finishes first.
+//
+// In a step, warp w takes the 32 tokens from 32 w, through its own ring of
+// TMA boxes of 16 tokens (one block holds at least 16).  A lane looks up the
+// block, scales and constants of one half tile for 16 tiles at a time.
 //
 // Matrix operand layout: in m16n8k16 a lane (g = lane / 4, t = lane % 4) feeds
 // B[k = 2t, 2t+1, 2t+8, 2t+9][n = g].  The order of the summed index is free,
 // so for the scores (k = dim, n = token) lane t takes 32 consecutive dims of
 // token g: two 16-byte loads.  For the output (k = token, n = dim) lane g
-// takes 16 consecutive dims of tokens 2t, 2t+1, 2t+8, 2t+9.
+// takes 16 consecutive dims of tokens 2t, 2t+1, 2t+8, 2t+9.  With the 128-byte
+// TMA swizzle both are free of bank conflicts.
+
+constexpr int kStepTokens = kAttWarps * 32;
+constexpr int kRing = 2;  // stages per warp
+
+template <int HD, int MT>
+struct StreamLayout {
+  static constexpr int kStage = 2 * 32 * HD;  // K and V of 32 tokens
+  static constexpr int kRingBytes = kAttWarps * kRing * kStage;
+  static constexpr int kRows = 16 * MT;
+  static constexpr int kJoin = kAttWarps * 16 * HD * 4;  // one m tile of every warp, in the ring's memory
+  static constexpr int kQ = MT * (HD / 16) * 512;
+  static constexpr int kBars = kRingBytes + kQ;
+  static constexpr int kRowInfo = kBars + 128;
+  static constexpr int kMl = kRowInfo + kRows * 8;                 // [warps][kRows] m, l
+  static constexpr int kTotal = kMl + kAttWarps * kRows * 8 + 64 + 1024;  // + alignment
+  static_assert(kJoin <= kRingBytes, "the join uses the ring's memory");
+};
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
 template <int HD, int F, int MT>
-__global__ void __launch_bounds__(kAttWarps * 32) attend_simple_kernel(const AttendArgs p) {
+__global__ void __launch_bounds__(kAttWarps * 32)
+    attend_stream_kernel(const AttendArgs p, const __grid_constant__ CUtensorMap kmap,
+                         const __grid_constant__ CUtensorMap vmap, float* parts, int* counters) {
+  using L = StreamLayout<HD, MT>;
   constexpr int kParts = HD >= 128 ? HD / 128 : 1;  // 128-dim parts
   constexpr int kPart = HD >= 128 ? 128 : 64;
   constexpr int kWords = kPart / 16;   // 32-bit words of K per lane, token and part (= k16 steps)
   constexpr int kSteps = HD / 16;      // k16 steps of the scores
   constexpr int kTiles = HD / 8;       // n8 tiles of the output
   constexpr int kVWords = kPart / 32;  // 32-bit words of V per lane, token and part
-  constexpr int kRows = 16 * MT;
-  extern __shared__ __align__(16) unsigned char smem[];
-  uint4* qf = reinterpret_cast<uint4*>(smem);                               // [MT][kSteps][32]
-  float* qexp = reinterpret_cast<float*>(smem + MT * kSteps * 512);         // [kRows]
-  int* qlim = reinterpret_cast<int*>(qexp + kRows);                         // [kRows] last visible position
-  float* joined = reinterpret_cast<float*>(qlim + kRows);                   // [warps][kRows][HD]
-  float* jm = joined + kAttWarps * kRows * HD;                              // [warps][kRows]
-  float* jl = jm + kAttWarps * kRows;                                       // [warps][kRows]
+  constexpr int kRows = L::kRows;
+  constexpr int kHalfBytes = 16 * HD;  // K (or V) of 16 tokens
+  constexpr int kBox = 16 * kPart;     // one TMA box
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+  uint4* qf = reinterpret_cast<uint4*>(smem + L::kRingBytes);  // [MT][kSteps][32]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  float* qexp = reinterpret_cast<float*>(smem + L::kRowInfo);  // [kRows]
+  int* qlim = reinterpret_cast<int*>(qexp + kRows);            // [kRows] last visible position
+  float* jm = reinterpret_cast<float*>(smem + L::kMl);         // [warps][kRows]
+  float* jl = jm + kAttWarps * kRows;
+  int* shared_int = reinterpret_cast<int*>(jl + kAttWarps * kRows);  // [4]
+  long long* shared_ll = reinterpret_cast<long long*>(shared_int + 4);  // [5]
+  float* joined = reinterpret_cast<float*>(smem);              // [warps][16][HD]
 
-  const int r = blockIdx.z, h = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
+  unsigned char* ring = smem + warp * kRing * L::kStage;
+  uint64_t* full = bars + warp * kRing;
+  if (lane == 0) {
+    for (int s = 0; s < kRing; ++s) mbar_init(full + s, 1);
+    fence_barrier_init();
+    prefetch_tensor_map(&kmap);
+    prefetch_tensor_map(&vmap);
+  }
   pdl_launch_dependents();
   pdl_wait_primary();
-  const int start = p.starts[r];
-  const int n = min(p.starts[r + 1], p.tokens) - start;
-  const int len = p.seq_lens[r];
-  const int rows = n * p.group;
-  const int row0 = blockIdx.x * kRows;
-  if (start < 0 || row0 >= rows) return;
 
-  // Q rows: power-of-two scale, fp16, in operand order.
-  for (int i = warp; i < kRows; i += kAttWarps) {
-    const int row = row0 + i;
-    const int qi = row / p.group, gq = row % p.group;
-    float v[HD / 32];
-    float most = 0.f;
+  // The schedule: every CTA adds up all requests' steps and finds its first.
+  const int most_len = p.table_width << p.block_shift;
+  auto rows_of = [&](int r) { return max(min(p.starts[r + 1], p.tokens) - max(p.starts[r], 0), 0) * p.group; };
+  auto steps_of = [&](int r) { return max(ceil_div(min(p.seq_lens[r], most_len), kStepTokens), 1); };
+  const int per = ceil_div(p.requests, kAttWarps * 32);
+  const int ra = min((int)threadIdx.x * per, p.requests), rb = min(ra + per, p.requests);
+  long long mine = 0;
+  for (int r = ra; r < rb; ++r) mine += (long long)ceil_div(rows_of(r), kRows) * p.kv_heads * steps_of(r);
+  long long upto = mine;
 #pragma unroll
-    for (int e = 0; e < HD / 32; ++e) {
-      const long long at = (long long)(start + qi) * p.q_token_stride +
-                           (long long)(h * p.group + gq) * p.q_head_stride + lane * (HD / 32) + e;
-      v[e] = row < rows ? load_q(p, at) : 0.f;
-      most = fmaxf(most, fabsf(v[e]));
-    }
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += x;
+  }
+  if (lane == 31) shared_ll[warp] = upto;
+  if (threadIdx.x == 0) shared_int[0] = -1;
+  __syncthreads();
+  long long all = 0, before = upto - mine;
 #pragma unroll
-    for (int m = 16; m > 0; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
-    int ex = (int)(__float_as_uint(most) >> 23) - 126;  // most < 2^ex
-    ex = isfinite(most) ? min(max(ex, -100), 100) : 0;
-    const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
-    if (lane == 0) {
-      qexp[i] = __uint_as_float((uint32_t)(127 + ex) << 23);
-      qlim[i] = row < rows ? len - n + qi : -1;
+  for (int w = 0; w < kAttWarps; ++w) {
+    if (w < warp) before += shared_ll[w];
+    all += shared_ll[w];
+  }
+  const long long C = min((long long)gridDim.x, all);  // every CTA in use has a step
+  if (blockIdx.x >= C) return;
+  long long s0 = all * blockIdx.x / C;
+  const long long s1 = all * (blockIdx.x + 1) / C;
+  if (before <= s0 && s0 < before + mine) {
+    int r = ra;
+    long long at = before;
+    for (; r < rb; ++r) {
+      const long long n = (long long)ceil_div(rows_of(r), kRows) * p.kv_heads * steps_of(r);
+      if (s0 < at + n) break;
+      at += n;
     }
-    // dim d: part, lane t = (d % kPart) / (2 kWords) ... see the layout above
-#pragma unroll
-    for (int e = 0; e < HD / 32; ++e) {
-      const int d = lane * (HD / 32) + e;
-      const int part = d / kPart, dd = d % kPart;
-      const int tt = dd / (4 * kWords), w = (dd / 4) % kWords, b = dd & 3;
-      const int step = part * kWords + w;
-      // a0: row g, k 2t,2t+1; a1: row g + 8; a2: row g, k 2t+8,2t+9; a3: row g + 8
-      const int reg = ((i & 15) >> 3) + 2 * (b >> 1);
-      const int ln = (i & 7) * 4 + tt;
-      reinterpret_cast<__half*>(qf + ((i >> 4) * kSteps + step) * 32 + ln)[reg * 2 + (b & 1)] =
-          __float2half_rn(v[e] * down);
-    }
+    shared_int[0] = r;
+    shared_ll[4] = at;
   }
   __syncthreads();
+  int r = shared_int[0];
+  long long request_at = shared_ll[4];  // first step of request r
+  uint32_t used = 0;                    // tiles that this warp's ring has delivered
+  bool dead = false;                    // a copy never arrived
 
-  float o[MT][kTiles][4];
-  float m[MT][2], l[MT][2], qe[MT][2];
-  int lim[MT][2];
-  int last = -1;
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-    for (int j = 0; j < kTiles; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.f;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      m[mt][x] = -INFINITY;
-      l[mt][x] = 0.f;
-      qe[mt][x] = qexp[mt * 16 + x * 8 + g];
-      lim[mt][x] = min(qlim[mt * 16 + x * 8 + g], len - 1);
+  while (s0 < s1) {
+    const int start = max(p.starts[r], 0);
+    const int n = max(min(p.starts[r + 1], p.tokens) - start, 0);
+    const int rows = n * p.group;
+    const int row_tiles = ceil_div(rows, kRows);
+    const int len = min(p.seq_lens[r], most_len);
+    if (len < p.seq_lens[r]) record_device_error(kDevErrBadIndex);
+    const int steps = max(ceil_div(len, kStepTokens), 1);
+    const long long request_steps = (long long)row_tiles * p.kv_heads * steps;
+    if (s0 >= request_at + request_steps) {
+      request_at += request_steps;
+      ++r;
+      continue;
     }
-  }
-  for (int i = 0; i < kRows; ++i) last = max(last, min(qlim[i], len - 1));
-  const int kv_len = last + 1;
-  const int bs_mask = (1 << p.block_shift) - 1;
+    const int item = (int)((s0 - request_at) / steps);
+    const int step = (int)((s0 - request_at) % steps);
+    const int step_end = (int)min((long long)steps, step + (s1 - s0));
+    const int h = item / row_tiles, row0 = (item % row_tiles) * kRows;
+    const long long item_at = request_at + (long long)item * steps;
+    const int first_lim = len - n + row0 / p.group;
+    const int kv_len = max(min(len, len - n + (min(rows, row0 + kRows) - 1) / p.group + 1), 0);
+    const int t0 = step * kStepTokens + warp * 32, t1 = min(kv_len, step_end * kStepTokens);
+    const int count = t0 < t1 ? (t1 - t0 + kStepTokens - 1) / kStepTokens : 0;  // this warp's tiles
 
-  for (int j0 = warp * 32; j0 < kv_len; j0 += kAttWarps * 32) {
-    size_t base[2];
-    float3 pc[2];
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const int pos = min(j0 + 16 * hh, (kv_len - 1) & ~15);
+    // Lane's half tile of a batch of 16 tiles: its row in the cache and constants.
+    auto half_row = [&](int i) {
+      const int pos = min(t0 + (i + (lane >> 1)) * kStepTokens + (lane & 1) * 16, (t1 - 1) & ~15);
       const int col = pos >> p.block_shift;
       int page = col < p.table_width ? p.table[(size_t)r * p.table_width + col] : -1;
       if ((unsigned)page >= (unsigned)p.num_blocks) {
         record_device_error(kDevErrBadIndex);
         page = 0;
       }
-      base[hh] = ((((size_t)page * p.kv_heads + h) << p.block_shift) + (pos & bs_mask)) * HD;
-      pc[hh] = page_constants(p, page, h, Code<F>::kLogFactor);
-    }
-    // scores of 32 tokens: 4 n8 tiles
-    float s[MT][4][4];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[mt][j][e] = 0.f;
-#pragma unroll
-    for (int part = 0; part < kParts; ++part) {
-      uint32_t kw[4][kWords];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint8_t* src = p.k_cache + base[j >> 1] + (size_t)((j & 1) * 8 + g) * HD + part * 128 + t * (4 * kWords);
-#pragma unroll
-        for (int w = 0; w < kWords; w += 4) {
-          const uint4 x = *reinterpret_cast<const uint4*>(src + 4 * w);
-          kw[j][w] = x.x; kw[j][w + 1] = x.y; kw[j][w + 2] = x.z; kw[j][w + 3] = x.w;
-        }
-      }
-#pragma unroll
-      for (int w = 0; w < kWords; ++w) {
-        uint4 a[MT];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) a[mt] = qf[(mt * kSteps + part * kWords + w) * 32 + lane];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t b0, b1;
-          Code<F>::unpack(kw[j][w], b0, b1);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) mma_16816(s[mt][j], a[mt], b0, b1);
-        }
-      }
-    }
-    // weights; s[.][j][2x + y]: row g + 8x, token 8 j + 2 t + y
-    uint4 pa[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      float top[2] = {m[mt][0], m[mt][1]};
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int x = e >> 1;
-          const int pos = j0 + 8 * j + 2 * t + (e & 1);
-          const float v = pos <= lim[mt][x] ? fmaf(s[mt][j][e], pc[j >> 1].x * qe[mt][x], pc[j >> 1].y) : -INFINITY;
-          s[mt][j][e] = v;
-          top[x] = fmaxf(top[x], v);
-        }
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
-        top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
-        const float ref = top[x] == -INFINITY ? 0.f : top[x];
-        const float fade = exp2_approx(m[mt][x] - ref);  // 0 while m is -inf
-        m[mt][x] = top[x];
-        l[mt][x] *= fade;
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j) {
-          o[mt][j][2 * x] *= fade;
-          o[mt][j][2 * x + 1] *= fade;
-        }
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          float sum = 0.f;
-#pragma unroll
-          for (int j = 2 * hh; j < 2 * hh + 2; ++j) {
-            s[mt][j][2 * x] = exp2_approx(s[mt][j][2 * x] - ref);
-            s[mt][j][2 * x + 1] = exp2_approx(s[mt][j][2 * x + 1] - ref);
-            sum += s[mt][j][2 * x] + s[mt][j][2 * x + 1];
-          }
-          l[mt][x] = fmaf(sum, pc[hh].z, l[mt][x]);
-        }
-      }
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        pa[mt][hh].x = h2_as_u32(__floats2half2_rn(s[mt][2 * hh][0], s[mt][2 * hh][1]));
-        pa[mt][hh].y = h2_as_u32(__floats2half2_rn(s[mt][2 * hh][2], s[mt][2 * hh][3]));
-        pa[mt][hh].z = h2_as_u32(__floats2half2_rn(s[mt][2 * hh + 1][0], s[mt][2 * hh + 1][1]));
-        pa[mt][hh].w = h2_as_u32(__floats2half2_rn(s[mt][2 * hh + 1][2], s[mt][2 * hh + 1][3]));
-      }
-    }
-    // output += weights x V
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh)
+      return make_int2(page, (int)((((long long)page * p.kv_heads + h) << p.block_shift) + (pos & ((1 << p.block_shift) - 1))));
+    };
+    auto issue = [&](int i, int row_lo, int row_hi) {  // lane 0: tile i's boxes
+      unsigned char* st = ring + ((used + i) % kRing) * L::kStage;
+      uint64_t* bar = full + (used + i) % kRing;
+      mbar_arrive_expect_tx(bar, L::kStage);
+      const uint64_t policy = row_tiles == 1 ? l2_policy_evict_first() : l2_policy_normal();
 #pragma unroll
       for (int part = 0; part < kParts; ++part) {
-        uint32_t vw[4][kVWords];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tok = 2 * t + (i & 1) + 8 * (i >> 1);
-          const uint8_t* src = p.v_cache + base[hh] + (size_t)tok * HD + part * 128 + g * (4 * kVWords);
-          if constexpr (kVWords == 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(src);
-            vw[i][0] = x.x; vw[i][1] = x.y; vw[i][2] = x.z; vw[i][3] = x.w;
-          } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(src);
-            vw[i][0] = x.x; vw[i][1] = x.y;
-          }
-        }
-#pragma unroll
-        for (int w = 0; w < kVWords; ++w) {
-          uint32_t b[4][2];  // [dim of the word][k half]
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t a01 = __byte_perm(vw[2 * i][w], vw[2 * i + 1][w], 0x5140);
-            const uint32_t a23 = __byte_perm(vw[2 * i][w], vw[2 * i + 1][w], 0x7362);
-            Code<F>::unpack(a01, b[0][i], b[1][i]);
-            Code<F>::unpack(a23, b[2][i], b[3][i]);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-              mma_16816(o[mt][part * (kPart / 8) + 4 * w + e], pa[mt][hh], b[e][0], b[e][1]);
-        }
+        tma_load_2d(st + part * kBox, &kmap, part * 128, row_lo, bar, policy);
+        tma_load_2d(st + kHalfBytes + part * kBox, &kmap, part * 128, row_hi, bar, policy);
+        tma_load_2d(st + 2 * kHalfBytes + part * kBox, &vmap, part * 128, row_lo, bar, policy);
+        tma_load_2d(st + 3 * kHalfBytes + part * kBox, &vmap, part * 128, row_hi, bar, policy);
       }
-  }
+    };
+    int2 cur = make_int2(0, 0), nxt = make_int2(0, 0);
+    if (count > 0) {
+      cur = half_row(0);
+#pragma unroll
+      for (int i = 0; i < kRing; ++i) {
+        const int lo = __shfl_sync(0xffffffffu, cur.y, 2 * i), hi = __shfl_sync(0xffffffffu, cur.y, 2 * i + 1);
+        if (lane == 0 && i < count && !dead) issue(i, lo, hi);
+      }
+    }
 
-  // Join the warps.  o[.][j][2x + y]: row g + 8x, dim of n = 2t + y in tile j.
+    // Q rows: power-of-two scale, fp16, in operand order.
+    constexpr int kMine = kRows / kAttWarps, kPairs = HD / 64;
+    uint32_t raw[kMine][kPairs];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+    for (int i = 0; i < kMine; ++i) {
+      const int row = row0 + warp + i * kAttWarps;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int row = mt * 16 + x * 8 + g;
-      float sum = l[mt][x];
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      if (t == 0) {
-        jm[warp * kRows + row] = m[mt][x];
-        jl[warp * kRows + row] = sum;
+      for (int e = 0; e < kPairs; ++e) raw[i][e] = 0;
+      if (row < rows)
+        load_q<kPairs>(p, (long long)(start + row / p.group) * p.q_token_stride +
+                              (long long)(h * p.group + row % p.group) * p.q_head_stride + lane * (HD / 32), raw[i]);
+    }
+#pragma unroll
+    for (int ii = 0; ii < kMine; ++ii) {
+      const int i = warp + ii * kAttWarps, row = row0 + i;
+      float v[HD / 32];
+      float most = 0.f;
+#pragma unroll
+      for (int e = 0; e < kPairs; ++e) {
+        const float2 x = unpack_q(p.bf16, raw[ii][e]);
+        v[2 * e] = x.x;
+        v[2 * e + 1] = x.y;
+        most = fmaxf(most, fmaxf(fabsf(x.x), fabsf(x.y)));
       }
+      most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+      int ex = (int)(__float_as_uint(most) >> 23) - 126;  // most < 2^ex
+      ex = isfinite(most) ? min(max(ex, -100), 100) : 0;
+      const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
+      if (lane == 0) {
+        qexp[i] = __uint_as_float((uint32_t)(127 + ex) << 23);
+        qlim[i] = row < rows ? len - n + row / p.group : kv_len - 1;  // rows past the end are not written
+      }
+#pragma unroll
+      for (int e = 0; e < HD / 32; e += 2) {
+        const int d = lane * (HD / 32) + e;
+        const int part = d / kPart, dd = d % kPart;
+        const int tt = dd / (4 * kWords), w = (dd / 4) % kWords, b = dd & 3;
+        // a0: row g, k 2t,2t+1; a1: row g + 8; a2: row g, k 2t+8,2t+9; a3: row g + 8
+        const int reg = ((i & 15) >> 3) + (b & 2);
+        const int ln = (i & 7) * 4 + tt;
+        reinterpret_cast<uint32_t*>(qf + ((i >> 4) * kSteps + part * kWords + w) * 32 + ln)[reg] =
+            h2_as_u32(__floats2half2_rn(v[e] * down, v[e + 1] * down));
+      }
+    }
+    float3 cc = make_float3(0.f, 0.f, 0.f), nc = cc;
+    if (count > 0) cc = page_constants(p, cur.x, h, Code<F>::kLogFactor);
+    __syncthreads();
+
+    float o[MT][kTiles][4];
+    float m[MT][2], l[MT][2], qe[MT][2];
+    int lim[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
       for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int part = j / (kPart / 8), jj = j % (kPart / 8);
-          joined[(warp * kRows + row) * HD + part * kPart + (2 * t + y) * (kPart / 8) + jj] = o[mt][j][2 * x + y];
+        for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.f;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        m[mt][x] = -INFINITY;
+        l[mt][x] = 0.f;
+        qe[mt][x] = qexp[mt * 16 + x * 8 + g];
+        lim[mt][x] = min(qlim[mt * 16 + x * 8 + g], t1 - 1);
+      }
+    }
+
+    for (int i = 0; i < count; ++i) {
+      const int j0 = t0 + i * kStepTokens;
+      const int u = i & 15;
+      if (u == 0 && i > 0) {
+        cur = nxt;
+        cc = nc;
+      }
+      if (u == 0 && i + 16 < count) nxt = half_row(i + 16);
+      if (u == 8 && i + 8 < count) nc = page_constants(p, nxt.x, h, Code<F>::kLogFactor);
+      float3 pc[2];
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+        pc[hh] = make_float3(__shfl_sync(0xffffffffu, cc.x, 2 * u + hh), __shfl_sync(0xffffffffu, cc.y, 2 * u + hh),
+                             __shfl_sync(0xffffffffu, cc.z, 2 * u + hh));
+      const uint32_t stage = (used + i) % kRing;
+      const uint32_t kb = smem_addr(ring + stage * L::kStage), vb = kb + 2 * kHalfBytes;
+      if (!dead && !mbar_wait(full + stage, ((used + i) / kRing) & 1)) {
+        record_device_error(kDevErrBarrierTimeout);
+        dead = true;
+      }
+      dead = __any_sync(0xffffffffu, dead);
+
+      // scores of 32 tokens: 4 n8 tiles
+      float s[MT][4][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[mt][j][e] = 0.f;
+#pragma unroll
+      for (int part = 0; part < kParts; ++part) {
+        uint32_t kw[4][kWords];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t row = kb + (j >> 1) * kHalfBytes + part * kBox + ((j & 1) * 8 + g) * kPart;
+          if constexpr (kWords == 8) {
+            const uint4 x = lds128(row + (((2 * t) ^ g) << 4)), y = lds128(row + (((2 * t + 1) ^ g) << 4));
+            kw[j][0] = x.x; kw[j][1] = x.y; kw[j][2] = x.z; kw[j][3] = x.w;
+            kw[j][4] = y.x; kw[j][5] = y.y; kw[j][6] = y.z; kw[j][7] = y.w;
+          } else {
+            const uint4 x = lds128(row + ((t ^ (g >> 1)) << 4));
+            kw[j][0] = x.x; kw[j][1] = x.y; kw[j][2] = x.z; kw[j][3] = x.w;
+          }
         }
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+          uint4 a[MT];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) a[mt] = qf[(mt * kSteps + part * kWords + w) * 32 + lane];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t b0, b1;
+            Code<F>::unpack(kw[j][w], b0, b1);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) mma_16816(s[mt][j], a[mt], b0, b1);
+          }
+        }
+      }
+      // weights; s[.][j][2x + y]: row g + 8x, token 8 j + 2 t + y
+      const bool cut = j0 + 31 > min(first_lim, t1 - 1);
+      uint4 pa[MT][2];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        float top[2] = {m[mt][0], m[mt][1]};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int x = e >> 1;
+            float v = fmaf(s[mt][j][e], pc[j >> 1].x * qe[mt][x], pc[j >> 1].y);
+            if (cut && j0 + 8 * j + 2 * t + (e & 1) > lim[mt][x]) v = -INFINITY;
+            s[mt][j][e] = v;
+            top[x] = fmaxf(top[x], v);
+          }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
+          top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
+        }
+        if (__any_sync(0xffffffffu, top[0] > m[mt][0] || top[1] > m[mt][1])) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float fade = m[mt][x] == -INFINITY ? 0.f : exp2_approx(m[mt][x] - top[x]);
+            m[mt][x] = top[x];
+            l[mt][x] *= fade;
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) {
+              o[mt][j][2 * x] *= fade;
+              o[mt][j][2 * x + 1] *= fade;
+            }
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float ref = m[mt][x] == -INFINITY ? 0.f : m[mt][x];
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 2 * hh; j < 2 * hh + 2; ++j) {
+              s[mt][j][2 * x] = exp2_approx(s[mt][j][2 * x] - ref);
+              s[mt][j][2 * x + 1] = exp2_approx(s[mt][j][2 * x + 1] - ref);
+              sum += s[mt][j][2 * x] + s[mt][j][2 * x + 1];
+            }
+            l[mt][x] = fmaf(sum, pc[hh].z, l[mt][x]);
+          }
+        }
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          pa[mt][hh].x = h2_as_u32(__floats2half2_rn(s[mt][2 * hh][0], s[mt][2 * hh][1]));
+          pa[mt][hh].y = h2_as_u32(__floats2half2_rn(s[mt][2 * hh][2], s[mt][2 * hh][3]));
+          pa[mt][hh].z = h2_as_u32(__floats2half2_rn(s[mt][2 * hh + 1][0], s[mt][2 * hh + 1][1]));
+          pa[mt][hh].w = h2_as_u32(__floats2half2_rn(s[mt][2 * hh + 1][2], s[mt][2 * hh + 1][3]));
+        }
+      }
+      // output += weights x V
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+          uint32_t vw[4][kVWords];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int tok = 2 * t + (c & 1) + 8 * (c >> 1);
+            const uint32_t row = vb + hh * kHalfBytes + part * kBox + tok * kPart;
+            if constexpr (kVWords == 4) {
+              const uint4 x = lds128(row + ((g ^ (tok & 7)) << 4));
+              vw[c][0] = x.x; vw[c][1] = x.y; vw[c][2] = x.z; vw[c][3] = x.w;
+            } else {
+              const uint32_t at = row + (((g >> 1) ^ ((tok >> 1) & 3)) << 4) + (g & 1) * 8;
+              vw[c][0] = lds32(at);
+              vw[c][1] = lds32(at + 4);
+            }
+          }
+#pragma unroll
+          for (int w = 0; w < kVWords; ++w) {
+            uint32_t b[4][2];  // [dim of the word][k half]
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t a01 = __byte_perm(vw[2 * c][w], vw[2 * c + 1][w], 0x5140);
+              const uint32_t a23 = __byte_perm(vw[2 * c][w], vw[2 * c + 1][w], 0x7362);
+              Code<F>::unpack(a01, b[0][c], b[1][c]);
+              Code<F>::unpack(a23, b[2][c], b[3][c]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt)
+                mma_16816(o[mt][part * (kPart / 8) + 4 * w + e], pa[mt][hh], b[e][0], b[e][1]);
+          }
+        }
+      // the stage is free: fetch tile i + kRing into it
+      const int v2 = (u + kRing) & 15;
+      const int src = u + kRing < 16 ? cur.y : nxt.y;
+      const int lo = __shfl_sync(0xffffffffu, src, 2 * v2), hi = __shfl_sync(0xffffffffu, src, 2 * v2 + 1);
+      if (lane == 0 && i + kRing < count && !dead) {
+        fence_proxy_async_smem();
+        issue(i + kRing, lo, hi);
+      }
+      __syncwarp();
     }
-  __syncthreads();
-  for (int i = threadIdx.x; i < kRows * HD; i += kAttWarps * 32) {
-    const int row = i / HD, d = i % HD;
-    if (row0 + row >= rows) break;
-    float top = -INFINITY;
-    for (int w = 0; w < kAttWarps; ++w) top = fmaxf(top, jm[w * kRows + row]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float num = 0.f, den = 0.f;
-    for (int w = 0; w < kAttWarps; ++w) {
-      const float f = exp2_approx(jm[w * kRows + row] - ref);
-      num = fmaf(joined[(w * kRows + row) * HD + d], f, num);
-      den = fmaf(jl[w * kRows + row], f, den);
+    used += count;
+
+    // Join the warps, an m tile at a time, in the ring's memory (it is empty now).
+    // o[.][j][2x + y]: row g + 8x, dim of n = 2t + y in tile j.
+    const bool whole = step == 0 && step_end == steps;
+    const int slot = (int)blockIdx.x * 2 + (s0 == item_at ? 1 : 0);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int row = x * 8 + g;
+        float sum = l[mt][x];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (t == 0) {
+          jm[warp * kRows + mt * 16 + row] = m[mt][x];
+          jl[warp * kRows + mt * 16 + row] = sum;
+        }
+        if (row0 + mt * 16 + row < rows) {
+#pragma unroll
+          for (int part = 0; part < kParts; ++part)
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+              for (int j = 0; j < kPart / 8; j += 4) {
+                float* dst = joined + (warp * 16 + row) * HD + part * kPart + (2 * t + y) * (kPart / 8) + j;
+                const int jj = part * (kPart / 8) + j;
+                *reinterpret_cast<float4*>(dst) = make_float4(o[mt][jj][2 * x + y], o[mt][jj + 1][2 * x + y],
+                                                              o[mt][jj + 2][2 * x + y], o[mt][jj + 3][2 * x + y]);
+              }
+        }
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < 16 * HD / 4; i += kAttWarps * 32) {
+        const int row = i / (HD / 4), d = (i % (HD / 4)) * 4;
+        const int tr = mt * 16 + row;
+        if (row0 + tr >= rows) break;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kAttWarps; ++w) top = fmaxf(top, jm[w * kRows + tr]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
+#pragma unroll
+        for (int w = 0; w < kAttWarps; ++w) {
+          const float f = exp2_approx(jm[w * kRows + tr] - ref);
+          const float4 x = *reinterpret_cast<const float4*>(joined + (w * 16 + row) * HD + d);
+          num[0] = fmaf(x.x, f, num[0]);
+          num[1] = fmaf(x.y, f, num[1]);
+          num[2] = fmaf(x.z, f, num[2]);
+          num[3] = fmaf(x.w, f, num[3]);
+          den = fmaf(jl[w * kRows + tr], f, den);
+        }
+        if (whole) {
+          store_out(p, start, h, row0 + tr, d, num, den);
+        } else {
+          float* part = parts + (size_t)slot * kRows * (HD + 2);
+          *reinterpret_cast<float4*>(part + (size_t)tr * HD + d) = make_float4(num[0], num[1], num[2], num[3]);
+          if (d == 0) *reinterpret_cast<float2*>(part + kRows * HD + 2 * tr) = make_float2(top, den);
+        }
+      }
     }
-    const float v = den == 0.f ? 0.f : num / den;
-    const int qi = (row0 + row) / p.group, gq = (row0 + row) % p.group;
-    const long long at = (long long)(start + qi) * p.out_token_stride +
-                         (long long)(h * p.group + gq) * p.out_head_stride + d;
-    if (p.bf16)
-      static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-    else
-      static_cast<__half*>(p.out)[at] = __float2half_rn(v);
+    if (!whole) {
+      // the CTAs that hold the item's first and last step
+      const int c0 = (int)(((item_at + 1) * C - 1) / all), c1 = (int)(((item_at + steps) * C - 1) / all);
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) shared_int[1] = atomicAdd(counters + c0, 1) == c1 - c0;
+      __syncthreads();
+      if (shared_int[1]) {
+        __threadfence();
+        const int live = min(rows - row0, kRows);
+        for (int i = threadIdx.x; i < live * (HD / 4); i += kAttWarps * 32) {
+          const int tr = i / (HD / 4), d = (i % (HD / 4)) * 4;
+          float top = -INFINITY;
+          for (int c = c0; c <= c1; ++c) {
+            const float* part = parts + (size_t)(2 * c + (c == c0)) * kRows * (HD + 2);
+            top = fmaxf(top, __ldcg(part + kRows * HD + 2 * tr));
+          }
+          const float ref = top == -INFINITY ? 0.f : top;
+          float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
+          for (int c = c0; c <= c1; ++c) {
+            const float* part = parts + (size_t)(2 * c + (c == c0)) * kRows * (HD + 2);
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + kRows * HD + 2 * tr));
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(part + (size_t)tr * HD + d));
+            const float f = exp2_approx(ml.x - ref);
+            num[0] = fmaf(x.x, f, num[0]);
+            num[1] = fmaf(x.y, f, num[1]);
+            num[2] = fmaf(x.z, f, num[2]);
+            num[3] = fmaf(x.w, f, num[3]);
+            den = fmaf(ml.y, f, den);
+          }
+          store_out(p, start, h, row0 + tr, d, num, den);
+        }
+        if (threadIdx.x == 0) counters[c0] = 0;
+      }
+    }
+    fence_proxy_async_smem();  // the ring's memory goes back to the copies
+    __syncthreads();
+    s0 += step_end - step;
   }
 }
 
-template <int HD, int F>
-int launch_attend(AttendArgs& a, int max_query_len, const DeviceInfo& dev, cudaStream_t stream) {
-  const long long rows = (long long)max_query_len * a.group;
-  constexpr int kBig = HD == 256 ? 1 : 2;
-  const bool big = rows > 16 && kBig == 2;
-  const int mt = big ? 2 : 1;
-  const int kr = 16 * mt;
-  const size_t smem = (size_t)mt * (HD / 16) * 512 + kr * 8 + (size_t)kAttWarps * kr * (HD + 2) * 4;
-  auto kernel = big ? attend_simple_kernel<HD, F, kBig> : attend_simple_kernel<HD, F, 1>;
-  cudaError_t e = ensure_smem(kernel, (int)smem, dev.ordinal);
+constexpr int kStreamPerSm = 3;  // CTAs per SM that the grid is sized for (2 where shared memory allows no more)
+
+template <int HD, int MT>
+constexpr int stream_per_sm() {
+  return StreamLayout<HD, MT>::kTotal <= 75 * 1024 ? kStreamPerSm : StreamLayout<HD, MT>::kTotal <= 113 * 1024 ? 2 : 1;
+}
+
+// One counter per CTA, then partial sums of two items per CTA.  The counters
+// are where they are for every variant, since they must stay zero between calls.
+constexpr size_t kCounterBytes = 16384;
+
+template <int HD, int MT>
+size_t stream_workspace(int sms) {
+  return kCounterBytes + (size_t)sms * stream_per_sm<HD, MT>() * 2 * (16 * MT) * (HD + 2) * 4;
+}
+
+struct CacheMapKey {
+  uintptr_t ptr;
+  long long rows;
+  int dim;
+  bool operator==(const CacheMapKey& o) const { return ptr == o.ptr && rows == o.rows && dim == o.dim; }
+};
+struct CacheMapHash {
+  size_t operator()(const CacheMapKey& k) const {
+    return std::hash<uintptr_t>()(k.ptr) ^ ((size_t)k.rows << 8) ^ (size_t)k.dim;
+  }
+};
+std::mutex g_cache_map_mutex;
+std::unordered_map<CacheMapKey, CUtensorMap, CacheMapHash> g_cache_maps[kMaxDevices];
+constexpr size_t kMaxCacheMaps = 4096;
+
+// The cache as a 2-D tensor of bytes [blocks * kv_heads * block_size][dim]; one
+// box is 16 tokens of one head (a 128-dim part of them), swizzled.  A map only
+// describes addresses, so it is looked up by them.
+int cache_map(const DeviceInfo& dev, const void* cache, long long rows, int dim, CUtensorMap* out) {
+  const CacheMapKey key{reinterpret_cast<uintptr_t>(cache), rows, dim};
+  {
+    std::lock_guard<std::mutex> lock(g_cache_map_mutex);
+    auto it = g_cache_maps[dev.ordinal].find(key);
+    if (it != g_cache_maps[dev.ordinal].end()) {
+      *out = it->second;
+      return GDSQ_OK;
+    }
+  }
+  PFN_cuTensorMapEncodeTiled_v12000 encode;
+  int st = get_encoder(&encode);
+  if (st != GDSQ_OK) return st;
+  CUtensorMap map;
+  const cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)dim};
+  const cuuint32_t box[2] = {(cuuint32_t)std::min(dim, 128), 16};
+  const cuuint32_t estr[2] = {1, 1};
+  CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(cache), dims, strides, box, estr,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(GDSQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for a cache of %lld x %d bytes", (int)r, rows, dim);
+  std::lock_guard<std::mutex> lock(g_cache_map_mutex);
+  if (g_cache_maps[dev.ordinal].size() >= kMaxCacheMaps) g_cache_maps[dev.ordinal].clear();
+  g_cache_maps[dev.ordinal][key] = map;
+  *out = map;
+  return GDSQ_OK;
+}
+
+template <int HD, int F, int MT>
+int launch_stream(const AttendArgs& a, const DeviceInfo& dev, void* workspace, size_t bytes, cudaStream_t stream) {
+  const size_t need = stream_workspace<HD, MT>(dev.sms);
+  if (bytes < need)
+    return fail(GDSQ_ERR_INVALID_VALUE, "attend_kv8: workspace of %zu bytes, %zu needed", bytes, need);
+  const long long rows = ((long long)a.num_blocks * a.kv_heads) << a.block_shift;
+  CUtensorMap kmap, vmap;
+  int st = cache_map(dev, a.k_cache, rows, HD, &kmap);
+  if (st == GDSQ_OK) st = cache_map(dev, a.v_cache, rows, HD, &vmap);
+  if (st != GDSQ_OK) return st;
+  auto kernel = attend_stream_kernel<HD, F, MT>;
+  constexpr int smem = StreamLayout<HD, MT>::kTotal;
+  cudaError_t e = ensure_smem(kernel, smem, dev.ordinal);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(attend)");
-  const dim3 grid((unsigned)((rows + kr - 1) / kr), a.kv_heads, a.requests);
-  e = launch(kernel, grid, dim3(kAttWarps * 32), smem, stream, g_pdl_enabled != 0, a);
+  const int ctas = dev.sms * stream_per_sm<HD, MT>();
+  if ((size_t)ctas * sizeof(int) > kCounterBytes) return fail(GDSQ_ERR_UNSUPPORTED, "attend_kv8: %d SMs", dev.sms);
+  int* counters = static_cast<int*>(workspace);
+  float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
+  e = launch(kernel, dim3(ctas), dim3(kAttWarps * 32), smem, stream, g_pdl_enabled != 0, a, kmap, vmap, parts, counters);
   return e == cudaSuccess ? GDSQ_OK : cuda_fail(e, "attend launch");
+}
+
+template <int HD, int F>
+int launch_attend(const AttendArgs& a, int max_query_len, const DeviceInfo& dev, void* workspace, size_t bytes,
+                  cudaStream_t stream) {
+  if constexpr (HD != 256)
+    if ((long long)max_query_len * a.group > 16) return launch_stream<HD, F, 2>(a, dev, workspace, bytes, stream);
+  return launch_stream<HD, F, 1>(a, dev, workspace, bytes, stream);
 }
 
 }  // namespace
@@ -436,8 +791,13 @@ using namespace gdsq;
 
 extern "C" size_t gdsq_attend_kv8_workspace(int num_requests, int max_query_len, int num_heads, int num_kv_heads,
                                             int head_dim) {
-  (void)num_requests; (void)max_query_len; (void)num_heads; (void)num_kv_heads; (void)head_dim;
-  return 0;
+  if (num_requests <= 0 || max_query_len <= 0 || num_heads <= 0 || num_kv_heads <= 0) return 0;
+  const DeviceInfo* dev = nullptr;
+  if (device_info(&dev) != GDSQ_OK) return 0;
+  const bool few = (long long)max_query_len * (num_heads / num_kv_heads) <= 16;
+  if (head_dim == 64) return few ? stream_workspace<64, 1>(dev->sms) : stream_workspace<64, 2>(dev->sms);
+  if (head_dim == 128) return few ? stream_workspace<128, 1>(dev->sms) : stream_workspace<128, 2>(dev->sms);
+  return stream_workspace<256, 1>(dev->sms);
 }
 
 extern "C" int gdsq_attend_kv8(const void* q, int elem_type, long long q_token_stride, long long q_head_stride,
@@ -472,8 +832,11 @@ extern "C" int gdsq_attend_kv8(const void* q, int elem_type, long long q_token_s
   if (!aligned(k_cache, 128) || !aligned(v_cache, 128) || !aligned(k_scale, 4) || !aligned(v_scale, 4) ||
       !aligned(block_table, 4) || !aligned(seq_lens, 4) || !aligned(query_starts, 4))
     return fail(GDSQ_ERR_MISALIGNED, "attend_kv8: caches 128-byte, scales, table and lengths 4-byte alignment");
-  (void)workspace;
-  (void)workspace_bytes;
+  if (!workspace || !aligned(workspace, 16))
+    return fail(GDSQ_ERR_MISALIGNED, "attend_kv8: a 16-byte aligned workspace is needed");
+  if ((((long long)num_blocks * num_kv_heads * block_size) >> 31) != 0 || num_blocks < 1)
+    return fail(GDSQ_ERR_UNSUPPORTED, "attend_kv8: %d blocks of %d heads x %d tokens, not 1 to 2^31 - 1 rows", num_blocks,
+                num_kv_heads, block_size);
   const DeviceInfo* dev = nullptr;
   int st = device_info(&dev);
   if (st != GDSQ_OK) return st;
@@ -503,11 +866,11 @@ extern "C" int gdsq_attend_kv8(const void* q, int elem_type, long long q_token_s
   a.scale = softmax_scale * kLog2e * factor;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   if (cache_type == GDSQ_CACHE_INT8) {
-    if (head_dim == 64) return launch_attend<64, GDSQ_CACHE_INT8>(a, max_query_len, *dev, stream);
-    if (head_dim == 128) return launch_attend<128, GDSQ_CACHE_INT8>(a, max_query_len, *dev, stream);
-    return launch_attend<256, GDSQ_CACHE_INT8>(a, max_query_len, *dev, stream);
+    if (head_dim == 64) return launch_attend<64, GDSQ_CACHE_INT8>(a, max_query_len, *dev, workspace, workspace_bytes, stream);
+    if (head_dim == 128) return launch_attend<128, GDSQ_CACHE_INT8>(a, max_query_len, *dev, workspace, workspace_bytes, stream);
+    return launch_attend<256, GDSQ_CACHE_INT8>(a, max_query_len, *dev, workspace, workspace_bytes, stream);
   }
-  if (head_dim == 64) return launch_attend<64, GDSQ_CACHE_E4M3>(a, max_query_len, *dev, stream);
-  if (head_dim == 128) return launch_attend<128, GDSQ_CACHE_E4M3>(a, max_query_len, *dev, stream);
-  return launch_attend<256, GDSQ_CACHE_E4M3>(a, max_query_len, *dev, stream);
+  if (head_dim == 64) return launch_attend<64, GDSQ_CACHE_E4M3>(a, max_query_len, *dev, workspace, workspace_bytes, stream);
+  if (head_dim == 128) return launch_attend<128, GDSQ_CACHE_E4M3>(a, max_query_len, *dev, workspace, workspace_bytes, stream);
+  return launch_attend<256, GDSQ_CACHE_E4M3>(a, max_query_len, *dev, workspace, workspace_bytes, stream);
 }
