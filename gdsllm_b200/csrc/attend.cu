@@ -43,6 +43,7 @@ namespace {
 
 constexpr int kAttWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoMax = -1e30f;       // the running maximum before any score
 constexpr float kMaxLogScale = 100.f;  // |log2| of a value scale is held to this
 
 struct AttendArgs {
@@ -70,6 +71,13 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint4& a, uint32_
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+// Lane (g, t) holds elements (g, 2t), (g, 2t + 1) of an 8 x 8 matrix and gets (2t, g), (2t + 1, g).
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -171,7 +179,7 @@ __device__ __forceinline__ float3 page_constants(const AttendArgs& p, int page, 
 // Few rows per (request, KV head): single tokens, drafts, short chunks.
 //
 // Bound by reading the cache, so the work is cut by cache tokens, evenly: an
-// item is (request, KV head, tile of 16 * MT rows), its steps are 128 tokens
+// item is (request, KV head, tile of 8 * NT rows), its steps are 128 tokens
 // each, and CTA c of C takes the steps [c S / C, (c + 1) S / C) of all items in
 // order.  An item that ends in the CTA it began in is written out; the others
 // leave partial sums, and the CTA that arrives last at an item's counter adds
@@ -182,49 +190,60 @@ __device__ __forceinline__ float3 page_constants(const AttendArgs& p, int page, 
 // TMA boxes of 16 tokens (one block holds at least 16).  A lane looks up the
 // block, scales and constants of one half tile for 16 tiles at a time.
 //
-// Matrix operand layout: in m16n8k16 a lane (g = lane / 4, t = lane % 4) feeds
-// B[k = 2t, 2t+1, 2t+8, 2t+9][n = g].  The order of the summed index is free,
-// so for the scores (k = dim, n = token) lane t takes 32 consecutive dims of
-// token g: two 16-byte loads.  For the output (k = token, n = dim) lane g
-// takes 16 consecutive dims of tokens 2t, 2t+1, 2t+8, 2t+9.  With the 128-byte
-// TMA swizzle both are free of bank conflicts.
+// The products are taken transposed, tokens (scores) and dims (output) as the
+// 16 rows of m16n8k16 and 8 query rows as its columns, so that eight queries
+// of a group waste nothing.  A lane (g = lane / 4, t = lane % 4) feeds A[rows
+// g, g + 8][k = 2t, 2t+1, 2t+8, 2t+9].  The order of the summed index is free:
+// for the scores lane t takes 32 consecutive dims of tokens g and g + 8, two
+// 16-byte loads each; for the output lane g takes 16 consecutive dims of
+// tokens 2t, 2t+1, 2t+8, 2t+9.  With the 128-byte TMA swizzle both are free of
+// bank conflicts.  The weights come out as [token][query] and are fed back as
+// [query][token], one 8 x 8 transpose per 8 tokens.
 
 constexpr int kStepTokens = kAttWarps * 32;
 constexpr int kRing = 2;  // stages per warp
 
-template <int HD, int MT>
+template <int HD, int NT>
 struct StreamLayout {
   static constexpr int kStage = 2 * 32 * HD;  // K and V of 32 tokens
   static constexpr int kRingBytes = kAttWarps * kRing * kStage;
-  static constexpr int kRows = 16 * MT;
-  static constexpr int kJoin = kAttWarps * 16 * HD * 4;  // one m tile of every warp, in the ring's memory
-  static constexpr int kQ = MT * (HD / 16) * 512;
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kPitch = HD + 4;  // floats of a row in the join: eight rows of every warp, in the ring's memory
+  static constexpr int kQ = NT * (HD / 16) * 256;
   static constexpr int kBars = kRingBytes + kQ;
   static constexpr int kRowInfo = kBars + 128;
   static constexpr int kMl = kRowInfo + kRows * 8;                 // [warps][kRows] m, l
   static constexpr int kTotal = kMl + kAttWarps * kRows * 8 + 64 + 1024;  // + alignment
-  static_assert(kJoin <= kRingBytes, "the join uses the ring's memory");
+  static_assert(kAttWarps * 8 * kPitch * 4 <= kRingBytes, "the join uses the ring's memory");
 };
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-template <int HD, int F, int MT>
-__global__ void __launch_bounds__(kAttWarps * 32)
+// CTAs per SM that registers and shared memory allow, which the grid is sized for.
+template <int HD, int NT>
+constexpr int stream_per_sm() {
+  constexpr int by_smem = 227 * 1024 / (StreamLayout<HD, NT>::kTotal + 1024);
+  constexpr int by_regs = HD * NT <= 256 ? 3 : 2;
+  return by_smem < by_regs ? by_smem : by_regs;
+}
+
+template <int HD, int F, int NT>
+__global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
     attend_stream_kernel(const AttendArgs p, const __grid_constant__ CUtensorMap kmap,
                          const __grid_constant__ CUtensorMap vmap, float* parts, int* counters) {
-  using L = StreamLayout<HD, MT>;
+  using L = StreamLayout<HD, NT>;
   constexpr int kParts = HD >= 128 ? HD / 128 : 1;  // 128-dim parts
   constexpr int kPart = HD >= 128 ? 128 : 64;
   constexpr int kWords = kPart / 16;   // 32-bit words of K per lane, token and part (= k16 steps)
   constexpr int kSteps = HD / 16;      // k16 steps of the scores
-  constexpr int kTiles = HD / 8;       // n8 tiles of the output
+  constexpr int kTiles = HD / 16;      // m16 tiles of the output
   constexpr int kVWords = kPart / 32;  // 32-bit words of V per lane, token and part
   constexpr int kRows = L::kRows;
   constexpr int kHalfBytes = 16 * HD;  // K (or V) of 16 tokens
   constexpr int kBox = 16 * kPart;     // one TMA box
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
-  uint4* qf = reinterpret_cast<uint4*>(smem + L::kRingBytes);  // [MT][kSteps][32]
+  uint4* qf = reinterpret_cast<uint4*>(smem + L::kRingBytes);  // [NT][kSteps / 2][32]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
   float* qexp = reinterpret_cast<float*>(smem + L::kRowInfo);  // [kRows]
   int* qlim = reinterpret_cast<int*>(qexp + kRows);            // [kRows] last visible position
@@ -232,7 +251,7 @@ __global__ void __launch_bounds__(kAttWarps * 32)
   float* jl = jm + kAttWarps * kRows;
   int* shared_int = reinterpret_cast<int*>(jl + kAttWarps * kRows);  // [4]
   long long* shared_ll = reinterpret_cast<long long*>(shared_int + 4);  // [5]
-  float* joined = reinterpret_cast<float*>(smem);              // [warps][16][HD]
+  float* joined = reinterpret_cast<float*>(smem);              // [warps][8][kPitch]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -386,10 +405,10 @@ __global__ void __launch_bounds__(kAttWarps * 32)
         const int d = lane * (HD / 32) + e;
         const int part = d / kPart, dd = d % kPart;
         const int tt = dd / (4 * kWords), w = (dd / 4) % kWords, b = dd & 3;
-        // a0: row g, k 2t,2t+1; a1: row g + 8; a2: row g, k 2t+8,2t+9; a3: row g + 8
-        const int reg = ((i & 15) >> 3) + (b & 2);
+        // b0: dims 0,1 of the word, b1: dims 2,3; two steps side by side
+        const int reg = (w & 1) * 2 + (b >> 1);
         const int ln = (i & 7) * 4 + tt;
-        reinterpret_cast<uint32_t*>(qf + ((i >> 4) * kSteps + part * kWords + w) * 32 + ln)[reg] =
+        reinterpret_cast<uint32_t*>(qf + (((i >> 3) * kSteps + part * kWords + w) >> 1) * 32 + ln)[reg] =
             h2_as_u32(__floats2half2_rn(v[e] * down, v[e + 1] * down));
       }
     }
@@ -397,23 +416,24 @@ __global__ void __launch_bounds__(kAttWarps * 32)
     if (count > 0) cc = page_constants(p, cur.x, h, Code<F>::kLogFactor);
     __syncthreads();
 
-    float o[MT][kTiles][4];
-    float m[MT][2], l[MT][2], qe[MT][2];
-    int lim[MT][2];
+    float o[kTiles][NT][4];
+    float m[NT][2], l[NT][2], qe[NT][2];  // of rows 8 nt + 2 t + y
+    int lim[NT][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+    for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-      for (int j = 0; j < kTiles; ++j)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.f;
+        for (int e = 0; e < 4; ++e) o[j][nt][e] = 0.f;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        m[mt][x] = -INFINITY;
-        l[mt][x] = 0.f;
-        qe[mt][x] = qexp[mt * 16 + x * 8 + g];
-        lim[mt][x] = min(qlim[mt * 16 + x * 8 + g], t1 - 1);
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        m[nt][y] = kNoMax;
+        l[nt][y] = 0.f;
+        qe[nt][y] = qexp[nt * 8 + 2 * t + y];
+        lim[nt][y] = min(qlim[nt * 8 + 2 * t + y], t1 - 1);
       }
-    }
 
     for (int i = 0; i < count; ++i) {
       const int j0 = t0 + i * kStepTokens;
@@ -437,101 +457,121 @@ __global__ void __launch_bounds__(kAttWarps * 32)
       }
       dead = __any_sync(0xffffffffu, dead);
 
-      // scores of 32 tokens: 4 n8 tiles
-      float s[MT][4][4];
+      // scores; s[hh][nt][2 x + y]: token 16 hh + 8 x + g, row 8 nt + 2 t + y
+      float s[2][NT][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[mt][j][e] = 0.f;
+          for (int e = 0; e < 4; ++e) s[hh][nt][e] = 0.f;
 #pragma unroll
-      for (int part = 0; part < kParts; ++part) {
-        uint32_t kw[4][kWords];
+      for (int part = 0; part < kParts; ++part)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t row = kb + (j >> 1) * kHalfBytes + part * kBox + ((j & 1) * 8 + g) * kPart;
-          if constexpr (kWords == 8) {
-            const uint4 x = lds128(row + (((2 * t) ^ g) << 4)), y = lds128(row + (((2 * t + 1) ^ g) << 4));
-            kw[j][0] = x.x; kw[j][1] = x.y; kw[j][2] = x.z; kw[j][3] = x.w;
-            kw[j][4] = y.x; kw[j][5] = y.y; kw[j][6] = y.z; kw[j][7] = y.w;
-          } else {
-            const uint4 x = lds128(row + ((t ^ (g >> 1)) << 4));
-            kw[j][0] = x.x; kw[j][1] = x.y; kw[j][2] = x.z; kw[j][3] = x.w;
-          }
-        }
-#pragma unroll
-        for (int w = 0; w < kWords; ++w) {
-          uint4 a[MT];
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) a[mt] = qf[(mt * kSteps + part * kWords + w) * 32 + lane];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t b0, b1;
-            Code<F>::unpack(kw[j][w], b0, b1);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) mma_16816(s[mt][j], a[mt], b0, b1);
-          }
-        }
-      }
-      // weights; s[.][j][2x + y]: row g + 8x, token 8 j + 2 t + y
-      const bool cut = j0 + 31 > min(first_lim, t1 - 1);
-      uint4 pa[MT][2];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        float top[2] = {m[mt][0], m[mt][1]};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int x = e >> 1;
-            float v = fmaf(s[mt][j][e], pc[j >> 1].x * qe[mt][x], pc[j >> 1].y);
-            if (cut && j0 + 8 * j + 2 * t + (e & 1) > lim[mt][x]) v = -INFINITY;
-            s[mt][j][e] = v;
-            top[x] = fmaxf(top[x], v);
-          }
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
-          top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
-        }
-        if (__any_sync(0xffffffffu, top[0] > m[mt][0] || top[1] > m[mt][1])) {
+        for (int hh = 0; hh < 2; ++hh) {
+          uint32_t kw[2][kWords];
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const float fade = m[mt][x] == -INFINITY ? 0.f : exp2_approx(m[mt][x] - top[x]);
-            m[mt][x] = top[x];
-            l[mt][x] *= fade;
+            const uint32_t row = kb + hh * kHalfBytes + part * kBox + (x * 8 + g) * kPart;
+            if constexpr (kWords == 8) {
+              const uint4 a = lds128(row + (((2 * t) ^ g) << 4)), b = lds128(row + (((2 * t + 1) ^ g) << 4));
+              kw[x][0] = a.x; kw[x][1] = a.y; kw[x][2] = a.z; kw[x][3] = a.w;
+              kw[x][4] = b.x; kw[x][5] = b.y; kw[x][6] = b.z; kw[x][7] = b.w;
+            } else {
+              const uint4 a = lds128(row + ((t ^ (g >> 1)) << 4));
+              kw[x][0] = a.x; kw[x][1] = a.y; kw[x][2] = a.z; kw[x][3] = a.w;
+            }
+          }
 #pragma unroll
-            for (int j = 0; j < kTiles; ++j) {
-              o[mt][j][2 * x] *= fade;
-              o[mt][j][2 * x + 1] *= fade;
+          for (int w = 0; w < kWords; w += 2) {
+            uint4 a0, a1;
+            Code<F>::unpack(kw[0][w], a0.x, a0.z);
+            Code<F>::unpack(kw[1][w], a0.y, a0.w);
+            Code<F>::unpack(kw[0][w + 1], a1.x, a1.z);
+            Code<F>::unpack(kw[1][w + 1], a1.y, a1.w);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint4 b = qf[((nt * kSteps + part * kWords + w) >> 1) * 32 + lane];
+              mma_16816(s[hh][nt], a0, b.x, b.y);
+              mma_16816(s[hh][nt], a1, b.z, b.w);
             }
           }
         }
+      // weights
+      const bool cut = j0 + 31 > min(first_lim, t1 - 1);
+      uint32_t pb[2][NT][2];  // [hh][nt][x]: operand registers of tokens 8 x + 2 t, + 1, row g
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float ref = m[mt][x] == -INFINITY ? 0.f : m[mt][x];
+      for (int nt = 0; nt < NT; ++nt) {
+        float v[2][4];
+        float most[2] = {kNoMax, kNoMax};
 #pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            float sum = 0.f;
+        for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-            for (int j = 2 * hh; j < 2 * hh + 2; ++j) {
-              s[mt][j][2 * x] = exp2_approx(s[mt][j][2 * x] - ref);
-              s[mt][j][2 * x + 1] = exp2_approx(s[mt][j][2 * x + 1] - ref);
-              sum += s[mt][j][2 * x] + s[mt][j][2 * x + 1];
+          for (int y = 0; y < 2; ++y) {
+            const float c = pc[hh].x * qe[nt][y], b = pc[hh].y - m[nt][y];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              float z = fmaf(s[hh][nt][2 * x + y], c, b);
+              if (cut && j0 + 16 * hh + 8 * x + g > lim[nt][y]) z = -INFINITY;
+              v[hh][2 * x + y] = z;
+              most[y] = fmaxf(most[y], z);
             }
-            l[mt][x] = fmaf(sum, pc[hh].z, l[mt][x]);
+          }
+        // The reference point moves only when a weight would pass 2^8: fp16 holds that as exactly as smaller ones.
+        if (__any_sync(0xffffffffu, fmaxf(most[0], most[1]) > 8.f)) {
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            float top = most[y];  // relative to m
+            if (m[nt][y] == kNoMax) {
+              top = -INFINITY;
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                  const bool in = !cut || j0 + 16 * hh + 8 * x + g <= lim[nt][y];
+                  const float z = fmaf(s[hh][nt][2 * x + y], pc[hh].x * qe[nt][y], pc[hh].y);
+                  if (in) top = fmaxf(top, z);
+                }
+            }
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            float up;  // how far m rises
+            if (m[nt][y] == kNoMax) {
+              up = top == -INFINITY ? 0.f : INFINITY;
+              if (top != -INFINITY) m[nt][y] = top;
+            } else {
+              up = fmaxf(top, 0.f);
+              m[nt][y] += up;
+            }
+            const float fade = exp2_approx(-up);
+            l[nt][y] *= fade;
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) {
+              o[j][nt][y] *= fade;
+              o[j][nt][2 + y] *= fade;
+            }
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                float z = fmaf(s[hh][nt][2 * x + y], pc[hh].x * qe[nt][y], pc[hh].y - m[nt][y]);
+                if (cut && j0 + 16 * hh + 8 * x + g > lim[nt][y]) z = -INFINITY;
+                v[hh][2 * x + y] = z;
+              }
           }
         }
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
-          pa[mt][hh].x = h2_as_u32(__floats2half2_rn(s[mt][2 * hh][0], s[mt][2 * hh][1]));
-          pa[mt][hh].y = h2_as_u32(__floats2half2_rn(s[mt][2 * hh][2], s[mt][2 * hh][3]));
-          pa[mt][hh].z = h2_as_u32(__floats2half2_rn(s[mt][2 * hh + 1][0], s[mt][2 * hh + 1][1]));
-          pa[mt][hh].w = h2_as_u32(__floats2half2_rn(s[mt][2 * hh + 1][2], s[mt][2 * hh + 1][3]));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[hh][e] = exp2_approx(v[hh][e]);
+#pragma unroll
+          for (int y = 0; y < 2; ++y) l[nt][y] = fmaf(v[hh][y] + v[hh][2 + y], pc[hh].z, l[nt][y]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            pb[hh][nt][x] = transpose_8x8(h2_as_u32(__floats2half2_rn(v[hh][2 * x], v[hh][2 * x + 1])));
         }
       }
-      // output += weights x V
+      // output += V^T x weights; o[.][nt][2 x + y]: dim 16 g + 2 tile + x, row 8 nt + 2 t + y
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
@@ -552,7 +592,7 @@ __global__ void __launch_bounds__(kAttWarps * 32)
           }
 #pragma unroll
           for (int w = 0; w < kVWords; ++w) {
-            uint32_t b[4][2];  // [dim of the word][k half]
+            uint32_t b[4][2];  // [dim of the word][token half]
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               const uint32_t a01 = __byte_perm(vw[2 * c][w], vw[2 * c + 1][w], 0x5140);
@@ -561,10 +601,12 @@ __global__ void __launch_bounds__(kAttWarps * 32)
               Code<F>::unpack(a23, b[2][c], b[3][c]);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 2; ++e) {
+              const uint4 a = make_uint4(b[2 * e][0], b[2 * e + 1][0], b[2 * e][1], b[2 * e + 1][1]);
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt)
-                mma_16816(o[mt][part * (kPart / 8) + 4 * w + e], pa[mt][hh], b[e][0], b[e][1]);
+              for (int nt = 0; nt < NT; ++nt)
+                mma_16816(o[part * (kPart / 16) + 2 * w + e][nt], a, pb[hh][nt][0], pb[hh][nt][1]);
+            }
           }
         }
       // the stage is free: fetch tile i + kRing into it
@@ -579,51 +621,48 @@ __global__ void __launch_bounds__(kAttWarps * 32)
     }
     used += count;
 
-    // Join the warps, an m tile at a time, in the ring's memory (it is empty now).
-    // o[.][j][2x + y]: row g + 8x, dim of n = 2t + y in tile j.
+    // Join the warps, eight rows at a time, in the ring's memory (it is empty now).
     const bool whole = step == 0 && step_end == steps;
     const int slot = (int)blockIdx.x * 2 + (s0 == item_at ? 1 : 0);
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+    for (int nt = 0; nt < NT; ++nt) {
+      if (row0 + nt * 8 >= rows) break;
       __syncthreads();
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int row = x * 8 + g;
-        float sum = l[mt][x];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if (t == 0) {
-          jm[warp * kRows + mt * 16 + row] = m[mt][x];
-          jl[warp * kRows + mt * 16 + row] = sum;
+      for (int y = 0; y < 2; ++y) {
+        const int row = 2 * t + y;
+        float sum = l[nt][y];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (g == 0) {
+          jm[warp * kRows + nt * 8 + row] = m[nt][y];
+          jl[warp * kRows + nt * 8 + row] = sum;
         }
-        if (row0 + mt * 16 + row < rows) {
+        if (row0 + nt * 8 + row < rows) {
 #pragma unroll
           for (int part = 0; part < kParts; ++part)
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
-#pragma unroll
-              for (int j = 0; j < kPart / 8; j += 4) {
-                float* dst = joined + (warp * 16 + row) * HD + part * kPart + (2 * t + y) * (kPart / 8) + j;
-                const int jj = part * (kPart / 8) + j;
-                *reinterpret_cast<float4*>(dst) = make_float4(o[mt][jj][2 * x + y], o[mt][jj + 1][2 * x + y],
-                                                              o[mt][jj + 2][2 * x + y], o[mt][jj + 3][2 * x + y]);
-              }
+            for (int j = 0; j < kPart / 16; j += 2) {
+              float* dst = joined + (warp * 8 + row) * L::kPitch + part * kPart + g * (kPart / 8) + 2 * j;
+              const int jj = part * (kPart / 16) + j;
+              *reinterpret_cast<float4*>(dst) =
+                  make_float4(o[jj][nt][y], o[jj][nt][2 + y], o[jj + 1][nt][y], o[jj + 1][nt][2 + y]);
+            }
         }
       }
       __syncthreads();
-      for (int i = threadIdx.x; i < 16 * HD / 4; i += kAttWarps * 32) {
+      for (int i = threadIdx.x; i < 8 * HD / 4; i += kAttWarps * 32) {
         const int row = i / (HD / 4), d = (i % (HD / 4)) * 4;
-        const int tr = mt * 16 + row;
+        const int tr = nt * 8 + row;
         if (row0 + tr >= rows) break;
-        float top = -INFINITY;
+        float top = kNoMax;
 #pragma unroll
         for (int w = 0; w < kAttWarps; ++w) top = fmaxf(top, jm[w * kRows + tr]);
-        const float ref = top == -INFINITY ? 0.f : top;
         float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
 #pragma unroll
         for (int w = 0; w < kAttWarps; ++w) {
-          const float f = exp2_approx(jm[w * kRows + tr] - ref);
-          const float4 x = *reinterpret_cast<const float4*>(joined + (w * 16 + row) * HD + d);
+          const float f = exp2_approx(jm[w * kRows + tr] - top);
+          const float4 x = *reinterpret_cast<const float4*>(joined + (w * 8 + row) * L::kPitch + d);
           num[0] = fmaf(x.x, f, num[0]);
           num[1] = fmaf(x.y, f, num[1]);
           num[2] = fmaf(x.z, f, num[2]);
@@ -651,18 +690,17 @@ __global__ void __launch_bounds__(kAttWarps * 32)
         const int live = min(rows - row0, kRows);
         for (int i = threadIdx.x; i < live * (HD / 4); i += kAttWarps * 32) {
           const int tr = i / (HD / 4), d = (i % (HD / 4)) * 4;
-          float top = -INFINITY;
+          float top = kNoMax;
           for (int c = c0; c <= c1; ++c) {
             const float* part = parts + (size_t)(2 * c + (c == c0)) * kRows * (HD + 2);
             top = fmaxf(top, __ldcg(part + kRows * HD + 2 * tr));
           }
-          const float ref = top == -INFINITY ? 0.f : top;
           float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
           for (int c = c0; c <= c1; ++c) {
             const float* part = parts + (size_t)(2 * c + (c == c0)) * kRows * (HD + 2);
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + kRows * HD + 2 * tr));
             const float4 x = __ldcg(reinterpret_cast<const float4*>(part + (size_t)tr * HD + d));
-            const float f = exp2_approx(ml.x - ref);
+            const float f = exp2_approx(ml.x - top);
             num[0] = fmaf(x.x, f, num[0]);
             num[1] = fmaf(x.y, f, num[1]);
             num[2] = fmaf(x.z, f, num[2]);
@@ -680,20 +718,13 @@ __global__ void __launch_bounds__(kAttWarps * 32)
   }
 }
 
-constexpr int kStreamPerSm = 3;  // CTAs per SM that the grid is sized for (2 where shared memory allows no more)
-
-template <int HD, int MT>
-constexpr int stream_per_sm() {
-  return StreamLayout<HD, MT>::kTotal <= 75 * 1024 ? kStreamPerSm : StreamLayout<HD, MT>::kTotal <= 113 * 1024 ? 2 : 1;
-}
-
 // One counter per CTA, then partial sums of two items per CTA.  The counters
 // are where they are for every variant, since they must stay zero between calls.
 constexpr size_t kCounterBytes = 16384;
 
-template <int HD, int MT>
+template <int HD, int NT>
 size_t stream_workspace(int sms) {
-  return kCounterBytes + (size_t)sms * stream_per_sm<HD, MT>() * 2 * (16 * MT) * (HD + 2) * 4;
+  return kCounterBytes + (size_t)sms * stream_per_sm<HD, NT>() * 2 * (8 * NT) * (HD + 2) * 4;
 }
 
 struct CacheMapKey {
@@ -744,9 +775,9 @@ int cache_map(const DeviceInfo& dev, const void* cache, long long rows, int dim,
   return GDSQ_OK;
 }
 
-template <int HD, int F, int MT>
+template <int HD, int F, int NT>
 int launch_stream(const AttendArgs& a, const DeviceInfo& dev, void* workspace, size_t bytes, cudaStream_t stream) {
-  const size_t need = stream_workspace<HD, MT>(dev.sms);
+  const size_t need = stream_workspace<HD, NT>(dev.sms);
   if (bytes < need)
     return fail(GDSQ_ERR_INVALID_VALUE, "attend_kv8: workspace of %zu bytes, %zu needed", bytes, need);
   const long long rows = ((long long)a.num_blocks * a.kv_heads) << a.block_shift;
@@ -754,11 +785,11 @@ int launch_stream(const AttendArgs& a, const DeviceInfo& dev, void* workspace, s
   int st = cache_map(dev, a.k_cache, rows, HD, &kmap);
   if (st == GDSQ_OK) st = cache_map(dev, a.v_cache, rows, HD, &vmap);
   if (st != GDSQ_OK) return st;
-  auto kernel = attend_stream_kernel<HD, F, MT>;
-  constexpr int smem = StreamLayout<HD, MT>::kTotal;
+  auto kernel = attend_stream_kernel<HD, F, NT>;
+  constexpr int smem = StreamLayout<HD, NT>::kTotal;
   cudaError_t e = ensure_smem(kernel, smem, dev.ordinal);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(attend)");
-  const int ctas = dev.sms * stream_per_sm<HD, MT>();
+  const int ctas = dev.sms * stream_per_sm<HD, NT>();
   if ((size_t)ctas * sizeof(int) > kCounterBytes) return fail(GDSQ_ERR_UNSUPPORTED, "attend_kv8: %d SMs", dev.sms);
   int* counters = static_cast<int*>(workspace);
   float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
@@ -769,9 +800,11 @@ int launch_stream(const AttendArgs& a, const DeviceInfo& dev, void* workspace, s
 template <int HD, int F>
 int launch_attend(const AttendArgs& a, int max_query_len, const DeviceInfo& dev, void* workspace, size_t bytes,
                   cudaStream_t stream) {
+  const long long rows = (long long)max_query_len * a.group;
+  if (rows <= 8) return launch_stream<HD, F, 1>(a, dev, workspace, bytes, stream);
   if constexpr (HD != 256)
-    if ((long long)max_query_len * a.group > 16) return launch_stream<HD, F, 2>(a, dev, workspace, bytes, stream);
-  return launch_stream<HD, F, 1>(a, dev, workspace, bytes, stream);
+    if (rows > 16) return launch_stream<HD, F, 4>(a, dev, workspace, bytes, stream);
+  return launch_stream<HD, F, 2>(a, dev, workspace, bytes, stream);
 }
 
 }  // namespace
@@ -794,10 +827,12 @@ extern "C" size_t gdsq_attend_kv8_workspace(int num_requests, int max_query_len,
   if (num_requests <= 0 || max_query_len <= 0 || num_heads <= 0 || num_kv_heads <= 0) return 0;
   const DeviceInfo* dev = nullptr;
   if (device_info(&dev) != GDSQ_OK) return 0;
-  const bool few = (long long)max_query_len * (num_heads / num_kv_heads) <= 16;
-  if (head_dim == 64) return few ? stream_workspace<64, 1>(dev->sms) : stream_workspace<64, 2>(dev->sms);
-  if (head_dim == 128) return few ? stream_workspace<128, 1>(dev->sms) : stream_workspace<128, 2>(dev->sms);
-  return stream_workspace<256, 1>(dev->sms);
+  const long long rows = (long long)max_query_len * (num_heads / num_kv_heads);
+  auto of = [&](size_t one, size_t two, size_t four) { return rows <= 8 ? one : rows <= 16 ? two : four; };
+  if (head_dim == 64) return of(stream_workspace<64, 1>(dev->sms), stream_workspace<64, 2>(dev->sms), stream_workspace<64, 4>(dev->sms));
+  if (head_dim == 128)
+    return of(stream_workspace<128, 1>(dev->sms), stream_workspace<128, 2>(dev->sms), stream_workspace<128, 4>(dev->sms));
+  return of(stream_workspace<256, 1>(dev->sms), stream_workspace<256, 2>(dev->sms), stream_workspace<256, 2>(dev->sms));
 }
 
 extern "C" int gdsq_attend_kv8(const void* q, int elem_type, long long q_token_stride, long long q_head_stride,
