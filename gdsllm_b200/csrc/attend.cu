@@ -14,7 +14,7 @@
 // one matrix product per (request, KV head).
 //
 // Products run on 16-bit matrix instructions with fp32 sums.  Every code is
-// exact in fp16 (an e4m3 code as value * 2^-8), and a query row is scaled by a
+// exact in fp16, and a query row is scaled by a
 // power of two to at most 1 before it becomes fp16, so the only operand that
 // is rounded is the softmax weight (11 bits, as the output has).
 //
@@ -106,17 +106,16 @@ struct Code<GDSQ_CACHE_INT8> {
 
 template <>
 struct Code<GDSQ_CACHE_E4M3> {
-  static constexpr float kFactor = 256.f;
-  static constexpr float kLogFactor = 8.f;
-  // seeeemmm to s0eeeemmm0000000: the fp16 with that exponent field is the
-  // code's value * 2^-8, subnormal codes included.  The NaN codes become
-  // 480 * 2^-8, so bytes past a request's end cannot reach a sum as NaN.
-  static __device__ __forceinline__ uint32_t widen(uint32_t x) {  // codes in the high bytes
-    return ((x & 0x7f007f00u) >> 1) | (x & 0x80008000u);
+  static constexpr float kFactor = 1.f;
+  static constexpr float kLogFactor = 0.f;
+  static __device__ __forceinline__ uint32_t widen(uint16_t x) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(x));
+    return d;
   }
   static __device__ __forceinline__ void unpack(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    lo = widen(__byte_perm(w, 0, 0x1404));
-    hi = widen(__byte_perm(w, 0, 0x3424));
+    lo = widen((uint16_t)w);
+    hi = widen((uint16_t)(w >> 16));
   }
 };
 
@@ -580,6 +579,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int tok = 2 * t + (c & 1) + 8 * (c >> 1);
+            const bool past = F == GDSQ_CACHE_E4M3 && cut && j0 + 16 * hh + tok >= t1;  // may hold NaN codes
             const uint32_t row = vb + hh * kHalfBytes + part * kBox + tok * kPart;
             if constexpr (kVWords == 4) {
               const uint4 x = lds128(row + ((g ^ (tok & 7)) << 4));
@@ -589,6 +589,9 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
               vw[c][0] = lds32(at);
               vw[c][1] = lds32(at + 4);
             }
+            if (past)
+#pragma unroll
+              for (int w = 0; w < kVWords; ++w) vw[c][w] = 0;
           }
 #pragma unroll
           for (int w = 0; w < kVWords; ++w) {
