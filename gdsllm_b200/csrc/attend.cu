@@ -178,9 +178,9 @@ __device__ __forceinline__ float3 page_constants(const AttendArgs& p, int page, 
 // Few rows per (request, KV head): single tokens, drafts, short chunks.
 //
 // Bound by reading the cache, so the work is cut by cache tokens, evenly: an
-// item is (request, KV head, tile of 8 * NT rows), its steps are 128 tokens
-// each, and CTA c of C takes the steps [c S / C, (c + 1) S / C) of all items in
-// order.  An item that ends in the CTA it began in is written out; the others
+// item is (request, KV head, tile of 8 * NT rows) and counts kItemCost steps
+// plus one for each 128 tokens; CTA c of C takes the steps [c S / C, (c + 1) S
+// / C) of all items in order.  An item that ends in the CTA it began in is written out; the others
 // leave partial sums, and the CTA that arrives last at an item's counter adds
 // them in CTA order.  So neither ragged lengths nor few requests leave SMs
 // idle, and the result does not depend on who finishes first.
@@ -200,20 +200,21 @@ __device__ __forceinline__ float3 page_constants(const AttendArgs& p, int page, 
 // [query][token], one 8 x 8 transpose per 8 tokens.
 
 constexpr int kStepTokens = kAttWarps * 32;
-constexpr int kRing = 2;  // stages per warp
+constexpr int kRing = 2;      // stages per warp
+constexpr int kItemCost = 2;  // what beginning and ending an item costs, in steps
 
 template <int HD, int NT>
 struct StreamLayout {
   static constexpr int kStage = 2 * 32 * HD;  // K and V of 32 tokens
   static constexpr int kRingBytes = kAttWarps * kRing * kStage;
   static constexpr int kRows = 8 * NT;
-  static constexpr int kPitch = HD + 4;  // floats of a row in the join: eight rows of every warp, in the ring's memory
+  static constexpr int kPitch = HD + 4;  // floats of a row in the join
   static constexpr int kQ = NT * (HD / 16) * 256;
-  static constexpr int kBars = kRingBytes + kQ;
+  static constexpr int kJoin = kRingBytes + kQ;  // eight rows
+  static constexpr int kBars = kJoin + 8 * kPitch * 4;
   static constexpr int kRowInfo = kBars + 128;
   static constexpr int kMl = kRowInfo + kRows * 8;                 // [warps][kRows] m, l
   static constexpr int kTotal = kMl + kAttWarps * kRows * 8 + 64 + 1024;  // + alignment
-  static_assert(kAttWarps * 8 * kPitch * 4 <= kRingBytes, "the join uses the ring's memory");
 };
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
   float* jl = jm + kAttWarps * kRows;
   int* shared_int = reinterpret_cast<int*>(jl + kAttWarps * kRows);  // [4]
   long long* shared_ll = reinterpret_cast<long long*>(shared_int + 4);  // [5]
-  float* joined = reinterpret_cast<float*>(smem);              // [warps][8][kPitch]
+  float* joined = reinterpret_cast<float*>(smem + L::kJoin);   // [8][kPitch]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -272,7 +273,10 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
   const int per = ceil_div(p.requests, kAttWarps * 32);
   const int ra = min((int)threadIdx.x * per, p.requests), rb = min(ra + per, p.requests);
   long long mine = 0;
-  for (int r = ra; r < rb; ++r) mine += (long long)ceil_div(rows_of(r), kRows) * p.kv_heads * steps_of(r);
+  auto cost_of = [&](int r) {
+    return (long long)ceil_div(rows_of(r), kRows) * p.kv_heads * (steps_of(r) + kItemCost);
+  };
+  for (int r = ra; r < rb; ++r) mine += cost_of(r);
   long long upto = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -296,7 +300,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
     int r = ra;
     long long at = before;
     for (; r < rb; ++r) {
-      const long long n = (long long)ceil_div(rows_of(r), kRows) * p.kv_heads * steps_of(r);
+      const long long n = cost_of(r);
       if (s0 < at + n) break;
       at += n;
     }
@@ -309,76 +313,111 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
   uint32_t used = 0;                    // tiles that this warp's ring has delivered
   bool dead = false;                    // a copy never arrived
 
-  while (s0 < s1) {
-    const int start = max(p.starts[r], 0);
-    const int n = max(min(p.starts[r + 1], p.tokens) - start, 0);
-    const int rows = n * p.group;
-    const int row_tiles = ceil_div(rows, kRows);
-    const int len = min(p.seq_lens[r], most_len);
-    if (len < p.seq_lens[r]) record_device_error(kDevErrBadIndex);
-    const int steps = max(ceil_div(len, kStepTokens), 1);
-    const long long request_steps = (long long)row_tiles * p.kv_heads * steps;
-    if (s0 >= request_at + request_steps) {
-      request_at += request_steps;
-      ++r;
-      continue;
+  // The steps of one item that this CTA takes.
+  struct Segment {
+    int r, h, row0, rows, start, lim0;  // row i of the item sees positions up to lim0 + (row0 + i) / group
+    int t0, t1, count;                  // this warp's first token, the end, and its tiles
+    int kv_len, steps;
+    long long first_step;  // of the item, among all steps
+    bool opens, whole, once;
+  };
+  auto next_segment = [&](Segment& a) {
+    while (s0 < s1) {
+      const int start = max(p.starts[r], 0);
+      const int n = max(min(p.starts[r + 1], p.tokens) - start, 0);
+      const int rows = n * p.group;
+      const int row_tiles = ceil_div(rows, kRows);
+      const int len = min(p.seq_lens[r], most_len);
+      if (len < p.seq_lens[r]) record_device_error(kDevErrBadIndex);
+      const int steps = max(ceil_div(len, kStepTokens), 1), cost = steps + kItemCost;
+      const long long request_cost = (long long)row_tiles * p.kv_heads * cost;
+      if (s0 >= request_at + request_cost) {
+        request_at += request_cost;
+        ++r;
+        continue;
+      }
+      const int item = (int)((s0 - request_at) / cost);
+      const long long first_step = request_at + (long long)item * cost + kItemCost;
+      const int step = (int)max(s0 - first_step, 0ll);
+      s0 = first_step + step;
+      if (s0 >= s1) return false;
+      const int step_end = (int)min((long long)steps, step + (s1 - s0));
+      s0 += step_end - step;
+      a.r = r;
+      a.h = item / row_tiles;
+      a.row0 = (item % row_tiles) * kRows;
+      a.rows = rows;
+      a.start = start;
+      a.lim0 = len - n;
+      a.kv_len = max(min(len, a.lim0 + (min(rows, a.row0 + kRows) - 1) / p.group + 1), 0);
+      a.t0 = step * kStepTokens + warp * 32;
+      a.t1 = min(a.kv_len, step_end * kStepTokens);
+      a.count = a.t0 < a.t1 ? (a.t1 - a.t0 + kStepTokens - 1) / kStepTokens : 0;
+      a.steps = steps;
+      a.first_step = first_step;
+      a.opens = step == 0;
+      a.whole = step == 0 && step_end == steps;
+      a.once = row_tiles == 1;
+      return true;
     }
-    const int item = (int)((s0 - request_at) / steps);
-    const int step = (int)((s0 - request_at) % steps);
-    const int step_end = (int)min((long long)steps, step + (s1 - s0));
-    const int h = item / row_tiles, row0 = (item % row_tiles) * kRows;
-    const long long item_at = request_at + (long long)item * steps;
-    const int first_lim = len - n + row0 / p.group;
-    const int kv_len = max(min(len, len - n + (min(rows, row0 + kRows) - 1) / p.group + 1), 0);
-    const int t0 = step * kStepTokens + warp * 32, t1 = min(kv_len, step_end * kStepTokens);
-    const int count = t0 < t1 ? (t1 - t0 + kStepTokens - 1) / kStepTokens : 0;  // this warp's tiles
-
-    // Lane's half tile of a batch of 16 tiles: its row in the cache and constants.
-    auto half_row = [&](int i) {
-      const int pos = min(t0 + (i + (lane >> 1)) * kStepTokens + (lane & 1) * 16, (t1 - 1) & ~15);
-      const int col = pos >> p.block_shift;
-      int page = col < p.table_width ? p.table[(size_t)r * p.table_width + col] : -1;
-      if ((unsigned)page >= (unsigned)p.num_blocks) {
-        record_device_error(kDevErrBadIndex);
-        page = 0;
-      }
-      return make_int2(page, (int)((((long long)page * p.kv_heads + h) << p.block_shift) + (pos & ((1 << p.block_shift) - 1))));
-    };
-    auto issue = [&](int i, int row_lo, int row_hi) {  // lane 0: tile i's boxes
-      unsigned char* st = ring + ((used + i) % kRing) * L::kStage;
-      uint64_t* bar = full + (used + i) % kRing;
-      mbar_arrive_expect_tx(bar, L::kStage);
-      const uint64_t policy = row_tiles == 1 ? l2_policy_evict_first() : l2_policy_normal();
+    return false;
+  };
+  // Lane's half tile of the batch of 16 tiles from tile i: its block and row in the cache.
+  auto half_row = [&](const Segment& a, int i) {
+    const int pos = min(a.t0 + (i + (lane >> 1)) * kStepTokens + (lane & 1) * 16, (a.t1 - 1) & ~15);
+    const int col = pos >> p.block_shift;
+    int page = col < p.table_width ? p.table[(size_t)a.r * p.table_width + col] : -1;
+    if ((unsigned)page >= (unsigned)p.num_blocks) {
+      record_device_error(kDevErrBadIndex);
+      page = 0;
+    }
+    return make_int2(page, (int)((((long long)page * p.kv_heads + a.h) << p.block_shift) + (pos & ((1 << p.block_shift) - 1))));
+  };
+  auto issue = [&](uint32_t tile, bool once, int row_lo, int row_hi) {  // one lane: the boxes of the warp's tile-th tile
+    unsigned char* st = ring + (tile % kRing) * L::kStage;
+    uint64_t* bar = full + tile % kRing;
+    mbar_arrive_expect_tx(bar, L::kStage);
+    const uint64_t policy = once ? l2_policy_evict_first() : l2_policy_normal();
 #pragma unroll
-      for (int part = 0; part < kParts; ++part) {
-        tma_load_2d(st + part * kBox, &kmap, part * 128, row_lo, bar, policy);
-        tma_load_2d(st + kHalfBytes + part * kBox, &kmap, part * 128, row_hi, bar, policy);
-        tma_load_2d(st + 2 * kHalfBytes + part * kBox, &vmap, part * 128, row_lo, bar, policy);
-        tma_load_2d(st + 3 * kHalfBytes + part * kBox, &vmap, part * 128, row_hi, bar, policy);
-      }
-    };
-    int2 cur = make_int2(0, 0), nxt = make_int2(0, 0);
-    if (count > 0) {
-      cur = half_row(0);
+    for (int part = 0; part < kParts; ++part) {
+      tma_load_2d(st + part * kBox, &kmap, part * 128, row_lo, bar, policy);
+      tma_load_2d(st + kHalfBytes + part * kBox, &kmap, part * 128, row_hi, bar, policy);
+      tma_load_2d(st + 2 * kHalfBytes + part * kBox, &vmap, part * 128, row_lo, bar, policy);
+      tma_load_2d(st + 3 * kHalfBytes + part * kBox, &vmap, part * 128, row_hi, bar, policy);
+    }
+  };
+  constexpr int kMine = kRows / kAttWarps, kPairs = HD / 64;  // q rows per warp, pairs per lane
+  // A segment's first copies and its q rows, asked for while the one before it is being joined.
+  auto begin = [&](const Segment& a, int2& at, uint32_t(&raw)[kMine][kPairs]) {
+    if (a.count > 0) {
+      at = half_row(a, 0);
 #pragma unroll
       for (int i = 0; i < kRing; ++i) {
-        const int lo = __shfl_sync(0xffffffffu, cur.y, 2 * i), hi = __shfl_sync(0xffffffffu, cur.y, 2 * i + 1);
-        if (lane == 0 && i < count && !dead) issue(i, lo, hi);
+        const int lo = __shfl_sync(0xffffffffu, at.y, 2 * i), hi = __shfl_sync(0xffffffffu, at.y, 2 * i + 1);
+        if (lane == 0 && i < a.count && !dead) issue(used + i, a.once, lo, hi);
       }
     }
-
-    // Q rows: power-of-two scale, fp16, in operand order.
-    constexpr int kMine = kRows / kAttWarps, kPairs = HD / 64;
-    uint32_t raw[kMine][kPairs];
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
-      const int row = row0 + warp + i * kAttWarps;
+      const int row = a.row0 + warp + i * kAttWarps;
 #pragma unroll
       for (int e = 0; e < kPairs; ++e) raw[i][e] = 0;
-      if (row < rows)
-        load_q<kPairs>(p, (long long)(start + row / p.group) * p.q_token_stride +
-                              (long long)(h * p.group + row % p.group) * p.q_head_stride + lane * (HD / 32), raw[i]);
+      if (row < a.rows)
+        load_q<kPairs>(p, (long long)(a.start + row / p.group) * p.q_token_stride +
+                              (long long)(a.h * p.group + row % p.group) * p.q_head_stride + lane * (HD / 32), raw[i]);
     }
+  };
+
+  Segment now, after;
+  int2 cur = make_int2(0, 0);
+  uint32_t raw[kMine][kPairs];
+  bool more = next_segment(now);
+  if (more) begin(now, cur, raw);
+  while (more) {
+    const int h = now.h, row0 = now.row0, rows = now.rows, t0 = now.t0, t1 = now.t1, count = now.count;
+    const int first_lim = now.lim0 + row0 / p.group;
+    int2 nxt = make_int2(0, 0);
+    // Q rows: power-of-two scale, fp16, in operand order.
 #pragma unroll
     for (int ii = 0; ii < kMine; ++ii) {
       const int i = warp + ii * kAttWarps, row = row0 + i;
@@ -397,7 +436,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
       const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
       if (lane == 0) {
         qexp[i] = __uint_as_float((uint32_t)(127 + ex) << 23);
-        qlim[i] = row < rows ? len - n + row / p.group : kv_len - 1;  // rows past the end are not written
+        qlim[i] = row < rows ? now.lim0 + row / p.group : now.kv_len - 1;  // rows past the end are not written
       }
 #pragma unroll
       for (int e = 0; e < HD / 32; e += 2) {
@@ -441,7 +480,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
         cur = nxt;
         cc = nc;
       }
-      if (u == 0 && i + 16 < count) nxt = half_row(i + 16);
+      if (u == 0 && i + 16 < count) nxt = half_row(now, i + 16);
       if (u == 8 && i + 8 < count) nc = page_constants(p, nxt.x, h, Code<F>::kLogFactor);
       float3 pc[2];
 #pragma unroll
@@ -618,72 +657,88 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
       const int lo = __shfl_sync(0xffffffffu, src, 2 * v2), hi = __shfl_sync(0xffffffffu, src, 2 * v2 + 1);
       if (lane == 0 && i + kRing < count && !dead) {
         fence_proxy_async_smem();
-        issue(i + kRing, lo, hi);
+        issue(used + i + kRing, now.once, lo, hi);
       }
       __syncwarp();
     }
     used += count;
 
-    // Join the warps, eight rows at a time, in the ring's memory (it is empty now).
-    const bool whole = step == 0 && step_end == steps;
-    const int slot = (int)blockIdx.x * 2 + (s0 == item_at ? 1 : 0);
+    more = next_segment(after);
+    if (more) begin(after, cur, raw);
+
+    // Join the warps: each adds its sums, scaled to the largest maximum, in turn; eight rows at a time.
+    const bool whole = now.whole;
+    const int slot = (int)blockIdx.x * 2 + (now.opens ? 1 : 0);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      if (row0 + nt * 8 >= rows) break;
-      __syncthreads();
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const int row = 2 * t + y;
         float sum = l[nt][y];
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (g == 0) {
-          jm[warp * kRows + nt * 8 + row] = m[nt][y];
-          jl[warp * kRows + nt * 8 + row] = sum;
-        }
-        if (row0 + nt * 8 + row < rows) {
-#pragma unroll
-          for (int part = 0; part < kParts; ++part)
-#pragma unroll
-            for (int j = 0; j < kPart / 16; j += 2) {
-              float* dst = joined + (warp * 8 + row) * L::kPitch + part * kPart + g * (kPart / 8) + 2 * j;
-              const int jj = part * (kPart / 16) + j;
-              *reinterpret_cast<float4*>(dst) =
-                  make_float4(o[jj][nt][y], o[jj][nt][2 + y], o[jj + 1][nt][y], o[jj + 1][nt][2 + y]);
-            }
+          jm[warp * kRows + nt * 8 + 2 * t + y] = m[nt][y];
+          jl[warp * kRows + nt * 8 + 2 * t + y] = sum;
         }
       }
-      __syncthreads();
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      if (row0 + nt * 8 >= rows) break;
+      float fade[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        float top = kNoMax;
+#pragma unroll
+        for (int w = 0; w < kAttWarps; ++w) top = fmaxf(top, jm[w * kRows + nt * 8 + 2 * t + y]);
+        fade[y] = exp2_approx(m[nt][y] - top);
+      }
+      for (int w = 0; w < kAttWarps; ++w) {
+        if (w == warp) {
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            if (row0 + nt * 8 + 2 * t + y < rows) {
+#pragma unroll
+              for (int part = 0; part < kParts; ++part)
+#pragma unroll
+                for (int j = 0; j < kPart / 16; j += 2) {
+                  float4* dst = reinterpret_cast<float4*>(joined + (2 * t + y) * L::kPitch + part * kPart + g * (kPart / 8) + 2 * j);
+                  const int jj = part * (kPart / 16) + j;
+                  float4 x = w ? *dst : make_float4(0.f, 0.f, 0.f, 0.f);
+                  x.x = fmaf(o[jj][nt][y], fade[y], x.x);
+                  x.y = fmaf(o[jj][nt][2 + y], fade[y], x.y);
+                  x.z = fmaf(o[jj + 1][nt][y], fade[y], x.z);
+                  x.w = fmaf(o[jj + 1][nt][2 + y], fade[y], x.w);
+                  *dst = x;
+                }
+            }
+        }
+        __syncthreads();
+      }
       for (int i = threadIdx.x; i < 8 * HD / 4; i += kAttWarps * 32) {
         const int row = i / (HD / 4), d = (i % (HD / 4)) * 4;
         const int tr = nt * 8 + row;
         if (row0 + tr >= rows) break;
-        float top = kNoMax;
+        float top = kNoMax, den = 0.f;
 #pragma unroll
         for (int w = 0; w < kAttWarps; ++w) top = fmaxf(top, jm[w * kRows + tr]);
-        float num[4] = {0.f, 0.f, 0.f, 0.f}, den = 0.f;
 #pragma unroll
-        for (int w = 0; w < kAttWarps; ++w) {
-          const float f = exp2_approx(jm[w * kRows + tr] - top);
-          const float4 x = *reinterpret_cast<const float4*>(joined + (w * 8 + row) * L::kPitch + d);
-          num[0] = fmaf(x.x, f, num[0]);
-          num[1] = fmaf(x.y, f, num[1]);
-          num[2] = fmaf(x.z, f, num[2]);
-          num[3] = fmaf(x.w, f, num[3]);
-          den = fmaf(jl[w * kRows + tr], f, den);
-        }
+        for (int w = 0; w < kAttWarps; ++w) den = fmaf(jl[w * kRows + tr], exp2_approx(jm[w * kRows + tr] - top), den);
+        const float4 x = *reinterpret_cast<const float4*>(joined + row * L::kPitch + d);
+        const float num[4] = {x.x, x.y, x.z, x.w};
         if (whole) {
-          store_out(p, start, h, row0 + tr, d, num, den);
+          store_out(p, now.start, h, row0 + tr, d, num, den);
         } else {
           float* part = parts + (size_t)slot * kRows * (HD + 2);
           *reinterpret_cast<float4*>(part + (size_t)tr * HD + d) = make_float4(num[0], num[1], num[2], num[3]);
           if (d == 0) *reinterpret_cast<float2*>(part + kRows * HD + 2 * tr) = make_float2(top, den);
         }
       }
+      __syncthreads();
     }
     if (!whole) {
       // the CTAs that hold the item's first and last step
-      const int c0 = (int)(((item_at + 1) * C - 1) / all), c1 = (int)(((item_at + steps) * C - 1) / all);
+      const int c0 = (int)(((now.first_step + 1) * C - 1) / all), c1 = (int)(((now.first_step + now.steps) * C - 1) / all);
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) shared_int[1] = atomicAdd(counters + c0, 1) == c1 - c0;
@@ -710,14 +765,12 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
             num[3] = fmaf(x.w, f, num[3]);
             den = fmaf(ml.y, f, den);
           }
-          store_out(p, start, h, row0 + tr, d, num, den);
+          store_out(p, now.start, h, row0 + tr, d, num, den);
         }
         if (threadIdx.x == 0) counters[c0] = 0;
       }
     }
-    fence_proxy_async_smem();  // the ring's memory goes back to the copies
-    __syncthreads();
-    s0 += step_end - step;
+    now = after;
   }
 }
 

@@ -152,10 +152,11 @@ __global__ void __launch_bounds__(kTabThreads) build_tables_kernel(const TablesA
 // 448 (e4m3):
 //   need = m / top, base = 0 on a block begun by these tokens, else its scale
 //   scale = base if need <= base, else max(need, 2 base)
-// A scale that grows at least doubles, so the codes held before, multiplied by
+// A scale that grows at least doubles, so int8 codes held before, multiplied by
 // base / scale and rounded again, are off by less than one step of the new
-// scale after any number of growths (e4m3: not at all, while they stay normal,
-// when it just doubles).  A non-finite value makes the block's scale NaN and
+// scale after any number of growths.  An e4m3 code is not changed by a growth
+// that just doubles (while it stays normal) and is rounded once more by one
+// that more than doubles.  A non-finite value makes the block's scale NaN and
 // is itself stored as 0.  New tokens of one block are adjacent in the batch.
 
 constexpr int kAppThreads = 256;
