@@ -89,8 +89,9 @@ def build_ext(force: bool = False, verbose: bool = True) -> Path:
     import torch
     from torch.utils import cpp_extension
 
-    sources = [CSRC / "gds_io_ext.cpp", INCLUDE / "gdsq.h", LIB_PATH]
-    if not (force or _newer(EXT_PATH, sources)):
+    units = [(CSRC / name, BUILD / (Path(name).stem + ".o")) for name in ("gds_io_ext.cpp", "serve_ext.cpp")]
+    stale = [(src, obj) for src, obj in units if force or _newer(obj, _sources(src))]
+    if not stale and not _newer(EXT_PATH, [LIB_PATH, *[obj for _, obj in units]]):
         return EXT_PATH
     BUILD.mkdir(parents=True, exist_ok=True)
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
@@ -99,12 +100,20 @@ def build_ext(force: bool = False, verbose: bool = True) -> Path:
         includes += ["-I", p]
     includes += ["-I", str(CUDA_HOME / "include"), "-I", sysconfig.get_paths()["include"],
                  "-I", str(INCLUDE)]
+
+    def compile_unit(unit):
+        src, obj = unit
+        tmp = obj.with_suffix(".o.tmp")
+        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+              "-DTORCH_EXTENSION_NAME=gds_io_ext", "-DTORCH_API_INCLUDE_EXTENSION_H",
+              f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *includes, "-c", str(src), "-o", str(tmp)], verbose)
+        os.replace(tmp, obj)
+
+    with ThreadPoolExecutor(max_workers=4) as pool:
+        list(pool.map(compile_unit, stale))
     torch_lib = str(Path(torch.__file__).parent / "lib")
     tmp = EXT_PATH.with_suffix(".tmp")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           "-DTORCH_EXTENSION_NAME=gds_io_ext", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *includes,
-           str(CSRC / "gds_io_ext.cpp"), "-o", str(tmp),
+    cmd = ["g++", "-shared", *[str(obj) for _, obj in units], "-o", str(tmp),
            f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
            "-ltorch_python", f"-L{BUILD}", "-lgdsq", "-Wl,-rpath,$ORIGIN",
            f"-L{CUDA_HOME / 'lib64'}", "-lcudart", "-ldl"]

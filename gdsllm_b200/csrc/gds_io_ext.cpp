@@ -946,6 +946,8 @@ int py_device_error(int device, bool clear) {
 
 }  // namespace
 
+void bind_serving(py::module_& m);  // serve_ext.cpp
+
 PYBIND11_MODULE(gds_io_ext, m) {
   m.doc() = "GdsLLM decode-path op boundary on the gdsq sm_100a kernels (B200)";
   m.attr("backend") = "gdsq-sm100a";
@@ -1021,4 +1023,6 @@ PYBIND11_MODULE(gds_io_ext, m) {
         "Enable programmatic dependent launch for the GEMV kernels.", py::arg("enable"));
   m.def("device_error", &py_device_error, "Read (and optionally clear) the kernel-side error word.",
         py::arg("device") = 0, py::arg("clear") = true);
+
+  bind_serving(m);
 }

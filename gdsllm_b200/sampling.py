@@ -8,12 +8,7 @@ from __future__ import annotations
 
 import torch
 
-from ._native import check, lib
-from .paged import _ELEM, _ints
-
-
-def _param(t: torch.Tensor | None, name: str, rows: int, device, dtype=torch.float32) -> int | None:
-    return None if t is None else _ints(t, name, rows, device, dtype)
+from ._native import ext
 
 
 def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: torch.Tensor | None = None,
@@ -31,20 +26,4 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: torch.T
     share.  Temperature 0 takes the largest logit.  Each parameter is a [B]
     tensor (top_k int32, the rest fp32) or None.  A row with no logit above
     -inf gives token -1; NaN counts as -inf."""
-    if logits.dim() != 2 or logits.dtype not in _ELEM or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise ValueError(f"logits: [rows, vocab] fp16, bf16 or fp32 with contiguous rows, got {tuple(logits.shape)} "
-                         f"{logits.dtype} strides {logits.stride()}")
-    b, v = logits.shape
-    dev = logits.device
-    if tokens is None:
-        tokens = torch.empty(b, dtype=torch.int64, device=dev)
-    if logprobs is None:
-        logprobs = torch.empty(b, dtype=torch.float32, device=dev)
-    status = lib().gdsq_sample(
-        _ELEM[logits.dtype], logits.data_ptr(), logits.stride(0), b, v, _ints(uniforms, "uniforms", b, dev, torch.float32),
-        _param(temperature, "temperature", b, dev), _param(top_k, "top_k", b, dev, torch.int32),
-        _param(top_p, "top_p", b, dev), _param(min_p, "min_p", b, dev), _ints(tokens, "tokens", b, dev, torch.int64),
-        _ints(logprobs, "logprobs", b, dev, torch.float32), torch.cuda.current_stream(dev).cuda_stream)
-    if status:
-        check(status, "gdsq_sample")
-    return tokens, logprobs
+    return ext().sample(logits, uniforms, temperature, top_k, top_p, min_p, tokens, logprobs)
