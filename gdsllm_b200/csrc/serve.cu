@@ -8,6 +8,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstring>
+#include <type_traits>
 
 #include "gdsq.h"
 #include "host.h"
@@ -184,14 +186,14 @@ template <>
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 template <>
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <>
-__device__ __forceinline__ float to_f32(float v) { return v; }
 template <typename T>
 __device__ __forceinline__ T from_f32(float v);
 template <>
 __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ float from_f32(float v) { return v; }
 
 template <int N, typename T>
 __device__ __forceinline__ void load_row(const T* src, float (&x)[N]) {
@@ -326,7 +328,24 @@ __global__ void __launch_bounds__(kAppThreads) append_kv8_kernel(const AppendArg
 // top_k's, and with e >= min_p; the first is always kept.  The token is the
 // first kept index, in index order, whose running sum exceeds floor(u * sum).
 
-constexpr int kSampleThreads = 1024;
+// A row lives in the shared memory of one cluster: thread i of the cluster owns
+// the 32 logits from 32 i (counted from the 16-byte boundary below the row), so
+// that index order is thread order, and the logits are read once.  The work is
+// one exponential per logit where the whole weight is needed (no filter, or
+// top-p alone), else one per token that can be kept.
+//
+// A cut (top_k by count, top_p by weight) is found by histograms over the
+// distance of a logit's ordered bit pattern from the maximum's: 2048 bins over
+// the span of the candidates, then 2048 inside the bin where the cut falls,
+// until a bin is one logit value; ties then follow from counts alone.
+// Candidates are few: a token of weight 0 never matters; one below the k-th
+// largest of the threads' own maxima is not among the top k; tokens of weight
+// below (1 - p) W / V cannot add up to the part that top-p removes.
+
+constexpr int kSampleItems = 32;  // logits per thread
+constexpr int kSampleBins = 2048;
+constexpr int kSampleDirect = 8192;  // rows up to here go into the top-k histogram whole
+constexpr float kWeightCut = -21.6f;  // floor(2^31 exp(z)) = 0 below (ln 2^-31 = -21.49)
 
 struct SampleArgs {
   const void* logits;
@@ -352,209 +371,462 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-struct Bins {
-  uint32_t count[256];
-  unsigned long long weight[256];
+// The logits of one CTA in shared memory, 16-byte vectors in an order in which
+// lanes write neighbouring vectors and read their own stretch of 32 logits
+// without bank conflicts.
+template <typename T>
+struct SampleRow {
+  static constexpr int kVec = 16 / sizeof(T);           // logits per vector
+  static constexpr int kVecs = kSampleItems / kVec;     // vectors per thread
+  static constexpr int kDrop = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 13 : 16;  // low bits of the fp32 pattern that say nothing
+  uint32_t at;  // shared address
+
+  static __device__ __forceinline__ uint32_t place(uint32_t v) { return (v ^ ((v >> 3) & (kVecs - 1))) << 4; }
+
+  // Vectors first .. of the row, counted from the 16-byte boundary at or below its start; what lies outside becomes -inf.
+  __device__ __forceinline__ void load(const T* row, int skew, int first, int vocab, int threads) const {
+    constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+      const int v = j * threads + threadIdx.x;
+      const long long i = (long long)(first + v) * kVec - skew;
+      uint4 x = make_uint4(kNone, kNone, kNone, kNone);
+      if (i >= 0 && i + kVec <= vocab) {
+        x = __ldg(reinterpret_cast<const uint4*>(row + i));
+      } else if (i + kVec > 0 && i < vocab) {
+        T e[kVec];
+#pragma unroll
+        for (int y = 0; y < kVec; ++y) e[y] = i + y >= 0 && i + y < vocab ? row[i + y] : from_f32<T>(-INFINITY);
+        memcpy(&x, e, 16);
+      }
+      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + place(v)), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
+                   : "memory");
+    }
+  }
+
+  // f(i, logit) for this thread's 32 logits in index order.
+  template <typename Fn>
+  __device__ __forceinline__ void each(Fn f) const {
+#pragma unroll 1
+    for (int j = 0; j < kVecs; ++j) {
+      const uint4 x = lds128(at + place(threadIdx.x * kVecs + j));
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        float v;
+        if constexpr (sizeof(T) == 4) v = __uint_as_float(w[e]);
+        else if constexpr (std::is_same<T, __half>::value) v = __half2float(__ushort_as_half((unsigned short)(w[e >> 1] >> (16 * (e & 1)))));
+        else v = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+        f(j * kVec + e, v);
+      }
+    }
+  }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kSampleThreads) sample_simple_kernel(const SampleArgs p) {
-  __shared__ Bins bins;
-  __shared__ uint32_t red[32];
-  __shared__ unsigned long long wsum[32];
-  __shared__ unsigned wtie[32];
-  __shared__ uint32_t s_prefix;
-  __shared__ unsigned s_before_n;
-  __shared__ unsigned long long s_before_w;
-  __shared__ int s_found;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+struct SampleShared {
+  uint32_t lo[kSampleBins];  // counts, or low halves of weights
+  uint32_t hi[kSampleBins];  // high halves of weights
+  unsigned long long sum[32];
+  uint32_t num[32];
+  // by cluster rank, each written once
+  uint32_t rank_top[16];
+  unsigned long long rank_total[16];
+  unsigned long long rank_sum[16];
+  uint32_t rank_ties[16];
+  // the histogram's answer, written by the cluster's first CTA
+  uint32_t bin;
+  uint32_t found;
+  unsigned long long before, at;
+};
+
+// Grid: one cluster per row.
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const SampleArgs p, const int ranks) {
+  using Items = SampleRow<T>;
+  constexpr int kWarps = kThreads / 32;
+  __shared__ SampleShared sh;
+  extern __shared__ __align__(16) unsigned char logits_smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = ranks > 1 ? (int)(blockIdx.x % ranks) : 0;
+  const int b = blockIdx.x / ranks;
   const int V = p.vocab;
+  auto everyone = [&] {
+    if (ranks > 1) cluster_sync_all();
+    else __syncthreads();
+  };
+  // Stores `v` to *slot in every CTA of the cluster; one warp calls it.
+  auto tell_u64 = [&](unsigned long long* slot, unsigned long long v) {
+    if (ranks == 1) {
+      if (lane == 0) *slot = v;
+    } else if (lane < ranks) {
+      st_cluster_u64(map_to_rank(slot, lane), v);
+    }
+  };
+  auto tell_u32 = [&](uint32_t* slot, uint32_t v) {
+    if (ranks == 1) {
+      if (lane == 0) *slot = v;
+    } else if (lane < ranks) {
+      st_cluster_u32(map_to_rank(slot, lane), v);
+    }
+  };
+  // Sum over the cluster, the same in every thread; called once at most.
+  auto total = [&](unsigned long long v) {
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    if (lane == 0) sh.sum[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+      v = lane < kWarps ? sh.sum[lane] : 0;
+#pragma unroll
+      for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+      tell_u64(&sh.rank_total[rank], v);
+    }
+    everyone();
+    v = 0;
+    for (int r = 0; r < ranks; ++r) v += sh.rank_total[r];
+    return v;
+  };
+
+  if (ranks > 1) cluster_arrive_relaxed();  // waited for before the first store to a peer
   pdl_launch_dependents();
   pdl_wait_primary();
   const T* row = static_cast<const T*>(p.logits) + (long long)b * p.row_stride;
+  const int skew = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+  const int base = (rank * kThreads + tid) * kSampleItems - skew;  // index of this thread's first logit
+  const Items x{smem_addr(logits_smem)};
+  x.load(row, skew, rank * kThreads * Items::kVecs, V, kThreads);
   const float temp = p.temperature ? p.temperature[b] : 1.f;
   const bool greedy = !(temp > 0.f);
   const float inv = greedy ? 1.f : __frcp_rn(temp);
-  int k = p.top_k ? p.top_k[b] : 0;
-  if (greedy) k = 1;
-  if (k <= 0 || k > V) k = V;
   const float mp = p.min_p ? p.min_p[b] : 0.f;
-  if (mp > 1.f || !(mp == mp)) k = 1;  // nothing but the first passes
+  const float tp = p.top_p ? p.top_p[b] : 1.f;
+  const float u = p.uniforms[b];
+  int k = p.top_k ? p.top_k[b] : 0;
+  if (greedy || mp > 1.f || !(mp == mp)) k = 1;  // min_p above 1: nothing but the first passes
+  if (k <= 0 || k > V) k = V;
 
-  uint32_t top = 0;
-  for (int i = tid; i < V; i += kSampleThreads) top = max(top, order_key(to_f32(row[i])));
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0) red[warp] = top;
+  // the maximum
+  uint32_t own_top = 0;
   __syncthreads();
-  for (int w = 0; w < 32; ++w) top = max(top, red[w]);
+  x.each([&](int, float v) { own_top = max(own_top, order_key(v)); });
+  {
+    const uint32_t t = __reduce_max_sync(0xffffffffu, own_top);
+    if (lane == 0) sh.num[warp] = t;
+    __syncthreads();
+    if (ranks > 1) cluster_wait();
+    if (warp == 0) {
+      const uint32_t t2 = __reduce_max_sync(0xffffffffu, lane < kWarps ? sh.num[lane] : 0);
+      tell_u32(&sh.rank_top[rank], t2);
+    }
+    everyone();
+  }
+  uint32_t top = 0;
+  for (int r = 0; r < ranks; ++r) top = max(top, sh.rank_top[r]);
   const float most = key_value(top);
-  if (most == -INFINITY) {
-    if (tid == 0) {
+  if (most == -INFINITY) {  // the whole cluster leaves
+    if (rank == 0 && tid == 0) {
       p.tokens[b] = -1;
       if (p.logprobs) p.logprobs[b] = -INFINITY;
     }
     return;
   }
-  auto e_of = [&](uint32_t key) {
-    const float x = key_value(key);
-    if (key == top) return 1.f;
-    if (x == -INFINITY) return 0.f;
-    return expf(__fmul_rn(x - most, inv));
-  };
-  auto w_of = [&](uint32_t key) -> unsigned long long { return (uint32_t)(e_of(key) * 2147483648.f); };
+  auto z_of = [&](float v) { return __fmul_rn(v - most, inv); };  // NaN for a NaN logit, for inf - inf and for 0 x inf
+  auto e_of = [&](float v) { return v == most ? 1.f : expf(z_of(v)); };
+  auto w_of = [&](float v) { return (uint32_t)(e_of(v) * 2147483648.f); };
+  auto near = [&](float v, float cut) { return v == most || z_of(v) >= cut; };
 
-  // The key where a prefix ends: the first whose bin, bits taken from the top,
-  // brings the count to `want` (by_weight: the weight to `limit`).  Leaves the
-  // key, and the count and weight of the larger keys, in shared memory.
-  auto select = [&](bool by_weight, unsigned want, unsigned long long limit, uint32_t floor_key, unsigned floor_n) {
-    if (tid == 0) {
-      s_prefix = 0;
-      s_before_n = 0;
-      s_before_w = 0;
-      s_found = 1;
-    }
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) {
-        bins.count[tid] = 0;
-        bins.weight[tid] = 0;
-      }
-      __syncthreads();
-      const uint32_t prefix = s_prefix;
-      for (int i = tid; i < V; i += kSampleThreads) {
-        const uint32_t key = order_key(to_f32(row[i]));
-        if (shift < 24 && (key >> (shift + 8)) != (prefix >> (shift + 8))) continue;
-        if (key < floor_key) continue;
-        const int d = (key >> shift) & 255;
-        atomicAdd(&bins.count[d], 1u);
-        if (key > floor_key) atomicAdd(&bins.weight[d], w_of(key));
-      }
-      __syncthreads();
-      if (tid == 0) {
-        unsigned n = s_before_n;
-        unsigned long long w = s_before_w;
-        int d = 255;
-        for (; d >= 0; --d) {
-          unsigned c = bins.count[d];
-          unsigned long long bw = bins.weight[d];
-          if (floor_key && ((prefix | ((uint32_t)d << shift)) >> shift) == (floor_key >> shift)) bw += floor_n * w_of(floor_key);
-          if (by_weight ? w + bw >= limit : n + c >= want) break;
-          n += c;
-          w += bw;
-        }
-        if (d < 0) {
-          s_found = 0;
-          d = 0;
-        }
-        s_prefix = prefix | ((uint32_t)d << shift);
-        s_before_n = n;
-        s_before_w = w;
-      }
-      __syncthreads();
-      if (!s_found) return;
-    }
-  };
 
-  // kept: keys above `thr`, and the first `ties` of those equal to it
-  uint32_t thr = 0;
-  unsigned ties = 0xffffffffu;
-  if (k < V) {
-    select(false, (unsigned)k, 0, 0, 0);
-    thr = s_prefix;
-    ties = k - s_before_n;
-    __syncthreads();
-  }
-  const float tp = p.top_p ? p.top_p[b] : 1.f;
-  if (tp < 1.f || !(tp == tp)) {
-    unsigned long long all = 0;
-    if (k < V) {
-      all = s_before_w + ties * w_of(thr);
-    } else {
-      for (int i = tid; i < V; i += kSampleThreads) all += w_of(order_key(to_f32(row[i])));
+  // Where the running sum over falling logits reaches `want`: all shares of values
+  // at distances [first, first + width) from the maximum, with `before` the sum over
+  // nearer ones and `at` the sum in it.  each(f) calls f(logit) for the candidates,
+  // which lie at distances below `span`; their share is their weight, or 1.
+  // fix(from, to) is taken off the sum of the distances [from, to).  `coarse`
+  // stops at a bin, else width is 1: one logit value.
+  struct Cut {
+    uint32_t first, width;
+    unsigned long long before, at;
+    bool found;
+  };
+  const uint32_t top_key = top >> Items::kDrop;
+  auto histogram = [&](unsigned long long want, uint32_t span, bool weights, bool coarse, auto each, auto fix) {
+    Cut c{0, 0, 0, 0, true};
+    for (;;) {
+      const int shift = max(0, 21 - __clz(span - 1));  // span <= 2048 << shift
+      for (int i = tid; i < kSampleBins; i += kThreads) {
+        sh.lo[i] = 0;
+        sh.hi[i] = 0;
+      }
+      __syncthreads();
+      each([&](float v) {
+        const uint32_t d = top_key - (order_key(v) >> Items::kDrop) - c.first;
+        if (d >= span) return;
+        if (weights) {
+          const uint32_t w = w_of(v);
+          atomicAdd(&sh.lo[d >> shift], w & 0xffffu);
+          atomicAdd(&sh.hi[d >> shift], w >> 16);
+        } else {
+          atomicAdd(&sh.lo[d >> shift], 1u);
+        }
+      });
+      everyone();
+      if (rank == 0) {
+        constexpr int kPer = kSampleBins / kThreads;
+        unsigned long long mine[kPer], sum = 0;
 #pragma unroll
-      for (int m = 16; m > 0; m >>= 1) all += __shfl_xor_sync(0xffffffffu, all, m);
-      if (lane == 0) wsum[warp] = all;
-      __syncthreads();
-      all = 0;
-      for (int w = 0; w < 32; ++w) all += wsum[w];
+        for (int j = 0; j < kPer; ++j) {
+          mine[j] = sh.lo[tid * kPer + j];
+          if (weights) mine[j] += (unsigned long long)sh.hi[tid * kPer + j] << 16;
+        }
+#pragma unroll 4
+        for (int r = 1; r < ranks; ++r)
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            mine[j] += ld_cluster_u32(map_to_rank(&sh.lo[tid * kPer + j], r));
+            if (weights) mine[j] += (unsigned long long)ld_cluster_u32(map_to_rank(&sh.hi[tid * kPer + j], r)) << 16;
+          }
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const uint32_t bin = tid * kPer + j;
+          mine[j] -= fix(c.first + (bin << shift), c.first + ((bin + 1) << shift));
+          sum += mine[j];
+        }
+        unsigned long long upto = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const unsigned long long a = __shfl_up_sync(0xffffffffu, upto, d);
+          if (lane >= d) upto += a;
+        }
+        if (lane == 31) sh.sum[warp] = upto;
+        if (tid == 0) sh.found = 0;
+        __syncthreads();
+        unsigned long long at = c.before + upto - sum;
+        for (int w = 0; w < warp; ++w) at += sh.sum[w];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          if (at < want && at + mine[j] >= want) {
+            sh.bin = tid * kPer + j;
+            sh.before = at;
+            sh.at = mine[j];
+            sh.found = 1;
+          }
+          at += mine[j];
+        }
+        __syncthreads();
+        if (warp == 0 && ranks > 1) {
+          const uint32_t bin = sh.bin, found = sh.found;
+          const unsigned long long before = sh.before, in = sh.at;
+          __syncwarp();
+          tell_u32(&sh.bin, bin);
+          tell_u32(&sh.found, found);
+          tell_u64(&sh.before, before);
+          tell_u64(&sh.at, in);
+        }
+      }
+      everyone();
+      c.found = sh.found != 0;
+      if (!c.found) return c;
+      c.before = sh.before;
+      c.at = sh.at;
+      c.first += sh.bin << shift;
+      c.width = 1u << shift;
+      if (shift == 0 || coarse) return c;
+      span = c.width;
     }
+  };
+  // More than the distance of any logit with z >= cut.
+  auto span_of = [&](float cut) {
+    const float far = cut / inv;
+    const float low = isfinite(most) ? most + far - 1e-5f * (fabsf(most) + fabsf(far)) : -INFINITY;
+    return top_key - min(order_key(low) >> Items::kDrop, top_key) + 2;
+  };
+  auto no_fix = [](uint32_t, uint32_t) { return 0ull; };
+
+  // kept: keys above `thr`, and the first `ties` (in index order) of those equal to it
+  uint32_t thr = 0, ties = 0xffffffffu;
+  unsigned long long tied = 0;  // how many there are
+  bool cut_k = false;
+  if (k == 1) {
+    thr = top_key;
+    ties = 1;
+    cut_k = true;
+  } else if (k < V) {
+    uint32_t span = span_of(kWeightCut);
+    if (k <= ranks * kThreads && V > kSampleDirect) {
+      const float own = key_value(own_top);
+      const Cut c = histogram(k, span, false, true, [&](auto f) { if (near(own, kWeightCut)) f(own); }, no_fix);
+      if (c.found) span = c.first + c.width;
+    }
+    const Cut c = histogram(k, span, false, false, [&](auto f) {
+      x.each([&](int, float v) {
+        if (near(v, kWeightCut)) f(v);
+      });
+    }, no_fix);
+    if (c.found) {
+      thr = top_key - c.first;
+      ties = k - (uint32_t)c.before;
+      tied = c.at;
+      cut_k = true;
+    }
+  }
+  // the logit whose key is `thr`
+  auto value_of = [&](uint32_t key) {
+    const uint32_t full = key << Items::kDrop;
+    return key_value(full & 0x80000000u ? full : full | ((1u << Items::kDrop) - 1));
+  };
+  if (k > 1 && (tp < 1.f || !(tp == tp))) {
+    unsigned long long own = 0;
+    x.each([&](int, float v) {
+      if ((order_key(v) >> Items::kDrop) > thr && near(v, kWeightCut)) own += w_of(v);
+    });
+    const float at_thr = value_of(thr);
+    const unsigned long long w_thr = cut_k ? w_of(at_thr) : 0;
+    const unsigned long long all = total(own) + (cut_k ? ties * w_thr : 0);
     const double lim = (double)tp * (double)all;
     const unsigned long long limit = lim > 1.0 ? (unsigned long long)ceil(lim) : 1ull;
-    __syncthreads();
-    select(true, 0, limit, thr, k < V ? ties : 0);
-    if (s_found) {
-      const unsigned long long w = w_of(s_prefix);
-      const unsigned n = w ? (unsigned)((limit - s_before_w + w - 1) / w) : 0xffffffffu;
-      ties = s_prefix == thr && k < V ? min(ties, n) : n;
-      thr = s_prefix;
+    // weights below this add up to less than what top_p leaves out
+    const float least = 0.99f * (1.f - tp) * (float)all / (float)k;
+    const float cut = least > 1.f ? fmaxf(kWeightCut, logf(least * 4.656612873077393e-10f) - 1e-3f) : kWeightCut;
+    const uint32_t at = top_key - thr;
+    const unsigned long long extra = cut_k && near(at_thr, cut) ? (tied - ties) * w_thr : 0;
+    const Cut c = histogram(limit, span_of(cut), true, false, [&](auto f) {
+      x.each([&](int, float v) {
+        if (near(v, cut) && (order_key(v) >> Items::kDrop) >= thr) f(v);
+      });
+    }, [&](uint32_t from, uint32_t to) { return extra && from <= at && at < to ? extra : 0ull; });
+    if (c.found) {
+      const uint32_t key = top_key - c.first;
+      const unsigned long long w = w_of(value_of(key));
+      const uint32_t n = (uint32_t)min((limit - c.before + w - 1) / w, 0xffffffffull);
+      ties = cut_k && key == thr ? min(ties, n) : n;
+      thr = key;
     }
-    __syncthreads();
   }
 
-  auto kept = [&](uint32_t key) { return key >= thr && (e_of(key) >= mp || key == top); };
-  // Each warp sums a stretch of the row, then the one that holds the target walks it.
-  const int per = ((V + kSampleThreads - 1) / kSampleThreads) * 32;
-  const int i0 = min(warp * per, V), i1 = min(i0 + per, V);
-  unsigned long long ws = 0;
-  unsigned nt = 0;
-  for (int i = i0 + lane; i < i1; i += 32) {
-    const uint32_t key = order_key(to_f32(row[i]));
-    if (!kept(key)) continue;
-    if (key == thr) ++nt;
-    else ws += w_of(key);
-  }
+  // Running sums of the kept weight in index order.
+  const float cut = mp > 0.f ? fmaxf(kWeightCut, logf(mp) - 1e-3f) : kWeightCut;
+  unsigned long long own = 0;
+  uint32_t own_ties = 0;
+  x.each([&](int, float v) {
+    const uint32_t key = order_key(v) >> Items::kDrop;
+    if (key < thr || !near(v, cut)) return;
+    const float e = e_of(v);
+    if (!(e >= mp) && v != most) return;
+    if (key == thr) ++own_ties;
+    else own += (uint32_t)(e * 2147483648.f);
+  });
+  unsigned long long upto = own;
+  uint32_t upto_ties = own_ties;
 #pragma unroll
-  for (int m = 16; m > 0; m >>= 1) {
-    ws += __shfl_xor_sync(0xffffffffu, ws, m);
-    nt += __shfl_xor_sync(0xffffffffu, nt, m);
-  }
-  if (lane == 0) {
-    wsum[warp] = ws;
-    wtie[warp] = nt;
+  for (int d = 1; d < 32; d <<= 1) {
+    const unsigned long long a = __shfl_up_sync(0xffffffffu, upto, d);
+    const uint32_t c = __shfl_up_sync(0xffffffffu, upto_ties, d);
+    if (lane >= d) {
+      upto += a;
+      upto_ties += c;
+    }
   }
   __syncthreads();
-  const unsigned long long wthr = w_of(thr);
-  unsigned long long before = 0, whole = 0, sum_gt = 0;
-  unsigned tie_before = 0, tie_all = 0;
-  for (int w = 0; w < 32; ++w) {
-    if (w == warp) {
-      tie_before = tie_all;
-      before = sum_gt;
-    }
-    tie_all += wtie[w];
-    sum_gt += wsum[w];
+  if (lane == 31) {
+    sh.sum[warp] = upto;
+    sh.num[warp] = upto_ties;
   }
-  whole = sum_gt + (unsigned long long)min(tie_all, ties) * wthr;
-  const unsigned long long at_end = before + ws + (unsigned long long)min(tie_before + nt, ties) * wthr;
-  before += (unsigned long long)min(tie_before, ties) * wthr;
-  const double ud = (double)p.uniforms[b] * (double)whole;
-  unsigned long long target = ud > 0.0 ? (unsigned long long)ud : 0ull;
-  if (target > whole - 1) target = whole - 1;
-  if (before <= target && target < at_end) {
-    for (int i = i0; i < i1; i += 32) {
-      const uint32_t key = i + lane < i1 ? order_key(to_f32(row[i + lane])) : 0;
-      const bool in = i + lane < i1 && kept(key);
-      const bool tie = in && key == thr;
-      const unsigned tm = __ballot_sync(0xffffffffu, tie);
-      const bool take = in && (!tie || tie_before + __popc(tm & ((1u << lane) - 1)) < ties);
-      const unsigned long long own = take ? w_of(key) : 0ull;
-      unsigned long long sum = own;
+  __syncthreads();
+  if (warp == 0) {
+    unsigned long long a = lane < kWarps ? sh.sum[lane] : 0;
+    uint32_t c = lane < kWarps ? sh.num[lane] : 0;
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const unsigned long long a = __shfl_up_sync(0xffffffffu, sum, d);
-        if (lane >= d) sum += a;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, before + sum > target);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) {
-          p.tokens[b] = i + lane;
-          if (p.logprobs) p.logprobs[b] = logf((float)((double)own / (double)whole));
-        }
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, sum, 31);
-      tie_before += __popc(tm);
-    }
+    for (int m = 16; m > 0; m >>= 1) a += __shfl_xor_sync(0xffffffffu, a, m);
+    c = __reduce_add_sync(0xffffffffu, c);
+    tell_u64(&sh.rank_sum[rank], a);
+    tell_u32(&sh.rank_ties[rank], c);
   }
+  everyone();
+  unsigned long long before = upto - own, sum = 0;
+  unsigned long long ties_before = upto_ties - own_ties, ties_all = 0;
+  for (int w = 0; w < warp; ++w) {
+    before += sh.sum[w];
+    ties_before += sh.num[w];
+  }
+  for (int r = 0; r < ranks; ++r) {
+    if (r < rank) {
+      before += sh.rank_sum[r];
+      ties_before += sh.rank_ties[r];
+    }
+    sum += sh.rank_sum[r];
+    ties_all += sh.rank_ties[r];
+  }
+  const unsigned long long w_thr = ties_all ? w_of(value_of(thr)) : 0, most_ties = ties;
+  const unsigned long long whole = sum + min(ties_all, most_ties) * w_thr;
+  const unsigned long long end = before + own + min(ties_before + own_ties, most_ties) * w_thr;
+  before += min(ties_before, most_ties) * w_thr;
+  const double ud = (double)u * (double)whole;
+  unsigned long long target = ud > 0.0 ? (unsigned long long)ud : 0ull;
+  target = min(target, whole - 1);
+  if (before <= target && target < end) {  // this thread holds the token
+    int chosen = -1;
+    uint32_t weight = 0;
+    x.each([&](int i, float v) {
+      const uint32_t key = order_key(v) >> Items::kDrop;
+      if (chosen >= 0 || key < thr || !near(v, cut)) return;
+      const float e = e_of(v);
+      if (!(e >= mp) && v != most) return;
+      if (key == thr && ties_before++ >= most_ties) return;
+      weight = (uint32_t)(e * 2147483648.f);
+      before += weight;
+      if (before > target) chosen = i;
+    });
+    p.tokens[b] = base + chosen;
+    if (p.logprobs) p.logprobs[b] = logf((float)((double)weight / (double)whole));
+  }
+}
+
+// Threads per CTA and CTAs per row: as few CTAs as hold the row, so that a row
+// of up to 32768 logits needs no barrier across CTAs; smaller CTAs, two to an
+// SM, where a row takes a cluster anyway.
+template <typename T>
+int launch_sample(const SampleArgs& a, int rows, cudaStream_t stream) {
+  // and what lies between a row's start and the 16-byte boundary below it
+  const int skew = (a.row_stride * sizeof(T)) % 16 == 0 || rows == 1
+                       ? (int)((reinterpret_cast<uintptr_t>(a.logits) & 15) / sizeof(T))
+                       : SampleRow<T>::kVec - 1;
+  const int n = a.vocab + skew;
+  const bool small = n <= 512 * kSampleItems, wide = n > 8 * 512 * kSampleItems || (!small && n <= 1024 * kSampleItems);
+  const int threads = wide ? 1024 : 512;
+  int ranks = 1;
+  while (ranks * threads * kSampleItems < n) ranks *= 2;
+  auto kernel = wide ? sample_kernel<T, 1024> : sample_kernel<T, 512>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(rows * ranks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = (size_t)threads * kSampleItems * sizeof(T);
+  cfg.stream = stream;
+  const DeviceInfo* dev = nullptr;
+  const int st = device_info(&dev);
+  if (st != GDSQ_OK) return st;
+  cudaError_t e = ensure_smem(kernel, (int)(cfg.dynamicSmemBytes + sizeof(SampleShared)), dev->ordinal);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(sample)");
+  cudaLaunchAttribute attr[2];
+  int n_attr = 0;
+  if (ranks > 1) {
+    attr[n_attr].id = cudaLaunchAttributeClusterDimension;
+    attr[n_attr].val.clusterDim.x = ranks;
+    attr[n_attr].val.clusterDim.y = 1;
+    attr[n_attr].val.clusterDim.z = 1;
+    ++n_attr;
+  }
+  if (g_pdl_enabled) {
+    attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n_attr].val.programmaticStreamSerializationAllowed = 1;
+    ++n_attr;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n_attr;
+  if (ranks > 8) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(sample)");
+  }
+  e = cudaLaunchKernelEx(&cfg, kernel, a, ranks);
+  return e == cudaSuccess ? GDSQ_OK : cuda_fail(e, "sample launch");
 }
 
 }  // namespace
@@ -678,12 +950,10 @@ int gdsq_sample(int elem_type, const void* logits, long long row_stride, int num
       !aligned(top_k, 4) || !aligned(top_p, 4) || !aligned(min_p, 4) || !aligned(tokens, 8) || !aligned(logprobs, 4))
     return fail(GDSQ_ERR_MISALIGNED, "sample: logits to their own size, tokens 8-byte, the rest 4-byte alignment");
   const SampleArgs a = {logits, row_stride, uniforms, temperature, top_k, top_p, min_p, tokens, logprobs, vocab};
-  auto kernel = elem_type == GDSQ_ELEM_F16    ? sample_simple_kernel<__half>
-                : elem_type == GDSQ_ELEM_BF16 ? sample_simple_kernel<__nv_bfloat16>
-                                              : sample_simple_kernel<float>;
-  cudaError_t e = launch(kernel, dim3(num_rows), dim3(kSampleThreads), 0, static_cast<cudaStream_t>(stream_v),
-                         g_pdl_enabled != 0, a);
-  return e == cudaSuccess ? GDSQ_OK : cuda_fail(e, "sample launch");
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  if (elem_type == GDSQ_ELEM_F16) return launch_sample<__half>(a, num_rows, stream);
+  if (elem_type == GDSQ_ELEM_BF16) return launch_sample<__nv_bfloat16>(a, num_rows, stream);
+  return launch_sample<float>(a, num_rows, stream);
 }
 
 }  // extern "C"
