@@ -332,19 +332,24 @@ __global__ void __launch_bounds__(kAppThreads) append_kv8_kernel(const AppendArg
 // the 32 logits from 32 i (counted from the 16-byte boundary below the row), so
 // that index order is thread order, and the logits are read once.  The work is
 // one exponential per logit where the whole weight is needed (no filter, or
-// top-p alone), else one per token that can be kept.
+// top-p alone), else a comparison.
+//
+// With filters few tokens can be kept, and those that can are copied to one
+// CTA's list, which chooses alone while the others leave:
+//   top_k   each CTA finds a value that ceil(k / CTAs) of its threads' maxima
+//           reach; k logits of the row reach the lowest of these values
+//   top_p   tokens of weight below (1 - p) W / V cannot add up to what is left out
+//   min_p   the value itself
+//   any     a token of weight 0 never matters
+// A longer list than fits is worked on where it lies, by all of them.
 //
 // A cut (top_k by count, top_p by weight) is found by histograms over the
 // distance of a logit's ordered bit pattern from the maximum's: 2048 bins over
 // the span of the candidates, then 2048 inside the bin where the cut falls,
 // until a bin is one logit value; ties then follow from counts alone.
-// Candidates are few: a token of weight 0 never matters; one below the k-th
-// largest of the threads' own maxima is not among the top k; tokens of weight
-// below (1 - p) W / V cannot add up to the part that top-p removes.
 
 constexpr int kSampleItems = 32;  // logits per thread
 constexpr int kSampleBins = 2048;
-constexpr int kSampleDirect = 8192;  // rows up to here go into the top-k histogram whole
 constexpr float kWeightCut = -21.6f;  // floor(2^31 exp(z)) = 0 below (ln 2^-31 = -21.49)
 
 struct SampleArgs {
@@ -384,7 +389,9 @@ struct SampleRow {
   static __device__ __forceinline__ uint32_t place(uint32_t v) { return (v ^ ((v >> 3) & (kVecs - 1))) << 4; }
 
   // Vectors first .. of the row, counted from the 16-byte boundary at or below its start; what lies outside becomes -inf.
-  __device__ __forceinline__ void load(const T* row, int skew, int first, int vocab, int threads) const {
+  // Returns the largest of what this thread loaded, NaN aside.
+  __device__ __forceinline__ float load(const T* row, int skew, int first, int vocab, int threads) const {
+    float most = -INFINITY;
     constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) {
@@ -401,6 +408,31 @@ struct SampleRow {
       }
       asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + place(v)), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
                    : "memory");
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = fmaxf(most, __uint_as_float(w[e]));
+      } else {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        T2 m[4];
+        memcpy(m, w, 16);
+        m[0] = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
+        most = fmaxf(most, fmaxf(to_f32(m[0].x), to_f32(m[0].y)));
+      }
+    }
+    return most;
+  }
+
+  __device__ __forceinline__ float get(int i) const {  // this thread's i-th
+    const uint32_t a = at + place(threadIdx.x * kVecs + i / kVec) + (i % kVec) * (uint32_t)sizeof(T);
+    if constexpr (sizeof(T) == 4) {
+      return lds32f(a);
+    } else {
+      unsigned short v;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+      T x;
+      memcpy(&x, &v, 2);
+      return to_f32(x);
     }
   }
 
@@ -430,6 +462,8 @@ struct SampleShared {
   uint32_t num[32];
   // by cluster rank, each written once
   uint32_t rank_top[16];
+  uint32_t rank_bound[16];
+  uint32_t rank_count[16];
   unsigned long long rank_total[16];
   unsigned long long rank_sum[16];
   uint32_t rank_ties[16];
@@ -438,6 +472,10 @@ struct SampleShared {
   uint32_t found;
   unsigned long long before, at;
 };
+
+// Tokens that the list of one CTA holds.
+template <typename T>
+constexpr int kSampleList = sizeof(T) == 4 ? 2048 : 4096;
 
 // Grid: one cluster per row.
 template <typename T, int kThreads>
@@ -450,22 +488,24 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   const int rank = ranks > 1 ? (int)(blockIdx.x % ranks) : 0;
   const int b = blockIdx.x / ranks;
   const int V = p.vocab;
+  int team = ranks;   // CTAs that work on the row: all of them, or the first alone
+  bool solo = false;  // on the list
   auto everyone = [&] {
-    if (ranks > 1) cluster_sync_all();
+    if (team > 1) cluster_sync_all();
     else __syncthreads();
   };
   // Stores `v` to *slot in every CTA of the cluster; one warp calls it.
   auto tell_u64 = [&](unsigned long long* slot, unsigned long long v) {
-    if (ranks == 1) {
+    if (team == 1) {
       if (lane == 0) *slot = v;
-    } else if (lane < ranks) {
+    } else if (lane < team) {
       st_cluster_u64(map_to_rank(slot, lane), v);
     }
   };
   auto tell_u32 = [&](uint32_t* slot, uint32_t v) {
-    if (ranks == 1) {
+    if (team == 1) {
       if (lane == 0) *slot = v;
-    } else if (lane < ranks) {
+    } else if (lane < team) {
       st_cluster_u32(map_to_rank(slot, lane), v);
     }
   };
@@ -483,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     }
     everyone();
     v = 0;
-    for (int r = 0; r < ranks; ++r) v += sh.rank_total[r];
+    for (int r = 0; r < team; ++r) v += sh.rank_total[r];
     return v;
   };
 
@@ -494,7 +534,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   const int skew = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
   const int base = (rank * kThreads + tid) * kSampleItems - skew;  // index of this thread's first logit
   const Items x{smem_addr(logits_smem)};
-  x.load(row, skew, rank * kThreads * Items::kVecs, V, kThreads);
+  const float own_most = x.load(row, skew, rank * kThreads * Items::kVecs, V, kThreads);
+  uint32_t* list_value = reinterpret_cast<uint32_t*>(logits_smem + kThreads * kSampleItems * sizeof(T));
+  int* list_index = reinterpret_cast<int*>(list_value + kSampleList<T>);
   const float temp = p.temperature ? p.temperature[b] : 1.f;
   const bool greedy = !(temp > 0.f);
   const float inv = greedy ? 1.f : __frcp_rn(temp);
@@ -505,18 +547,58 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   if (greedy || mp > 1.f || !(mp == mp)) k = 1;  // min_p above 1: nothing but the first passes
   if (k <= 0 || k > V) k = V;
 
-  // the maximum
-  uint32_t own_top = 0;
-  __syncthreads();
-  x.each([&](int, float v) { own_top = max(own_top, order_key(v)); });
+  // The maximum, and for top_k a value that `share` of this CTA's threads' maxima reach.
+  const uint32_t own_top = order_key(own_most);
+  const int share = (k + ranks - 1) / ranks;
+  const bool by_count = k > 1 && k < V;
   {
-    const uint32_t t = __reduce_max_sync(0xffffffffu, own_top);
-    if (lane == 0) sh.num[warp] = t;
+    const uint32_t w = __reduce_max_sync(0xffffffffu, own_top);
+    if (lane == 0) sh.num[warp] = w;
+    if (by_count && share <= kThreads)
+      for (int i = tid; i < kSampleBins; i += kThreads) sh.lo[i] = 0;
+    if (tid == 0) sh.found = 0;
     __syncthreads();
+    const uint32_t cta_top = __reduce_max_sync(0xffffffffu, lane < kWarps ? sh.num[lane] : 0);
+    float bound = -INFINITY;
+    if (by_count && share <= kThreads) {
+      // bins of equal width in the logit, down to where weights vanish
+      const float high = key_value(cta_top), width = -kWeightCut / inv / kSampleBins;
+      const float d = (high - own_most) / width;
+      if (d < (float)kSampleBins) atomicAdd(&sh.lo[(int)d], 1u);
+      __syncthreads();
+      constexpr int kPer = kSampleBins / kThreads;
+      uint32_t n[kPer], sum = 0;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) sum += n[j] = sh.lo[tid * kPer + j];
+      uint32_t upto = sum;
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) {
+        const uint32_t a = __shfl_up_sync(0xffffffffu, upto, s);
+        if (lane >= s) upto += a;
+      }
+      if (lane == 31) sh.num[warp] = upto;
+      __syncthreads();
+      uint32_t at = upto - sum;
+      for (int w2 = 0; w2 < warp; ++w2) at += sh.num[w2];
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        if (at < (uint32_t)share && at + n[j] >= (uint32_t)share) {
+          sh.bin = tid * kPer + j;
+          sh.found = 1;
+        }
+        at += n[j];
+      }
+      __syncthreads();
+      if (sh.found) {
+        const float far = (float)(sh.bin + 1) * width;
+        bound = high - far - 1e-5f * (fabsf(high) + far);
+        if (!(bound == bound)) bound = -INFINITY;
+      }
+    }
     if (ranks > 1) cluster_wait();
     if (warp == 0) {
-      const uint32_t t2 = __reduce_max_sync(0xffffffffu, lane < kWarps ? sh.num[lane] : 0);
-      tell_u32(&sh.rank_top[rank], t2);
+      tell_u32(&sh.rank_top[rank], cta_top);
+      tell_u32(&sh.rank_bound[rank], order_key(bound));
     }
     everyone();
   }
@@ -536,20 +618,18 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   auto near = [&](float v, float cut) { return v == most || z_of(v) >= cut; };
 
 
-  // Where the running sum over falling logits reaches `want`: all shares of values
-  // at distances [first, first + width) from the maximum, with `before` the sum over
-  // nearer ones and `at` the sum in it.  each(f) calls f(logit) for the candidates,
+  // The value where the running sum over falling logits reaches `want`: its distance
+  // `first` from the maximum, `before` the sum over nearer ones, `at` the value's own.  each(f) calls f(logit) for the candidates,
   // which lie at distances below `span`; their share is their weight, or 1.
-  // fix(from, to) is taken off the sum of the distances [from, to).  `coarse`
-  // stops at a bin, else width is 1: one logit value.
+  // fix(from, to) is taken off the sum of the distances [from, to).
   struct Cut {
-    uint32_t first, width;
+    uint32_t first;
     unsigned long long before, at;
     bool found;
   };
   const uint32_t top_key = top >> Items::kDrop;
-  auto histogram = [&](unsigned long long want, uint32_t span, bool weights, bool coarse, auto each, auto fix) {
-    Cut c{0, 0, 0, 0, true};
+  auto histogram = [&](unsigned long long want, uint32_t span, bool weights, auto each, auto fix) {
+    Cut c{0, 0, 0, true};
     for (;;) {
       const int shift = max(0, 21 - __clz(span - 1));  // span <= 2048 << shift
       for (int i = tid; i < kSampleBins; i += kThreads) {
@@ -578,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
           if (weights) mine[j] += (unsigned long long)sh.hi[tid * kPer + j] << 16;
         }
 #pragma unroll 4
-        for (int r = 1; r < ranks; ++r)
+        for (int r = 1; r < team; ++r)
 #pragma unroll
           for (int j = 0; j < kPer; ++j) {
             mine[j] += ld_cluster_u32(map_to_rank(&sh.lo[tid * kPer + j], r));
@@ -612,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
           at += mine[j];
         }
         __syncthreads();
-        if (warp == 0 && ranks > 1) {
+        if (warp == 0 && team > 1) {
           const uint32_t bin = sh.bin, found = sh.found;
           const unsigned long long before = sh.before, in = sh.at;
           __syncwarp();
@@ -628,18 +708,99 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       c.before = sh.before;
       c.at = sh.at;
       c.first += sh.bin << shift;
-      c.width = 1u << shift;
-      if (shift == 0 || coarse) return c;
-      span = c.width;
+      if (shift == 0) return c;
+      span = 1u << shift;
     }
   };
-  // More than the distance of any logit with z >= cut.
-  auto span_of = [&](float cut) {
+  // Not above any logit with z >= cut.
+  auto low_of = [&](float cut) {
     const float far = cut / inv;
-    const float low = isfinite(most) ? most + far - 1e-5f * (fabsf(most) + fabsf(far)) : -INFINITY;
-    return top_key - min(order_key(low) >> Items::kDrop, top_key) + 2;
+    return isfinite(most) ? most + far - 1e-5f * (fabsf(most) + fabsf(far)) : -INFINITY;
   };
+  // More than the distance of any logit that is at least `low`.
+  auto span_of = [&](float low) { return top_key - min(order_key(low) >> Items::kDrop, top_key) + 2; };
   auto no_fix = [](uint32_t, uint32_t) { return 0ull; };
+  const bool by_weight = k > 1 && (tp < 1.f || !(tp == tp));
+  const float min_cut = mp > 0.f ? fmaxf(kWeightCut, logf(mp) - 1e-3f) : kWeightCut;
+  auto limit_of = [&](unsigned long long all) {
+    const double lim = (double)tp * (double)all;
+    return lim > 1.0 ? (unsigned long long)ceil(lim) : 1ull;
+  };
+
+  // No candidate lies below `low`; the list.
+  float low = low_of(kWeightCut);
+  unsigned long long all = 0;
+  if (by_count) {
+    uint32_t bound = 0xffffffffu;
+    for (int r = 0; r < ranks; ++r) bound = min(bound, sh.rank_bound[r]);
+    low = fmaxf(low, key_value(bound));
+    if (!by_weight) low = fmaxf(low, low_of(min_cut));
+  } else if (by_weight) {
+    unsigned long long own = 0;
+    x.each([&](int, float v) {
+      if (near(v, kWeightCut)) own += w_of(v);
+    });
+    all = total(own);
+    const float least = 0.99f * (1.f - tp) * (float)all / (float)V;
+    if (least > 1.f) low = fmaxf(low, low_of(logf(least * 4.656612873077393e-10f) - 1e-3f));
+    low = fmaxf(low, low_of(min_cut));
+  } else if (k > 1) {
+    low = fmaxf(low, low_of(min_cut));
+  }
+  int list = 0;
+  if (by_count || by_weight || (k > 1 && mp > 0.f)) {
+    uint32_t mask = 0;
+    x.each([&](int i, float v) { mask |= (uint32_t)(v >= low) << i; });
+    const int n = __popc(mask);
+    int upto = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += a;
+    }
+    __syncthreads();
+    if (lane == 31) sh.num[warp] = upto;
+    __syncthreads();
+    if (warp == 0) {
+      const uint32_t c = __reduce_add_sync(0xffffffffu, lane < kWarps ? sh.num[lane] : 0);
+      tell_u32(&sh.rank_count[rank], c);
+    }
+    everyone();
+    int at = upto - n;
+    for (int w = 0; w < warp; ++w) at += sh.num[w];
+    for (int r = 0; r < ranks; ++r) {
+      if (r < rank) at += sh.rank_count[r];
+      list += sh.rank_count[r];
+    }
+    if (list <= kSampleList<T>) {
+      for (; mask; mask &= mask - 1, ++at) {
+        const int i = __ffs(mask) - 1;
+        const uint32_t v = __float_as_uint(x.get(i));
+        if (ranks == 1) {
+          list_value[at] = v;
+          list_index[at] = base + i;
+        } else {
+          st_cluster_u32(map_to_rank(list_value + at, 0), v);
+          st_cluster_u32(map_to_rank(list_index + at, 0), (uint32_t)(base + i));
+        }
+      }
+      everyone();
+      if (rank != 0) return;
+      solo = true;
+      team = 1;
+    }
+  }
+  // fn(i, logit) for the candidates of this thread: a stretch of the list, or its own logits.
+  const int list_per = (list + kThreads - 1) / kThreads, list_at = min(tid * list_per, list), list_end = min(list_at + list_per, list);
+  auto walk = [&](auto fn) {
+    if (solo) {
+      for (int i = list_at; i < list_end; ++i) fn(i - list_at, __uint_as_float(list_value[i]));
+    } else {
+      x.each([&](int i, float v) {
+        if (v >= low) fn(i, v);
+      });
+    }
+  };
 
   // kept: keys above `thr`, and the first `ties` (in index order) of those equal to it
   uint32_t thr = 0, ties = 0xffffffffu;
@@ -649,15 +810,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     thr = top_key;
     ties = 1;
     cut_k = true;
-  } else if (k < V) {
-    uint32_t span = span_of(kWeightCut);
-    if (k <= ranks * kThreads && V > kSampleDirect) {
-      const float own = key_value(own_top);
-      const Cut c = histogram(k, span, false, true, [&](auto f) { if (near(own, kWeightCut)) f(own); }, no_fix);
-      if (c.found) span = c.first + c.width;
-    }
-    const Cut c = histogram(k, span, false, false, [&](auto f) {
-      x.each([&](int, float v) {
+  } else if (by_count) {
+    const Cut c = histogram(k, span_of(low), false, [&](auto f) {
+      walk([&](int, float v) {
         if (near(v, kWeightCut)) f(v);
       });
     }, no_fix);
@@ -673,26 +828,26 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     const uint32_t full = key << Items::kDrop;
     return key_value(full & 0x80000000u ? full : full | ((1u << Items::kDrop) - 1));
   };
-  if (k > 1 && (tp < 1.f || !(tp == tp))) {
-    unsigned long long own = 0;
-    x.each([&](int, float v) {
-      if ((order_key(v) >> Items::kDrop) > thr && near(v, kWeightCut)) own += w_of(v);
-    });
+  if (by_weight) {
     const float at_thr = value_of(thr);
     const unsigned long long w_thr = cut_k ? w_of(at_thr) : 0;
-    const unsigned long long all = total(own) + (cut_k ? ties * w_thr : 0);
-    const double lim = (double)tp * (double)all;
-    const unsigned long long limit = lim > 1.0 ? (unsigned long long)ceil(lim) : 1ull;
-    // weights below this add up to less than what top_p leaves out
-    const float least = 0.99f * (1.f - tp) * (float)all / (float)k;
-    const float cut = least > 1.f ? fmaxf(kWeightCut, logf(least * 4.656612873077393e-10f) - 1e-3f) : kWeightCut;
-    const uint32_t at = top_key - thr;
-    const unsigned long long extra = cut_k && near(at_thr, cut) ? (tied - ties) * w_thr : 0;
-    const Cut c = histogram(limit, span_of(cut), true, false, [&](auto f) {
-      x.each([&](int, float v) {
-        if (near(v, cut) && (order_key(v) >> Items::kDrop) >= thr) f(v);
+    float from = low;
+    if (by_count) {
+      unsigned long long own = 0;
+      walk([&](int, float v) {
+        if ((order_key(v) >> Items::kDrop) > thr && near(v, kWeightCut)) own += w_of(v);
       });
-    }, [&](uint32_t from, uint32_t to) { return extra && from <= at && at < to ? extra : 0ull; });
+      all = total(own) + (cut_k ? ties * w_thr : 0);
+      if (cut_k) from = at_thr;
+    }
+    const unsigned long long limit = limit_of(all);
+    const uint32_t at = top_key - thr;
+    const unsigned long long extra = cut_k && near(at_thr, kWeightCut) ? (tied - ties) * w_thr : 0;
+    const Cut c = histogram(limit, span_of(from), true, [&](auto f) {
+      walk([&](int, float v) {
+        if (v >= from && near(v, kWeightCut)) f(v);
+      });
+    }, [&](uint32_t lo, uint32_t hi) { return extra && lo <= at && at < hi ? extra : 0ull; });
     if (c.found) {
       const uint32_t key = top_key - c.first;
       const unsigned long long w = w_of(value_of(key));
@@ -703,12 +858,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   }
 
   // Running sums of the kept weight in index order.
-  const float cut = mp > 0.f ? fmaxf(kWeightCut, logf(mp) - 1e-3f) : kWeightCut;
   unsigned long long own = 0;
   uint32_t own_ties = 0;
-  x.each([&](int, float v) {
+  walk([&](int, float v) {
     const uint32_t key = order_key(v) >> Items::kDrop;
-    if (key < thr || !near(v, cut)) return;
+    if (key < thr || !near(v, min_cut)) return;
     const float e = e_of(v);
     if (!(e >= mp) && v != most) return;
     if (key == thr) ++own_ties;
@@ -747,7 +901,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     before += sh.sum[w];
     ties_before += sh.num[w];
   }
-  for (int r = 0; r < ranks; ++r) {
+  for (int r = 0; r < team; ++r) {
     if (r < rank) {
       before += sh.rank_sum[r];
       ties_before += sh.rank_ties[r];
@@ -765,9 +919,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   if (before <= target && target < end) {  // this thread holds the token
     int chosen = -1;
     uint32_t weight = 0;
-    x.each([&](int i, float v) {
+    walk([&](int i, float v) {
       const uint32_t key = order_key(v) >> Items::kDrop;
-      if (chosen >= 0 || key < thr || !near(v, cut)) return;
+      if (chosen >= 0 || key < thr || !near(v, min_cut)) return;
       const float e = e_of(v);
       if (!(e >= mp) && v != most) return;
       if (key == thr && ties_before++ >= most_ties) return;
@@ -775,7 +929,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       before += weight;
       if (before > target) chosen = i;
     });
-    p.tokens[b] = base + chosen;
+    p.tokens[b] = solo ? list_index[list_at + chosen] : base + chosen;
     if (p.logprobs) p.logprobs[b] = logf((float)((double)weight / (double)whole));
   }
 }
@@ -798,7 +952,7 @@ int launch_sample(const SampleArgs& a, int rows, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(rows * ranks);
   cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = (size_t)threads * kSampleItems * sizeof(T);
+  cfg.dynamicSmemBytes = (size_t)threads * kSampleItems * sizeof(T) + (size_t)kSampleList<T> * 8;
   cfg.stream = stream;
   const DeviceInfo* dev = nullptr;
   const int st = device_info(&dev);
