@@ -346,10 +346,12 @@ __global__ void __launch_bounds__(kAppThreads) append_kv8_kernel(const AppendArg
 // A cut (top_k by count, top_p by weight) is found by histograms over the
 // distance of a logit's ordered bit pattern from the maximum's: 2048 bins over
 // the span of the candidates, then 2048 inside the bin where the cut falls,
-// until a bin is one logit value; ties then follow from counts alone.
+// until a bin is one logit value; ties then follow from counts alone.  A list
+// of up to 256 is ordered by comparing all pairs instead, in one pass.
 
 constexpr int kSampleItems = 32;  // logits per thread
 constexpr int kSampleBins = 2048;
+constexpr int kSampleShort = 256;  // lists up to here are ordered by comparing all pairs
 constexpr float kWeightCut = -21.6f;  // floor(2^31 exp(z)) = 0 below (ln 2^-31 = -21.49)
 
 struct SampleArgs {
@@ -456,8 +458,8 @@ struct SampleRow {
 };
 
 struct SampleShared {
-  uint32_t lo[kSampleBins];  // counts, or low halves of weights
-  uint32_t hi[kSampleBins];  // high halves of weights
+  alignas(16) uint32_t lo[kSampleBins];  // counts, or low halves of weights
+  alignas(16) uint32_t hi[kSampleBins];  // high halves of weights
   unsigned long long sum[32];
   uint32_t num[32];
   // by cluster rank, each written once
@@ -618,6 +620,20 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   auto near = [&](float v, float cut) { return v == most || z_of(v) >= cut; };
 
 
+  // This thread's whole weight.  Where the maximum and 1 / T are finite, the plain formula gives 1 at the maximum and 0 for -inf
+  // and NaN by itself.
+  const bool regular = isfinite(most) && isfinite(inv);
+  auto own_weight = [&] {
+    unsigned long long sum = 0;
+    if (regular)
+      x.each([&](int, float v) { sum += (uint32_t)(expf(z_of(v)) * 2147483648.f); });
+    else
+      x.each([&](int, float v) {
+        if (near(v, kWeightCut)) sum += w_of(v);
+      });
+    return sum;
+  };
+
   // The value where the running sum over falling logits reaches `want`: its distance
   // `first` from the maximum, `before` the sum over nearer ones, `at` the value's own.  each(f) calls f(logit) for the candidates,
   // which lie at distances below `span`; their share is their weight, or 1.
@@ -727,6 +743,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     return lim > 1.0 ? (unsigned long long)ceil(lim) : 1ull;
   };
 
+  auto target_of = [&](unsigned long long whole) {
+    const double d = (double)u * (double)whole;
+    return min(d > 0.0 ? (unsigned long long)d : 0ull, whole - 1);
+  };
+
   // No candidate lies below `low`; the list.
   float low = low_of(kWeightCut);
   unsigned long long all = 0;
@@ -736,11 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     low = fmaxf(low, key_value(bound));
     if (!by_weight) low = fmaxf(low, low_of(min_cut));
   } else if (by_weight) {
-    unsigned long long own = 0;
-    x.each([&](int, float v) {
-      if (near(v, kWeightCut)) own += w_of(v);
-    });
-    all = total(own);
+    all = total(own_weight());
     const float least = 0.99f * (1.f - tp) * (float)all / (float)V;
     if (least > 1.f) low = fmaxf(low, low_of(logf(least * 4.656612873077393e-10f) - 1e-3f));
     low = fmaxf(low, low_of(min_cut));
@@ -789,6 +806,69 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       solo = true;
       team = 1;
     }
+  }
+  // A short list: one thread per candidate compares it with all others, which gives its place and the weight before it at once.
+  if (solo && list <= kSampleShort) {
+    const bool live = tid < list;
+    const float v = live ? __uint_as_float(list_value[tid]) : -INFINITY;
+    const uint32_t key = order_key(v);
+    const float e = live ? e_of(v) : 0.f;
+    const uint32_t w = (uint32_t)(e * 2147483648.f);
+    if (tid < kSampleShort) {
+      sh.lo[tid] = live ? key : 0;
+      sh.hi[tid] = w;
+    }
+    __syncthreads();
+    uint32_t place = 0;
+    unsigned long long ahead = 0;
+    if (warp * 32 < list) {
+      const uint32_t keys = smem_addr(sh.lo), weights = smem_addr(sh.hi);
+      for (int j = 0; j < list; j += 4) {
+        const uint4 kj = lds128(keys + 4 * j), wj = lds128(weights + 4 * j);
+        const uint32_t kk[4] = {kj.x, kj.y, kj.z, kj.w}, ww[4] = {wj.x, wj.y, wj.z, wj.w};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const bool first = kk[y] > key || (kk[y] == key && j + y < tid);
+          place += first;
+          ahead += first ? ww[y] : 0;
+        }
+      }
+    }
+    auto block_sum = [&](unsigned long long s) {
+#pragma unroll
+      for (int m = 16; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+      if (lane == 0) sh.sum[warp] = s;
+      __syncthreads();
+      s = 0;
+      for (int i = 0; i < kSampleShort / 32; ++i) s += sh.sum[i];
+      return s;
+    };
+    bool keep = live && place < (uint32_t)k;
+    if (by_weight) {
+      if (by_count) all = block_sum(keep ? w : 0);
+      keep = keep && ahead < limit_of(all);
+    }
+    keep = keep && (e >= mp || place == 0);
+    unsigned long long upto = keep ? w : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned long long a = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += a;
+    }
+    __syncthreads();
+    if (lane == 31) sh.sum[warp] = upto;
+    __syncthreads();
+    unsigned long long whole = 0;
+    for (int i = 0; i < kSampleShort / 32; ++i) {
+      if (i < warp) upto += sh.sum[i];
+      whole += sh.sum[i];
+    }
+    const unsigned long long target = target_of(whole);
+    if (keep && upto - w <= target && target < upto) {
+      p.tokens[b] = list_index[tid];
+      if (p.logprobs) p.logprobs[b] = logf((float)((double)w / (double)whole));
+    }
+    return;
   }
   // fn(i, logit) for the candidates of this thread: a stretch of the list, or its own logits.
   const int list_per = (list + kThreads - 1) / kThreads, list_at = min(tid * list_per, list), list_end = min(list_at + list_per, list);
@@ -860,14 +940,17 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   // Running sums of the kept weight in index order.
   unsigned long long own = 0;
   uint32_t own_ties = 0;
-  walk([&](int, float v) {
-    const uint32_t key = order_key(v) >> Items::kDrop;
-    if (key < thr || !near(v, min_cut)) return;
-    const float e = e_of(v);
-    if (!(e >= mp) && v != most) return;
-    if (key == thr) ++own_ties;
-    else own += (uint32_t)(e * 2147483648.f);
-  });
+  if (thr == 0 && !(mp > 0.f) && !solo)
+    own = own_weight();
+  else
+    walk([&](int, float v) {
+      const uint32_t key = order_key(v) >> Items::kDrop;
+      if (key < thr || !near(v, min_cut)) return;
+      const float e = e_of(v);
+      if (!(e >= mp) && v != most) return;
+      if (key == thr) ++own_ties;
+      else own += (uint32_t)(e * 2147483648.f);
+    });
   unsigned long long upto = own;
   uint32_t upto_ties = own_ties;
 #pragma unroll
@@ -913,9 +996,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   const unsigned long long whole = sum + min(ties_all, most_ties) * w_thr;
   const unsigned long long end = before + own + min(ties_before + own_ties, most_ties) * w_thr;
   before += min(ties_before, most_ties) * w_thr;
-  const double ud = (double)u * (double)whole;
-  unsigned long long target = ud > 0.0 ? (unsigned long long)ud : 0ull;
-  target = min(target, whole - 1);
+  const unsigned long long target = target_of(whole);
   if (before <= target && target < end) {  // this thread holds the token
     int chosen = -1;
     uint32_t weight = 0;
