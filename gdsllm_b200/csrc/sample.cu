@@ -645,6 +645,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs p,
 
   // 3: the kept weight of every block, apart from that of ties
   const bool all_of = thr == 0 && !(mp > 0.f);
+  const float edge = thr ? value_of(thr) : low_of(min_cut);  // no filter but min_p: below every kept logit, so equal to none
   x.each([&](int blk, const uint32_t(&w)[kWords]) {
     unsigned long long sum = 0;
     uint32_t tied = 0;
@@ -652,14 +653,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs p,
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum += w_of(Row::get(w, e));
     } else {
+      // thr is the key of `edge`, whose weight is not 0
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float v = Row::get(w, e);
-        const uint32_t key = order_key(v) >> kDrop;
-        if (key < thr || !near(v, min_cut)) continue;
+        if (v < edge) continue;
         const float x1 = e_of(v);
         if (!(x1 >= mp) && v != most) continue;
-        if (key == thr) ++tied;
+        if (v == edge) ++tied;
         else sum += (uint32_t)(x1 * kOne);
       }
     }
@@ -746,13 +747,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs p,
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float v = Row::get(w, e);
-    const uint32_t key = order_key(v) >> kDrop;
     weight[e] = 0;
-    if (key < thr || !near(v, min_cut)) continue;
+    if (v < edge) continue;
     const float x1 = e_of(v);
     if (!(x1 >= mp) && v != most) continue;
     weight[e] = (uint32_t)(x1 * kOne);
-    if (key == thr) {
+    if (v == edge) {
       is_tie |= 1u << e;
       ++tied;
     } else {
