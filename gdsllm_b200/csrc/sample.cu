@@ -49,7 +49,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBlock = 256;        // logits: 8 per lane
 constexpr int kMaxBlocks = 1024;   // per CTA
 constexpr int kBins = 2048;
-constexpr int kPerThread = kBins / kThreads;
+constexpr int kPerThread = kBins / kThreads;  // a 16-byte vector
+static_assert(kPerThread == 4, "bins are read by vectors");
 constexpr int kList = 2048;
 constexpr int kShort = 256;
 constexpr float kWeightCut = -21.6f;  // floor(2^31 exp(z)) = 0 below (ln 2^-31 = -21.49)
@@ -161,10 +162,7 @@ struct SampleShared {
   // a scan's answer
   uint32_t bin, found;
   unsigned long long before, at, all;
-  // the list's length; the block that holds the target, and the sums before it
-  int count, hit;
-  unsigned long long hit_before;
-  uint32_t hit_ties;
+  int count;  // the list's length
 };
 
 // Grid: one cluster of `ranks` CTAs per row.
@@ -301,8 +299,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs p,
   const bool regular = isfinite(most) && isfinite(inv);
   auto z_of = [&](float v) { return __fmul_rn(v - most, inv); };
   auto e_of = [&](float v) {
-    const float e = expf(z_of(v));
-    return regular ? e : v == most ? 1.f : v < most ? e : 0.f;
+    float e = expf(z_of(v));
+    if (!regular) e = v == most ? 1.f : v < most ? e : 0.f;
+    return e;
   };
   auto w_of = [&](float v) { return (uint32_t)(e_of(v) * kOne); };
   auto near = [&](float v, float cut) { return v == most || z_of(v) >= cut; };
@@ -341,13 +340,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs p,
         mine[j] = sh.lo[tid * kPerThread + j];
         if (weights) mine[j] += (unsigned long long)sh.hi[tid * kPerThread + j] << 16;
       }
-#pragma unroll 4
-      for (int r = 1; r < ranks; ++r)
+      // two peers' bins on their way at a time
+#pragma unroll 1
+      for (int r = 1; r < ranks; r += 2) {
+        uint4 lo[2], hi[2];
 #pragma unroll
-        for (int j = 0; j < kPerThread; ++j) {
-          mine[j] += ld_cluster_u32(map_to_rank(&sh.lo[tid * kPerThread + j], r));
-          if (weights) mine[j] += (unsigned long long)ld_cluster_u32(map_to_rank(&sh.hi[tid * kPerThread + j], r)) << 16;
+        for (int i = 0; i < 2; ++i) {
+          lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
+          if (r + i < ranks) {
+            lo[i] = ld_cluster_v4(map_to_rank(&sh.lo[tid * kPerThread], r + i));
+            if (weights) hi[i] = ld_cluster_v4(map_to_rank(&sh.hi[tid * kPerThread], r + i));
+          }
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          mine[0] += lo[i].x + ((unsigned long long)hi[i].x << 16);
+          mine[1] += lo[i].y + ((unsigned long long)hi[i].y << 16);
+          mine[2] += lo[i].z + ((unsigned long long)hi[i].z << 16);
+          mine[3] += lo[i].w + ((unsigned long long)hi[i].w << 16);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < kPerThread; ++j) {
         mine[j] -= fix(tid * kPerThread + j);
@@ -443,16 +455,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs p,
   int longest = 0, listed = 0;
   auto gather = [&](auto in) {
     x.each([&](int blk, const uint32_t(&w)[kWords]) {
+      uint32_t mask = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = Row::get(w, e);
-        if (in(v)) {
-          const int at = atomicAdd(&sh.count, 1);
-          if (at < kList) {
-            sh.value[at] = __float_as_uint(v);
-            sh.index[at] = x.first(blk) + e;
+      for (int e = 0; e < 8; ++e) mask |= (uint32_t)in(Row::get(w, e)) << e;
+      if (mask) {
+        int at = atomicAdd(&sh.count, __popc(mask));
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (mask >> e & 1) {
+            if (at < kList) {
+              sh.value[at] = __float_as_uint(Row::get(w, e));
+              sh.index[at] = x.first(blk) + e;
+            }
+            ++at;
           }
-        }
       }
     });
     __syncthreads();
@@ -623,19 +639,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs p,
     const float per_bin = kBins / -kWeightCut;
     auto bin_of = [&](float v) { return v == most ? 0 : min((int)(-z_of(v) * per_bin), kBins - 1); };
     x.each([&](int, const uint32_t(&w)[kWords]) {
+      uint32_t weight[8];
+      int at[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float v = Row::get(w, e);
-        const uint32_t weight = w_of(v);
-        if (weight) put(true, bin_of(v), weight);
+        weight[e] = w_of(Row::get(w, e));
+        at[e] = bin_of(Row::get(w, e));
       }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (weight[e]) put(true, at[e], weight[e]);
     });
     scan(true, 0, limit_of, [](uint32_t) { return 0ull; });
     if (sh.found) {
       const unsigned long long limit = limit_of(sh.all), before = sh.before;
       const int bin = sh.bin;
       const float low = low_of(-(float)(bin + 1) / per_bin), high = high_of(-(float)bin / per_bin);
-      auto in = [&](float v) { return v >= low && v <= high && bin_of(v) == bin; };
+      auto in = [&](float v) { return (v >= low) & (v <= high) && bin_of(v) == bin; };
       gather(in);
       const uint32_t first = distance(high);
       const Cut c = histogram(limit, first, distance(low) + 2 - first, before, true, [&](auto f) { candidates(in, f); }, no_fix);
@@ -643,46 +663,130 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs p,
     }
   }
 
-  // 3: the kept weight of every block, apart from that of ties
-  const bool all_of = thr == 0 && !(mp > 0.f);
+  // 3: the kept weight of every block, apart from that of ties, and of the warp's stretch
   const float edge = thr ? value_of(thr) : low_of(min_cut);  // no filter but min_p: below every kept logit, so equal to none
+  const bool all_of = thr == 0 && !(mp > 0.f);
+  // Kept weights of 8 logits, and which of them are ties.
+  auto kept = [&](const uint32_t(&w)[kWords], uint32_t(&weight)[8]) {
+    uint32_t tie = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = Row::get(w, e);
+      const float x1 = e_of(v);
+      const bool keep = v >= edge && (x1 >= mp || v == most);
+      weight[e] = keep ? (uint32_t)(x1 * kOne) : 0;
+      tie |= (uint32_t)(keep && v == edge) << e;
+    }
+    return thr ? tie : 0;
+  };
+  unsigned long long own = 0, own_ties = 0;
   x.each([&](int blk, const uint32_t(&w)[kWords]) {
+    float high = Row::get(w, 0);
+#pragma unroll
+    for (int e = 1; e < 8; ++e) high = fmaxf(high, Row::get(w, e));
     unsigned long long sum = 0;
     uint32_t tied = 0;
-    if (all_of) {
+    if (__any_sync(0xffffffffu, high >= edge)) {
+      uint32_t tie = 0;
+      if (all_of) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += w_of(Row::get(w, e));
-    } else {
-      // thr is the key of `edge`, whose weight is not 0
+        for (int e = 0; e < 8; ++e) sum += w_of(Row::get(w, e));
+      } else {
+        uint32_t weight[8];
+        tie = kept(w, weight);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = Row::get(w, e);
-        if (v < edge) continue;
-        const float x1 = e_of(v);
-        if (!(x1 >= mp) && v != most) continue;
-        if (v == edge) ++tied;
-        else sum += (uint32_t)(x1 * kOne);
+        for (int e = 0; e < 8; ++e) sum += tie >> e & 1 ? 0 : weight[e];
       }
+      // 8 x 2^31 at most: two sums of 32 lanes in 32 bits
+      const uint32_t a = __reduce_add_sync(0xffffffffu, (uint32_t)sum & 0xffffu), c = __reduce_add_sync(0xffffffffu, (uint32_t)(sum >> 16));
+      sum = a + ((unsigned long long)c << 16);
+      tied = thr ? __reduce_add_sync(0xffffffffu, __popc(tie)) : 0;
     }
-    // 8 x 2^31 at most: two sums of 32 lanes in 32 bits
-    const uint32_t a = __reduce_add_sync(0xffffffffu, (uint32_t)sum & 0xffffu), c = __reduce_add_sync(0xffffffffu, (uint32_t)(sum >> 16));
-    tied = __reduce_add_sync(0xffffffffu, tied);
     if (lane == 0) {
-      sh.block[blk - cta_begin] = a + ((unsigned long long)c << 16);
+      sh.block[blk - cta_begin] = sum;
       sh.block_ties[blk - cta_begin] = tied;
     }
+    own += sum;
+    own_ties += tied;
   });
-  __syncthreads();
-  const int mine = cta_end - cta_begin, per = (mine + kThreads - 1) / kThreads;
-  const int i0 = min(tid * per, mine), i1 = min(i0 + per, mine);
-  unsigned long long own = 0;
-  uint32_t own_ties = 0;
-  for (int i = i0; i < i1; ++i) {
-    own += sh.block[i];
-    own_ties += sh.block_ties[i];
+  if (lane == 0) {
+    sh.sum[warp] = own;
+    sh.num[warp] = (uint32_t)own_ties;
   }
-  unsigned long long upto = own;
-  uint32_t upto_ties = own_ties;
+  __syncthreads();
+  if (warp == 0) {
+    unsigned long long a = lane < kWarps ? sh.sum[lane] : 0;
+    const uint32_t c = __reduce_add_sync(0xffffffffu, lane < kWarps ? sh.num[lane] : 0);
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) a += __shfl_xor_sync(0xffffffffu, a, m);
+    tell_u64(&sh.rank_sum[rank], a);
+    tell_u32(&sh.rank_ties[rank], c);
+  }
+  everyone();
+  // Sums ahead of this warp: of its CTA's warps (lanes 0 to 15) and of the CTAs (from lane 16 on).
+  unsigned long long before = 0, whole = 0;
+  uint32_t ties_before = 0, ties_all = 0;
+  if (lane < kWarps && lane < warp) {
+    before = sh.sum[lane];
+    ties_before = sh.num[lane];
+  } else if (lane >= 16 && lane - 16 < ranks) {
+    whole = sh.rank_sum[lane - 16];
+    ties_all = sh.rank_ties[lane - 16];
+    if (lane - 16 < rank) {
+      before = whole;
+      ties_before = ties_all;
+    }
+  }
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, m);
+    whole += __shfl_xor_sync(0xffffffffu, whole, m);
+  }
+  ties_before = __reduce_add_sync(0xffffffffu, ties_before);
+  ties_all = __reduce_add_sync(0xffffffffu, ties_all);
+  const uint32_t w_thr = ties_all ? w_of(edge) : 0;
+  auto with_ties = [&](unsigned long long sum, uint32_t n) { return sum + (unsigned long long)min(n, ties) * w_thr; };
+  whole = with_ties(whole, ties_all);
+  const unsigned long long target = target_of(whole);
+  if (!(with_ties(before, ties_before) <= target && target < with_ties(before + own, ties_before + (uint32_t)own_ties))) return;
+
+  // 4: this warp's stretch holds the target: the block, then the logit
+  int blk = x.begin;
+  for (int at = x.begin; at < x.end; at += 32) {
+    const unsigned long long sum = at + lane < x.end ? sh.block[at + lane - cta_begin] : 0;
+    const uint32_t tied = at + lane < x.end ? sh.block_ties[at + lane - cta_begin] : 0;
+    unsigned long long upto = sum;
+    uint32_t upto_ties = tied;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned long long a = __shfl_up_sync(0xffffffffu, upto, d);
+      const uint32_t c = __shfl_up_sync(0xffffffffu, upto_ties, d);
+      if (lane >= d) {
+        upto += a;
+        upto_ties += c;
+      }
+    }
+    const unsigned hits = __ballot_sync(0xffffffffu, target < with_ties(before + upto, ties_before + upto_ties));
+    const int hit = hits ? __ffs(hits) - 1 : 31;
+    if (hits) {
+      upto -= sum;
+      upto_ties -= tied;
+    }
+    before += __shfl_sync(0xffffffffu, upto, hit);
+    ties_before += __shfl_sync(0xffffffffu, upto_ties, hit);
+    if (hits) {
+      blk = at + hit;
+      break;
+    }
+  }
+  uint32_t w[kWords], weight[8];
+  x.load(blk, x.end, w);
+  const uint32_t tie = kept(w, weight);
+  unsigned long long sum = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum += tie >> e & 1 ? 0 : weight[e];
+  unsigned long long upto = sum;
+  uint32_t upto_ties = __popc(tie);
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const unsigned long long a = __shfl_up_sync(0xffffffffu, upto, d);
@@ -692,98 +796,32 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs p,
       upto_ties += c;
     }
   }
-  if (lane == 31) {
-    sh.sum[warp] = upto;
-    sh.num[warp] = upto_ties;
-  }
-  if (tid == 0) sh.hit = -1;
-  __syncthreads();
-  if (warp == 0) {
-    unsigned long long a = lane < kWarps ? sh.sum[lane] : 0;
-    uint32_t c = lane < kWarps ? sh.num[lane] : 0;
-#pragma unroll
-    for (int m = 16; m > 0; m >>= 1) a += __shfl_xor_sync(0xffffffffu, a, m);
-    c = __reduce_add_sync(0xffffffffu, c);
-    tell_u64(&sh.rank_sum[rank], a);
-    tell_u32(&sh.rank_ties[rank], c);
-  }
-  everyone();
-  unsigned long long before = upto - own, whole = 0, ties_before = upto_ties - own_ties, ties_all = 0;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i)
-    if (i < warp) {
-      before += sh.sum[i];
-      ties_before += sh.num[i];
-    }
-  for (int r = 0; r < ranks; ++r) {
-    if (r < rank) {
-      before += sh.rank_sum[r];
-      ties_before += sh.rank_ties[r];
-    }
-    whole += sh.rank_sum[r];
-    ties_all += sh.rank_ties[r];
-  }
-  const unsigned long long w_thr = ties_all ? w_of(value_of(thr)) : 0, most_ties = ties;
-  whole += min(ties_all, most_ties) * w_thr;
-  const unsigned long long target = target_of(whole);
-  for (int i = i0; i < i1; ++i) {
-    const unsigned long long next = before + sh.block[i], next_ties = ties_before + sh.block_ties[i];
-    if (before + min(ties_before, most_ties) * w_thr <= target && target < next + min(next_ties, most_ties) * w_thr) {
-      sh.hit = cta_begin + i;
-      sh.hit_before = before;
-      sh.hit_ties = (uint32_t)ties_before;
-    }
-    before = next;
-    ties_before = next_ties;
-  }
-  __syncthreads();
-  // 4: one warp walks the block that holds the target
-  if (warp != 0 || sh.hit < 0) return;
-  const int blk = sh.hit;
-  uint32_t w[kWords], weight[8];
-  x.load(blk, cta_end, w);
-  unsigned long long sum = 0;
-  uint32_t tied = 0, is_tie = 0;
+  before += upto - sum;
+  ties_before += upto_ties - __popc(tie);
+  const bool here = with_ties(before, ties_before) <= target &&
+                    target < with_ties(before + sum, ties_before + __popc(tie));
+  if (!here) return;
+  int chosen = 0;
+  uint32_t share_of = 0;
+  bool found = false;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float v = Row::get(w, e);
-    weight[e] = 0;
-    if (v < edge) continue;
-    const float x1 = e_of(v);
-    if (!(x1 >= mp) && v != most) continue;
-    weight[e] = (uint32_t)(x1 * kOne);
-    if (v == edge) {
-      is_tie |= 1u << e;
-      ++tied;
-    } else {
-      sum += weight[e];
-    }
-  }
-  unsigned long long ahead = sum;
-  uint32_t ties_ahead = tied;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const unsigned long long a = __shfl_up_sync(0xffffffffu, ahead, d);
-    const uint32_t c = __shfl_up_sync(0xffffffffu, ties_ahead, d);
-    if (lane >= d) {
-      ahead += a;
-      ties_ahead += c;
-    }
-  }
-  before = sh.hit_before + ahead - sum;
-  ties_before = (unsigned long long)sh.hit_ties + ties_ahead - tied;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const bool tie = is_tie >> e & 1;
-    const unsigned long long start = before + min(ties_before, most_ties) * w_thr;
-    if (tie) ++ties_before;
+    if (tie >> e & 1) ++ties_before;
     else before += weight[e];
-    if (start <= target && target < before + min(ties_before, most_ties) * w_thr) say(x.first(blk) + e, weight[e], whole);
+    if (!found && target < with_ties(before, ties_before)) {
+      found = true;
+      chosen = e;
+      share_of = weight[e];
+    }
   }
+  say(x.first(blk) + chosen, share_of, whole);
 }
 
-// CTAs per row: enough to fill the GPU, two to an SM, with at least 32 blocks (8192
-// logits) each, at most 8, and at least as many as hold a row's block sums.
+// CTAs per row: enough to fill the GPU, two to an SM, with 16 blocks (4096 logits)
+// each at least, and at most 8; at least as many as hold a row's block sums.  With
+// top_p, which makes some rows several times as long as others, up to twice as
+// many CTAs as run at a time: 256 rows of 131072, one in four with top_p alone,
+// take 138 us with one CTA each and 104 with two (all with top_k: 30 and 39).
 template <typename T>
 int launch_sample(const SampleArgs& a, int rows, cudaStream_t stream) {
   const DeviceInfo* dev = nullptr;
@@ -791,7 +829,7 @@ int launch_sample(const SampleArgs& a, int rows, cudaStream_t stream) {
   if (st != GDSQ_OK) return st;
   const int blocks = (a.vocab + 8 + kBlock - 1) / kBlock;
   int ranks = 1;
-  while (ranks < 8 && (blocks > ranks * kMaxBlocks || (2 * ranks * rows <= 2 * dev->sms && blocks >= 64 * ranks))) ranks *= 2;
+  while (ranks < 8 && (blocks > ranks * kMaxBlocks || (ranks * rows <= dev->sms * (a.top_p ? 2 : 1) && blocks >= 32 * ranks))) ranks *= 2;
   auto kernel = sample_kernel<T>;
   cudaError_t e = ensure_smem(kernel, (int)sizeof(SampleShared), dev->ordinal);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(sample)");
