@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "gdsq.h"
 #include "host.h"
@@ -178,136 +179,259 @@ struct AppendArgs {
   int tokens, heads, kv_heads, num_blocks, block_shift, max_position;
 };
 
+// 8 values of a row as fp32.
 template <typename T>
-__device__ __forceinline__ float to_f32(T v);
-template <>
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
+  const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
+      const float2 f = __half22float2(u32_as_h2(ww[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    } else {
+      x[2 * i] = __uint_as_float(ww[i] << 16);
+      x[2 * i + 1] = __uint_as_float(ww[i] & 0xffff0000u);
+    }
+  }
+}
 template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
-
-template <int N, typename T>
-__device__ __forceinline__ void load_row(const T* src, float (&x)[N]) {
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = to_f32(src[i]);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, __half>::value) {
+      w[i] = h2_as_u32(__floats2half2_rn(x[2 * i], x[2 * i + 1]));
+    } else {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// (a + ib)(c + id) as separate fp32 products and sums, rounded to T: the
-// arithmetic of rotating the complex pairs in torch.
-template <typename T, int N>
-__device__ __forceinline__ void rotate(const float2* f, float (&x)[N]) {
+// The angles of 8 values, 4 (cos, sin) pairs.
+struct Angles {
+  float4 a, b;
+};
+__device__ __forceinline__ Angles load_angles(const float2* f) {
+  const float4* p = reinterpret_cast<const float4*>(f);
+  return {__ldg(p), __ldg(p + 1)};
+}
+// (x + iy)(c + is) as separate fp32 products and sums: the arithmetic of
+// rotating the complex pairs in torch.
+__device__ __forceinline__ void rotate8(const Angles& f, float (&x)[8]) {
+  const float c[4] = {f.a.x, f.a.z, f.b.x, f.b.z}, s[4] = {f.a.y, f.a.w, f.b.y, f.b.w};
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const float2 cs = f[i / 2];
-    const float a = x[i], b = x[i + 1];
-    x[i] = to_f32(from_f32<T>(__fsub_rn(__fmul_rn(a, cs.x), __fmul_rn(b, cs.y))));
-    x[i + 1] = to_f32(from_f32<T>(__fadd_rn(__fmul_rn(a, cs.y), __fmul_rn(b, cs.x))));
+  for (int i = 0; i < 4; ++i) {
+    const float a = x[2 * i], b = x[2 * i + 1];
+    x[2 * i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
+    x[2 * i + 1] = __fadd_rn(__fmul_rn(a, s[i]), __fmul_rn(b, c[i]));
   }
 }
 
+// 8 codes of x * f.
 template <int F>
-__device__ __forceinline__ uint8_t encode(float x) {
-  if (!(x == x)) x = 0.f;
-  if constexpr (F == GDSQ_CACHE_INT8) {
-    return (uint8_t)(int8_t)(int)rintf(fminf(fmaxf(x, -127.f), 127.f));
-  } else {
-    return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ uint2 encode8(const float (&x)[8], float f) {
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y[i] = __fmul_rn(x[4 * h + i], f);
+      if (!(y[i] == y[i])) y[i] = 0.f;
+    }
+    if constexpr (F == GDSQ_CACHE_INT8) {
+      uint32_t c[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = (uint32_t)__float2int_rn(fminf(fmaxf(y[i], -127.f), 127.f));
+      w[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    } else {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+      w[h] = lo | hi << 16;
+    }
   }
+  return make_uint2(w[0], w[1]);
 }
 template <int F>
-__device__ __forceinline__ float decode(uint8_t c) {
-  if constexpr (F == GDSQ_CACHE_INT8) {
-    return (float)(int8_t)c;
-  } else {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+__device__ __forceinline__ void decode8(const uint2& w, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t c = ((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xffu;
+    if constexpr (F == GDSQ_CACHE_INT8) x[i] = (float)(int8_t)c;
+    else x[i] = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3)));
   }
 }
 
-// Grid (tokens, 1 + (q > 0)).  y = 0: a warp writes the whole of one (block,
-// KV head, K or V) when the CTA's token is the first of its block; y = 1: the
-// token's q heads are rotated.
+// Bound by the bytes of q, k and v and, for single tokens, by latency.  A unit
+// is (the new tokens of one block, KV head, K or V): its tokens are held in
+// registers, 16 to a warp, between the maximum and the codes, so that k and v
+// are read once; a longer run takes 2, 4 or 8 warps.  Grid: x takes `chunk`
+// tokens and the runs that begin among them; y takes 8 units, and from
+// kv_groups on every (y - kv_groups)-th part of q's heads.
 template <typename T, int HD, int F>
-__global__ void __launch_bounds__(kAppThreads) append_kv8_kernel(const AppendArgs p) {
-  constexpr int N = HD / 32;
+__global__ void __launch_bounds__(kAppThreads) append_kv8_kernel(const AppendArgs p, const int chunk, const int kv_groups) {
   constexpr float kTop = F == GDSQ_CACHE_INT8 ? 127.f : 448.f;
-  const int i = blockIdx.x;
+  constexpr int kLanes = HD / 8;          // lanes per token, 8 values each
+  constexpr int kAtOnce = 32 / kLanes;    // tokens per load of a warp
+  constexpr int kLoads = 16 / kAtOnce;    // of 16 tokens
+  __shared__ uint32_t red[kAppThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int i0 = blockIdx.x * chunk;
   pdl_launch_dependents();
   pdl_wait_primary();
-  const long long pos = p.freqs ? p.positions[i] : 0;
-  const bool bad_pos = p.freqs && (pos < 0 || pos >= p.max_position);
-  if (bad_pos && threadIdx.x == 0) record_device_error(kDevErrBadIndex);
-  if (blockIdx.y == 1) {
-    if (bad_pos) return;
-    for (int h = warp; h < p.heads; h += kAppThreads / 32) {
-      float x[N];
-      load_row<N>(static_cast<const T*>(p.q) + i * p.q_token_stride + h * p.q_head_stride + lane * N, x);
-      rotate<T, N>(p.freqs + pos * (HD / 2) + lane * (N / 2), x);
-      T* dst = static_cast<T*>(p.q_out) + ((size_t)i * p.heads + h) * HD + lane * N;
-#pragma unroll
-      for (int e = 0; e < N; ++e) dst[e] = from_f32<T>(x[e]);
-    }
-    return;
-  }
-  const long long slot = p.slots[i];
-  if (slot < 0) return;
-  const long long page = slot >> p.block_shift;
-  if (page >= p.num_blocks) {
-    if (threadIdx.x == 0) record_device_error(kDevErrBadIndex);
-    return;
-  }
-  if (i > 0 && p.slots[i - 1] >= 0 && (p.slots[i - 1] >> p.block_shift) == page) return;
-  int n = 1;
-  while (i + n < p.tokens && p.slots[i + n] >= 0 && (p.slots[i + n] >> p.block_shift) == page) ++n;
-  const int bs = 1 << p.block_shift;
-  const int begin = (int)(slot & (bs - 1));
-  for (int u = warp; u < 2 * p.kv_heads; u += kAppThreads / 32) {
-    const bool is_v = u >= p.kv_heads;
-    const int h = is_v ? u - p.kv_heads : u;
-    const T* src = static_cast<const T*>(is_v ? p.v : p.k) + h * (is_v ? p.v_head_stride : p.k_head_stride) + lane * N;
-    const long long ts = is_v ? p.v_token_stride : p.k_token_stride;
-    float* scale = (is_v ? p.v_scale : p.k_scale) + page * p.kv_heads + h;
-    uint8_t* dst = (is_v ? p.v_cache : p.k_cache) + ((size_t)page * p.kv_heads + h) * bs * HD + lane * N;
-    auto row = [&](int j, float(&x)[N]) {
-      load_row<N>(src + (long long)(i + j) * ts, x);
-      if (!is_v && p.freqs) {
-        const long long pj = p.positions[i + j];
-        if (pj >= 0 && pj < p.max_position) rotate<T, N>(p.freqs + pj * (HD / 2) + lane * (N / 2), x);
+  const bool rope = p.freqs != nullptr;
+
+  if ((int)blockIdx.y >= kv_groups) {
+    // q: a thread takes 8 dims of one token for every heads_step-th head
+    const int row = threadIdx.x / kLanes, d = (threadIdx.x % kLanes) * 8;
+    constexpr int kRowsAtOnce = kAppThreads / kLanes;
+    const int parts = gridDim.y - kv_groups, part = blockIdx.y - kv_groups;
+    for (int j = row % chunk; j < chunk; j += kRowsAtOnce) {  // chunk is a power of two
+      const int i = i0 + j;
+      if (i >= p.tokens) break;
+      const long long pos = p.positions[i];
+      if (pos < 0 || pos >= p.max_position) {
+        record_device_error(kDevErrBadIndex);
+        continue;
       }
-    };
-    uint32_t most = 0;  // magnitudes order as their bits do, inf and NaN on top
-    for (int j = 0; j < n; ++j) {
-      float x[N];
-      row(j, x);
+      const Angles f = load_angles(p.freqs + pos * (HD / 2) + d / 2);
+      const int step = max(kRowsAtOnce / chunk, 1);
+      const T* src = static_cast<const T*>(p.q) + i * p.q_token_stride + d;
+      T* dst = static_cast<T*>(p.q_out) + (size_t)i * p.heads * HD + d;
+      constexpr int kAhead = 4;
+      for (int h0 = part * step + row / chunk; h0 < p.heads; h0 += kAhead * parts * step) {
+        uint4 w[kAhead];
 #pragma unroll
-      for (int e = 0; e < N; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
+        for (int y = 0; y < kAhead; ++y) {
+          const int h = h0 + y * parts * step;
+          if (h < p.heads) w[y] = __ldg(reinterpret_cast<const uint4*>(src + h * p.q_head_stride));
+        }
+#pragma unroll
+        for (int y = 0; y < kAhead; ++y) {
+          const int h = h0 + y * parts * step;
+          if (h >= p.heads) break;
+          float x[8];
+          unpack8<T>(w[y], x);
+          rotate8(f, x);
+          *reinterpret_cast<uint4*>(dst + (size_t)h * HD) = pack8<T>(x);
+        }
+      }
     }
-    most = __reduce_max_sync(0xffffffffu, most);
-    const float base = begin == 0 ? 0.f : *scale;
-    float need = __fmul_rn(__uint_as_float(most), 1.f / kTop);
-    if (need < kSmallestScale) need = 0.f;
-    float s = need <= base ? base : fmaxf(need, 2.f * base);
-    if (most >= 0x7f800000u || !(base == base)) s = __int_as_float(0x7fc00000);
-    const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
-    __syncwarp();
-    if (s != base && begin > 0) {
-      const float ratio = __fmul_rn(base, inv);
-      for (int j = 0; j < begin; ++j)
-#pragma unroll
-        for (int e = 0; e < N; ++e) dst[(size_t)j * HD + e] = encode<F>(__fmul_rn(decode<F>(dst[(size_t)j * HD + e]), ratio));
+    return;
+  }
+
+  const int bs = 1 << p.block_shift;
+  // Tokens that begin a run: the first of their block in the batch.
+  const int il = i0 + lane;
+  bool begins = false;
+  if (lane < chunk && il < p.tokens) {
+    const long long slot = p.slots[il], page = slot >> p.block_shift;
+    if (slot >= 0) {
+      if (page >= p.num_blocks) {
+        if (warp == 0) record_device_error(kDevErrBadIndex);
+      } else {
+        begins = il == 0 || p.slots[il - 1] < 0 || (p.slots[il - 1] >> p.block_shift) != page;
+      }
     }
-    if (lane == 0) *scale = s;
-    for (int j = 0; j < n; ++j) {
-      float x[N];
-      row(j, x);
-      const int off = (int)(p.slots[i + j] & (bs - 1));
+  }
+  for (unsigned heads = __ballot_sync(0xffffffffu, begins); heads; heads &= heads - 1) {
+    const int i = i0 + __ffs(heads) - 1;
+    const long long slot = p.slots[i], page = slot >> p.block_shift;
+    const int begin = (int)(slot & (bs - 1));
+    int n = 0;  // tokens of the run
+    for (;;) {
+      const int at = i + n + lane;
+      const bool same = at < p.tokens && n + lane < bs && p.slots[at] >= 0 && (p.slots[at] >> p.block_shift) == page;
+      const unsigned other = ~__ballot_sync(0xffffffffu, same);
+      if (other) {
+        n += __ffs(other) - 1;
+        break;
+      }
+      n += 32;
+    }
+    const int wide = n <= 16 ? 1 : n <= 32 ? 2 : n <= 64 ? 4 : 8;  // warps per unit
+    const int sub = warp / wide, part = warp % wide;
+    for (int pass = 0; pass < wide; ++pass) {
+      const int u = blockIdx.y * 8 + pass * (8 / wide) + sub;
+      const bool live_unit = u < 2 * p.kv_heads;
+      const bool is_v = u >= p.kv_heads;
+      const int h = live_unit ? (is_v ? u - p.kv_heads : u) : 0;
+      const T* src = static_cast<const T*>(is_v ? p.v : p.k) + h * (is_v ? p.v_head_stride : p.k_head_stride) + (lane % kLanes) * 8;
+      const long long stride = is_v ? p.v_token_stride : p.k_token_stride;
+      float* scale = (is_v ? p.v_scale : p.k_scale) + page * p.kv_heads + h;
+      uint8_t* dst = (is_v ? p.v_cache : p.k_cache) + ((size_t)page * p.kv_heads + h) * bs * HD + (lane % kLanes) * 8;
+      const float base = begin == 0 ? 0.f : *scale;
+      uint4 raw[kLoads];
+      uint32_t live = 0;
 #pragma unroll
-      for (int e = 0; e < N; ++e) dst[(size_t)off * HD + e] = encode<F>(__fmul_rn(x[e], inv));
+      for (int j = 0; j < kLoads; ++j) {
+        const int tk = part * 16 + j * kAtOnce + lane / kLanes;
+        raw[j] = make_uint4(0, 0, 0, 0);
+        if (live_unit && tk < n) {
+          raw[j] = __ldg(reinterpret_cast<const uint4*>(src + (long long)(i + tk) * stride));
+          live |= 1u << j;
+        }
+      }
+      uint32_t most = 0;  // magnitudes order as their bits do, inf and NaN on top; 0: no token
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        if (j * kAtOnce + part * 16 >= n) break;
+        if (rope && (live >> j & 1)) {
+          const long long pos = p.positions[i + part * 16 + j * kAtOnce + lane / kLanes];
+          if (pos < 0 || pos >= p.max_position) {
+            record_device_error(kDevErrBadIndex);
+            live &= ~(1u << j);
+          } else if (!is_v) {
+            float x[8];
+            unpack8<T>(raw[j], x);
+            rotate8(load_angles(p.freqs + pos * (HD / 2) + (lane % kLanes) * 4), x);
+            raw[j] = pack8<T>(x);
+          }
+        }
+        if (live >> j & 1) {
+          float x[8];
+          unpack8<T>(raw[j], x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) most = max(most, (__float_as_uint(x[e]) & 0x7fffffffu) + 1);
+        }
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (wide > 1) {
+        __syncthreads();
+        if (lane == 0) red[warp] = most;
+        __syncthreads();
+        for (int w = 0; w < wide; ++w) most = max(most, red[sub * wide + w]);
+      } else {
+        __syncwarp();
+      }
+      if (most == 0) continue;
+      --most;
+      float need = __fmul_rn(__uint_as_float(most), 1.f / kTop);
+      if (need < kSmallestScale) need = 0.f;
+      float s = need <= base ? base : fmaxf(need, 2.f * base);
+      if (most >= 0x7f800000u || !(base == base)) s = __int_as_float(0x7fc00000);
+      const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+      if (s != base && begin > 0) {
+        const float ratio = __fmul_rn(base, inv);
+        for (int j = part * kAtOnce + lane / kLanes; j < begin; j += wide * kAtOnce) {
+          uint2* at = reinterpret_cast<uint2*>(dst + (size_t)j * HD);
+          float x[8];
+          decode8<F>(*at, x);
+          *at = encode8<F>(x, ratio);
+        }
+      }
+      if (part == 0 && lane == 0) *scale = s;
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j)
+        if (live >> j & 1) {
+          const int off = (int)(p.slots[i + part * 16 + j * kAtOnce + lane / kLanes] & (bs - 1));
+          float x[8];
+          unpack8<T>(raw[j], x);
+          *reinterpret_cast<uint2*>(dst + (size_t)off * HD) = encode8<F>(x, inv);
+        }
     }
   }
 }
@@ -325,13 +449,21 @@ cudaError_t serve_error_bits(bool clear, int* bits) {
 
 namespace {
 
+// A CTA looks at one token where there are few, else at 16, so that runs of a
+// block's tokens do not leave most CTAs with nothing to do.
+constexpr int kAppManyTokens = 1024;
+
 template <typename T, int F>
 int launch_append(const AppendArgs& a, int head_dim, cudaStream_t stream) {
-  const dim3 grid(a.tokens, a.q_out ? 2 : 1);
+  const int chunk = a.tokens >= kAppManyTokens ? 16 : 1;
+  const int kv_groups = (2 * a.kv_heads + 7) / 8;
+  // q: 16 vectors of 8 values per thread, or 4 where there are few
+  const int q_groups = !a.q_out ? 0 : std::max(1, chunk * a.heads * head_dim / 8 / kAppThreads / (chunk == 1 ? 4 : 16));
+  const dim3 grid((a.tokens + chunk - 1) / chunk, kv_groups + q_groups);
   auto kernel = head_dim == 64    ? append_kv8_kernel<T, 64, F>
                 : head_dim == 128 ? append_kv8_kernel<T, 128, F>
                                   : append_kv8_kernel<T, 256, F>;
-  cudaError_t e = launch(kernel, grid, dim3(kAppThreads), 0, stream, g_pdl_enabled != 0, a);
+  cudaError_t e = launch(kernel, grid, dim3(kAppThreads), 0, stream, g_pdl_enabled != 0, a, chunk, kv_groups);
   return e == cudaSuccess ? GDSQ_OK : cuda_fail(e, "append_kv8 launch");
 }
 
