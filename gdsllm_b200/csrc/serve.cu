@@ -210,6 +210,12 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+template <typename T>
+__device__ __forceinline__ float value_of_bits(uint32_t bits) {
+  if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)bits));
+  return __uint_as_float(bits << 16);
+}
+
 // The angles of 8 values, 4 (cos, sin) pairs.
 struct Angles {
   float4 a, b;
@@ -230,7 +236,8 @@ __device__ __forceinline__ void rotate8(const Angles& f, float (&x)[8]) {
   }
 }
 
-// 8 codes of x * f.
+// 8 codes of x * f, which is at most the format's largest code, give or take a
+// rounding, by the choice of the scale.
 template <int F>
 __device__ __forceinline__ uint2 encode8(const float (&x)[8], float f) {
   uint32_t w[2];
@@ -238,14 +245,12 @@ __device__ __forceinline__ uint2 encode8(const float (&x)[8], float f) {
   for (int h = 0; h < 2; ++h) {
     float y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      y[i] = __fmul_rn(x[4 * h + i], f);
-      if (!(y[i] == y[i])) y[i] = 0.f;
-    }
+    for (int i = 0; i < 4; ++i) y[i] = __fmul_rn(x[4 * h + i], f);
     if constexpr (F == GDSQ_CACHE_INT8) {
+      // 1.5 * 2^23 + y is rounded to a whole number, half to even, whose two's complement is the low bits
       uint32_t c[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] = (uint32_t)__float2int_rn(fminf(fmaxf(y[i], -127.f), 127.f));
+      for (int i = 0; i < 4; ++i) c[i] = __float_as_uint(__fadd_rn(y[i], 12582912.f));
       w[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     } else {
       const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
@@ -268,27 +273,28 @@ __device__ __forceinline__ void decode8(const uint2& w, float (&x)[8]) {
 // Bound by the bytes of q, k and v and, for single tokens, by latency.  A unit
 // is (the new tokens of one block, KV head, K or V): its tokens are held in
 // registers, 16 to a warp, between the maximum and the codes, so that k and v
-// are read once; a longer run takes 2, 4 or 8 warps.  Grid: x takes `chunk`
-// tokens and the runs that begin among them; y takes 8 units, and from
-// kv_groups on every (y - kv_groups)-th part of q's heads.
+// are read once; a longer run takes 2, 4 or 8 warps.  A CTA takes `chunk` tokens
+// and the runs that begin among them, and 8 units or a part of q's heads; the
+// groups of one chunk are neighbours, so that a token's row is read at one time.
 template <typename T, int HD, int F>
-__global__ void __launch_bounds__(kAppThreads) append_kv8_kernel(const AppendArgs p, const int chunk, const int kv_groups) {
+__global__ void __launch_bounds__(kAppThreads, HD == 256 ? 2 : 4) append_kv8_kernel(const AppendArgs p, const int chunk, const int kv_groups,
+                                                                 const int groups) {
   constexpr float kTop = F == GDSQ_CACHE_INT8 ? 127.f : 448.f;
   constexpr int kLanes = HD / 8;          // lanes per token, 8 values each
   constexpr int kAtOnce = 32 / kLanes;    // tokens per load of a warp
   constexpr int kLoads = 16 / kAtOnce;    // of 16 tokens
   __shared__ uint32_t red[kAppThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int i0 = blockIdx.x * chunk;
+  const int group = blockIdx.x % groups, i0 = (int)(blockIdx.x / groups) * chunk;
   pdl_launch_dependents();
   pdl_wait_primary();
   const bool rope = p.freqs != nullptr;
 
-  if ((int)blockIdx.y >= kv_groups) {
+  if (group >= kv_groups) {
     // q: a thread takes 8 dims of one token for every heads_step-th head
     const int row = threadIdx.x / kLanes, d = (threadIdx.x % kLanes) * 8;
     constexpr int kRowsAtOnce = kAppThreads / kLanes;
-    const int parts = gridDim.y - kv_groups, part = blockIdx.y - kv_groups;
+    const int parts = groups - kv_groups, part = group - kv_groups;
     for (int j = row % chunk; j < chunk; j += kRowsAtOnce) {  // chunk is a power of two
       const int i = i0 + j;
       if (i >= p.tokens) break;
@@ -355,7 +361,7 @@ __global__ void __launch_bounds__(kAppThreads) append_kv8_kernel(const AppendArg
     const int wide = n <= 16 ? 1 : n <= 32 ? 2 : n <= 64 ? 4 : 8;  // warps per unit
     const int sub = warp / wide, part = warp % wide;
     for (int pass = 0; pass < wide; ++pass) {
-      const int u = blockIdx.y * 8 + pass * (8 / wide) + sub;
+      const int u = group * 8 + pass * (8 / wide) + sub;
       const bool live_unit = u < 2 * p.kv_heads;
       const bool is_v = u >= p.kv_heads;
       const int h = live_unit ? (is_v ? u - p.kv_heads : u) : 0;
@@ -375,7 +381,7 @@ __global__ void __launch_bounds__(kAppThreads) append_kv8_kernel(const AppendArg
           live |= 1u << j;
         }
       }
-      uint32_t most = 0;  // magnitudes order as their bits do, inf and NaN on top; 0: no token
+      uint32_t pair = 0;
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
         if (j * kAtOnce + part * 16 >= n) break;
@@ -392,13 +398,13 @@ __global__ void __launch_bounds__(kAppThreads) append_kv8_kernel(const AppendArg
           }
         }
         if (live >> j & 1) {
-          float x[8];
-          unpack8<T>(raw[j], x);
+          const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
 #pragma unroll
-          for (int e = 0; e < 8; ++e) most = max(most, (__float_as_uint(x[e]) & 0x7fffffffu) + 1);
+          for (int e = 0; e < 4; ++e) pair = __vmaxu2(pair, w[e] & 0x7fff7fffu);
         }
       }
-      most = __reduce_max_sync(0xffffffffu, most);
+      // 16-bit magnitudes order as their bits do, inf and NaN on top; 0 is no token, so 1 more
+      uint32_t most = __reduce_max_sync(0xffffffffu, live ? max(pair & 0xffffu, pair >> 16) + 1 : 0);
       if (wide > 1) {
         __syncthreads();
         if (lane == 0) red[warp] = most;
@@ -408,11 +414,11 @@ __global__ void __launch_bounds__(kAppThreads) append_kv8_kernel(const AppendArg
         __syncwarp();
       }
       if (most == 0) continue;
-      --most;
-      float need = __fmul_rn(__uint_as_float(most), 1.f / kTop);
+      const float top = value_of_bits<T>(most - 1);
+      float need = __fmul_rn(top, 1.f / kTop);
       if (need < kSmallestScale) need = 0.f;
       float s = need <= base ? base : fmaxf(need, 2.f * base);
-      if (most >= 0x7f800000u || !(base == base)) s = __int_as_float(0x7fc00000);
+      if (!isfinite(top) || !(base == base)) s = __int_as_float(0x7fc00000);
       const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
       if (s != base && begin > 0) {
         const float ratio = __fmul_rn(base, inv);
@@ -420,7 +426,9 @@ __global__ void __launch_bounds__(kAppThreads) append_kv8_kernel(const AppendArg
           uint2* at = reinterpret_cast<uint2*>(dst + (size_t)j * HD);
           float x[8];
           decode8<F>(*at, x);
-          *at = encode8<F>(x, ratio);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = inv > 0.f && x[e] == x[e] ? x[e] : 0.f;
+          *at = encode8<F>(x, inv > 0.f ? ratio : 0.f);
         }
       }
       if (part == 0 && lane == 0) *scale = s;
@@ -430,7 +438,7 @@ __global__ void __launch_bounds__(kAppThreads) append_kv8_kernel(const AppendArg
           const int off = (int)(p.slots[i + part * 16 + j * kAtOnce + lane / kLanes] & (bs - 1));
           float x[8];
           unpack8<T>(raw[j], x);
-          *reinterpret_cast<uint2*>(dst + (size_t)off * HD) = encode8<F>(x, inv);
+          *reinterpret_cast<uint2*>(dst + (size_t)off * HD) = inv > 0.f ? encode8<F>(x, inv) : make_uint2(0, 0);
         }
     }
   }
@@ -459,11 +467,12 @@ int launch_append(const AppendArgs& a, int head_dim, cudaStream_t stream) {
   const int kv_groups = (2 * a.kv_heads + 7) / 8;
   // q: 16 vectors of 8 values per thread, or 4 where there are few
   const int q_groups = !a.q_out ? 0 : std::max(1, chunk * a.heads * head_dim / 8 / kAppThreads / (chunk == 1 ? 4 : 16));
-  const dim3 grid((a.tokens + chunk - 1) / chunk, kv_groups + q_groups);
+  const int groups = kv_groups + q_groups;
+  const dim3 grid((unsigned)((a.tokens + chunk - 1) / chunk) * groups);
   auto kernel = head_dim == 64    ? append_kv8_kernel<T, 64, F>
                 : head_dim == 128 ? append_kv8_kernel<T, 128, F>
                                   : append_kv8_kernel<T, 256, F>;
-  cudaError_t e = launch(kernel, grid, dim3(kAppThreads), 0, stream, g_pdl_enabled != 0, a, chunk, kv_groups);
+  cudaError_t e = launch(kernel, grid, dim3(kAppThreads), 0, stream, g_pdl_enabled != 0, a, chunk, kv_groups, groups);
   return e == cudaSuccess ? GDSQ_OK : cuda_fail(e, "append_kv8 launch");
 }
 
