@@ -783,6 +783,600 @@ size_t stream_workspace(int sms) {
   return kCounterBytes + (size_t)sms * stream_per_sm<HD, NT>() * 2 * (8 * NT) * (HD + 2) * 4;
 }
 
+// ---------------------------------------------------------------------------
+// Many rows per (request, KV head): prompts and long chunks.
+//
+// Bound by the tensor cores and the exponentials, so the products run on
+// tcgen05: an item is QT tiles of 128 rows, a step is BN tokens.  The cut into
+// steps and the joining of partial sums are those of the kernel above, with one
+// CTA per SM.
+//
+//   warps 0-7   softmax: warp group t owns the rows of tile t, a thread a row.  Q
+//               row to fp16 in shared memory; then per step the scores from
+//               TMEM, weights back to TMEM over them, in the end the output.
+//   warps 8-11  widen the 8-bit tiles to fp16
+//   warp 12     issues the products
+//   warp 13     TMA of the 8-bit tiles, and the blocks' scales
+//
+// K and V are widened to the same layout, [64 dims][token][128 bytes], 128-byte
+// swizzled: K major for the scores (a row of B is a token) and N major for the
+// output (a column of B is a dim).  With two tiles the order of products is
+// O0(i) S0(i+1) O1(i) S1(i+1), so that one tile's softmax runs beside the other's
+// products; the weights take the scores' place in TMEM.  The widened tiles need
+// no second buffer: scores i are done long before K i+1 is needed.
+
+template <int HD>
+struct TileLayout {
+  static constexpr int QT = HD == 256 ? 1 : 2;   // tiles of 128 rows
+  static constexpr int BN = HD == 256 ? 64 : 128;  // tokens per step
+  static constexpr int kRows = 128 * QT;
+  static constexpr int kQ = 128 * HD * 2;        // one tile of Q
+  static constexpr int kWide = BN * HD * 2;      // K or V of a step in fp16
+  static constexpr int kRaw = BN * HD;           // in 8 bits
+  static constexpr int kKOff = QT * kQ, kVOff = kKOff + kWide, kRawOff = kVOff + kWide;
+  static constexpr int kConst = kRawOff + 4 * kRaw;  // [2][BN / 16] float4
+  static constexpr int kBars = kConst + 2 * (BN / 16) * 16;
+  static constexpr int kNeed = kBars + 512 + 1024;
+  static constexpr int kTotal = kNeed > 116 * 1024 ? kNeed : 116 * 1024;  // one CTA (512 TMEM columns) per SM
+};
+constexpr int kTileThreads = 14 * 32;
+
+__device__ __forceinline__ void tc_mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      : "memory");
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle: 8 rows of 128 bytes per
+// 1024-byte atom.  K major: `sbo` bytes between groups of 8 rows.  N major:
+// `sbo` bytes between groups of 8 K rows, `lbo` between blocks of 64 columns.
+__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)((lbo >> 4) & 0x3FFFu) << 16;
+  d |= (uint64_t)((sbo >> 4) & 0x3FFFu) << 32;
+  d |= (uint64_t)1 << 46;  // descriptor version for sm_100
+  d |= (uint64_t)2 << 61;  // 128-byte swizzle
+  return d;
+}
+
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// Each lane stores 32 consecutive 32-bit columns of its own TMEM lane.
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
+      "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
+      "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+
+template <int HD, int F>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    attend_tile_kernel(const AttendArgs p, const __grid_constant__ CUtensorMap kmap,
+                       const __grid_constant__ CUtensorMap vmap, float* parts, int* counters) {
+  using L = TileLayout<HD>;
+  constexpr int QT = L::QT, BN = L::BN, kRows = L::kRows;
+  constexpr int kParts = HD >= 128 ? HD / 128 : 1, kPart = HD >= 128 ? 128 : 64;
+  constexpr uint32_t kOCol = 2 * BN;  // scores of the tiles first (one tile: the second place is unused)
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+  const uint32_t sbase = smem_addr(smem);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  uint64_t* raw_full = bars;        // [2][K, V]
+  uint64_t* raw_empty = bars + 4;   // [2][K, V]
+  uint64_t* wide_full = bars + 8;   // [K, V]
+  uint64_t* wide_empty = bars + 10; // [K, V]
+  uint64_t* s_full = bars + 12;     // [QT]
+  uint64_t* p_full = bars + 14;     // [QT]
+  uint64_t* o_full = bars + 16;
+  uint64_t* q_full = bars + 17;
+  uint64_t* const_full = bars + 18;  // [2]
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 20);
+  volatile int* dead = reinterpret_cast<volatile int*>(tmem_at + 1);  // a wait ran out
+  int* last_one = reinterpret_cast<int*>(tmem_at + 2);
+  long long* shared_ll = reinterpret_cast<long long*>(bars + 24);    // [14] and one more
+  int* shared_r = reinterpret_cast<int*>(bars + 40);
+  uint64_t* const_empty = bars + 42;  // [2]
+  const float4* consts = reinterpret_cast<const float4*>(smem + L::kConst);  // [2][BN / 16]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kMmaWarp = 12, kTmaWarp = 13;
+  if (warp == kTmaWarp && lane == 0) {
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(raw_full + i, 1);
+      mbar_init(raw_empty + i, 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(wide_full + i, 4);
+      mbar_init(wide_empty + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(p_full + i, 4);
+      mbar_init(const_full + i, 1);
+      mbar_init(const_empty + i, 4 * QT);
+    }
+    mbar_init(o_full, 1);
+    mbar_init(q_full, 4 * QT);
+    *dead = 0;
+    fence_barrier_init();
+    prefetch_tensor_map(&kmap);
+    prefetch_tensor_map(&vmap);
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(tmem_at, 512);
+    tmem_relinquish();
+  }
+  pdl_launch_dependents();
+  pdl_wait_primary();
+
+  // The schedule, as in attend_stream_kernel.
+  const int most_len = p.table_width << p.block_shift;
+  auto rows_of = [&](int r) { return max(min(p.starts[r + 1], p.tokens) - max(p.starts[r], 0), 0) * p.group; };
+  auto cost_of = [&](int r) {
+    return (long long)ceil_div(rows_of(r), kRows) * p.kv_heads * (max(ceil_div(min(p.seq_lens[r], most_len), BN), 1) + kItemCost);
+  };
+  long long all, s0, s1, request_at;
+  const int per = ceil_div(p.requests, kTileThreads);
+  const int ra = min((int)threadIdx.x * per, p.requests), rb = min(ra + per, p.requests);
+  long long mine = 0;
+  for (int r = ra; r < rb; ++r) mine += cost_of(r);
+  long long upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += x;
+  }
+  if (lane == 31) shared_ll[warp] = upto;
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_at;
+  long long before = upto - mine;
+  all = 0;
+  for (int w = 0; w < kTileThreads / 32; ++w) {
+    if (w < warp) before += shared_ll[w];
+    all += shared_ll[w];
+  }
+  const long long C = min((long long)gridDim.x, all);
+  const bool works = blockIdx.x < C;
+  s0 = works ? all * blockIdx.x / C : 0;
+  s1 = works ? all * (blockIdx.x + 1) / C : 0;
+  if (works && before <= s0 && s0 < before + mine) {
+    int r = ra;
+    long long at = before;
+    for (; r < rb; ++r) {
+      const long long n = cost_of(r);
+      if (s0 < at + n) break;
+      at += n;
+    }
+    *shared_r = r;
+    shared_ll[15] = at;
+  }
+  __syncthreads();
+  int r = works ? *shared_r : 0;
+  request_at = works ? shared_ll[15] : 0;
+
+  struct Segment {
+    int r, h, row0, rows, start, lim0;  // row i of the item sees positions up to lim0 + (row0 + i) / group
+    int t0, t1, count;                  // first token, the end, and the steps
+    int kv_len, steps;
+    long long first_step;
+    bool opens, whole;
+  };
+  auto next_segment = [&](Segment& a) {
+    while (s0 < s1) {
+      const int start = max(p.starts[r], 0);
+      const int n = max(min(p.starts[r + 1], p.tokens) - start, 0);
+      const int rows = n * p.group;
+      const int row_tiles = ceil_div(rows, kRows);
+      const int len = min(p.seq_lens[r], most_len);
+      if (len < p.seq_lens[r]) record_device_error(kDevErrBadIndex);
+      const int steps = max(ceil_div(len, BN), 1), cost = steps + kItemCost;
+      const long long request_cost = (long long)row_tiles * p.kv_heads * cost;
+      if (s0 >= request_at + request_cost) {
+        request_at += request_cost;
+        ++r;
+        continue;
+      }
+      const int item = (int)((s0 - request_at) / cost);
+      const long long first_step = request_at + (long long)item * cost + kItemCost;
+      const int step = (int)max(s0 - first_step, 0ll);
+      s0 = first_step + step;
+      if (s0 >= s1) return false;
+      const int step_end = (int)min((long long)steps, step + (s1 - s0));
+      s0 += step_end - step;
+      a.r = r;
+      a.h = item / row_tiles;
+      a.row0 = (item % row_tiles) * kRows;
+      a.rows = rows;
+      a.start = start;
+      a.lim0 = len - n;
+      a.kv_len = max(min(len, a.lim0 + (min(rows, a.row0 + kRows) - 1) / p.group + 1), 0);
+      a.t0 = step * BN;
+      a.t1 = min(a.kv_len, step_end * BN);
+      a.count = a.t0 < a.t1 ? (a.t1 - a.t0 + BN - 1) / BN : 0;
+      a.steps = steps;
+      a.first_step = first_step;
+      a.opens = step == 0;
+      a.whole = step == 0 && step_end == steps;
+      return true;
+    }
+    return false;
+  };
+  // Waits of one warp; once one has run out nobody waits any more.
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (*dead) return;
+    if (!mbar_wait(bar, parity)) {
+      record_device_error(kDevErrBarrierTimeout);
+      *dead = 1;
+    }
+  };
+
+  Segment a;
+  if (warp == kTmaWarp) {
+    uint32_t i = 0;  // steps so far
+    while (next_segment(a))
+      for (int step = 0; step < a.count; ++step, ++i) {
+        const int j0 = a.t0 + step * BN, stage = i & 1;
+        // lane's group of 16 tokens
+        int page = 0, row = 0;
+        if (lane < BN / 16) {
+          const int pos = min(j0 + 16 * lane, (a.t1 - 1) & ~15);
+          const int col = pos >> p.block_shift;
+          page = col < p.table_width ? p.table[(size_t)a.r * p.table_width + col] : -1;
+          if ((unsigned)page >= (unsigned)p.num_blocks) {
+            record_device_error(kDevErrBadIndex);
+            page = 0;
+          }
+          row = (int)((((long long)page * p.kv_heads + a.h) << p.block_shift) + (pos & ((1 << p.block_shift) - 1)));
+        }
+        const float3 c = lane < BN / 16 ? page_constants(p, page, a.h, Code<F>::kLogFactor) : make_float3(0.f, 0.f, 0.f);
+        if (i >= 2) wait(const_empty + stage, ((i >> 1) - 1) & 1);
+        if (lane < BN / 16) reinterpret_cast<float4*>(smem + L::kConst)[stage * (BN / 16) + lane] = make_float4(c.x, c.y, c.z, 0.f);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(const_full + stage);
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          uint64_t* bar = raw_full + 2 * stage + kv;
+          if (i >= 2) wait(raw_empty + 2 * stage + kv, ((i >> 1) - 1) & 1);
+          if (lane == 0 && !*dead) mbar_arrive_expect_tx(bar, L::kRaw);
+          __syncwarp();
+          if (lane < BN / 16 && !*dead) {
+            const uint64_t policy = l2_policy_normal();
+            unsigned char* dst = smem + L::kRawOff + (2 * stage + kv) * L::kRaw + lane * 16 * kPart;
+#pragma unroll
+            for (int part = 0; part < kParts; ++part)
+              tma_load_2d(dst + part * BN * kPart, kv ? &vmap : &kmap, part * 128, row, bar, policy);
+          }
+          __syncwarp();
+        }
+      }
+  } else if (warp == kMmaWarp) {
+    constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | (8u << 24);
+    constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // B is N major
+    uint32_t i = 0, seg = 0;
+    auto scores = [&](int t) {
+      if (lane == 0) {
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint64_t qa = smem_desc_sw128(sbase + t * L::kQ + (k / 4) * (128 * 128) + (k % 4) * 32, 16, 1024);
+          const uint64_t kb = smem_desc_sw128(sbase + L::kKOff + (k / 4) * (BN * 128) + (k % 4) * 32, 16, 1024);
+          tc_mma_f16_ss(tmem + t * BN, qa, kb, kIdescS, k > 0);
+        }
+        tc_commit(s_full + t);
+      }
+      __syncwarp();
+    };
+    auto output = [&](int t, bool first) {
+      if (lane == 0) {
+#pragma unroll
+        for (int k = 0; k < BN / 16; ++k) {
+          const uint64_t vb = smem_desc_sw128(sbase + L::kVOff + k * 2048, BN * 128, 1024);
+          tc_mma_f16_ts(tmem + kOCol + t * HD, tmem + t * BN + k * 8, vb, kIdescO, !(first && k == 0));
+        }
+      }
+      __syncwarp();
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (lane == 0) tc_commit(bar);
+      __syncwarp();
+    };
+    while (next_segment(a)) {
+      if (a.count == 0) continue;
+      wait(q_full, seg & 1);
+      ++seg;
+      tc_fence_after_sync();
+      wait(wide_full + 0, i & 1);
+      tc_fence_after_sync();
+      for (int t = 0; t < QT; ++t) scores(t);
+      commit(wide_empty + 0);
+      for (int step = 0; step < a.count; ++step, ++i) {
+        const bool more = step + 1 < a.count;
+        wait(wide_full + 1, i & 1);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          wait(p_full + t, i & 1);
+          tc_fence_after_sync();
+          output(t, step == 0);
+          if (t == QT - 1) commit(wide_empty + 1);
+          if (more) {
+            if (t == 0) wait(wide_full + 0, (i + 1) & 1);
+            tc_fence_after_sync();
+            scores(t);
+            if (t == QT - 1) commit(wide_empty + 0);
+          }
+        }
+      }
+      commit(o_full);
+    }
+  } else if (warp >= 8) {
+    // widen: 16 codes of one token at a time
+    const int tid = threadIdx.x - 256;
+    uint32_t i = 0;
+    while (next_segment(a))
+      for (int step = 0; step < a.count; ++step, ++i) {
+        const int stage = i & 1, left = a.t1 - (a.t0 + step * BN);  // tokens from here on hold nothing
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          wait(raw_full + 2 * stage + kv, (i >> 1) & 1);
+          if (i >= 1) wait(wide_empty + kv, (i - 1) & 1);
+          const uint32_t raw = sbase + L::kRawOff + (2 * stage + kv) * L::kRaw;
+          const uint32_t wide = sbase + (kv ? L::kVOff : L::kKOff);
+#pragma unroll 4
+          for (int j = 0; j < BN * (HD / 16) / 128; ++j) {
+            const int unit = tid + j * 128, tok = unit % BN, c = unit / BN;  // chunk of 16 dims
+            uint32_t at;
+            if constexpr (kPart == 128)
+              at = raw + (c / 8) * (BN * 128) + tok * 128 + (((c % 8) ^ (tok & 7)) << 4);
+            else
+              at = raw + tok * 64 + ((c ^ ((tok >> 1) & 3)) << 4);
+            uint4 x = lds128(at);
+            if (F == GDSQ_CACHE_E4M3 && kv && tok >= left) x = make_uint4(0, 0, 0, 0);  // may hold NaN codes
+            uint32_t o[8];
+            Code<F>::unpack(x.x, o[0], o[1]);
+            Code<F>::unpack(x.y, o[2], o[3]);
+            Code<F>::unpack(x.z, o[4], o[5]);
+            Code<F>::unpack(x.w, o[6], o[7]);
+            const uint32_t row = wide + (c / 4) * (BN * 128) + tok * 128;
+            const uint32_t c0 = (c % 4) * 2;
+            sts128(row + ((c0 ^ (tok & 7)) << 4), o[0], o[1], o[2], o[3]);
+            sts128(row + (((c0 + 1) ^ (tok & 7)) << 4), o[4], o[5], o[6], o[7]);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(raw_empty + 2 * stage + kv);
+            mbar_arrive(wide_full + kv);
+          }
+        }
+      }
+  } else if (warp < 4 * QT) {
+    const int t = warp >> 2;                       // tile
+    const int local = t * 128 + (threadIdx.x & 127);  // row of the item
+    const uint32_t quarter = (uint32_t)(warp & 3) << 21;  // TMEM lane (warp % 4) * 32 in the address
+    const uint32_t s_at = tmem + quarter + t * BN, o_at = tmem + quarter + kOCol + t * HD;
+    uint32_t i = 0, seg = 0;
+    while (next_segment(a)) {
+      const int row = a.row0 + local;
+      const bool live = row < a.rows;
+      float m = kNoMax, l = 0.f, qe = 1.f;
+      int lim = a.t1 - 1;
+      if (a.count > 0) {
+        // the Q row: power-of-two scale, fp16
+        const long long q_at = (long long)(a.start + (live ? row : 0) / p.group) * p.q_token_stride +
+                               (long long)(a.h * p.group + (live ? row : 0) % p.group) * p.q_head_stride;
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + q_at);
+        float most = 0.f;
+        uint4 w[8];
+#pragma unroll
+        for (int half = 0; half < HD / 64; ++half) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) w[c] = live ? __ldg(src + half * 8 + c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const uint32_t ww[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = unpack_q(p.bf16, ww[e]);
+              most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          }
+        }
+        int ex = (int)(__float_as_uint(most) >> 23) - 126;  // most < 2^ex
+        ex = isfinite(most) ? min(max(ex, -100), 100) : 0;
+        const float down = copysignf(__uint_as_float((uint32_t)(127 - ex) << 23), p.scale);
+        qe = __uint_as_float((uint32_t)(127 + ex) << 23);
+        const uint32_t dst = sbase + t * L::kQ + (threadIdx.x & 127) * 128;
+#pragma unroll
+        for (int half = 0; half < HD / 64; ++half) {
+          if (HD > 64) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) w[c] = live ? __ldg(src + half * 8 + c) : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const uint32_t ww[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+            uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = unpack_q(p.bf16, ww[e]);
+              o[e] = h2_as_u32(__floats2half2_rn(f.x * down, f.y * down));
+            }
+            sts128(dst + half * (128 * 128) + ((c ^ (threadIdx.x & 7)) << 4), o[0], o[1], o[2], o[3]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+        if (live) lim = min(a.lim0 + row / p.group, a.t1 - 1);
+      }
+      for (int step = 0; step < a.count; ++step, ++i) {
+        const int j0 = a.t0 + step * BN, stage = i & 1;
+        wait(const_full + stage, (i >> 1) & 1);
+        wait(s_full + t, i & 1);
+        tc_fence_after_sync();
+        const float4* cs = consts + stage * (BN / 16);
+        const int seen = lim - j0;  // columns up to here count
+        const bool cut = __any_sync(0xffffffffu, seen < BN - 1);
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) {
+          uint32_t s[32];
+          tmem_ld32(s_at + c * 32, s);
+          tmem_wait_ld();
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const float4 k = cs[2 * c + g];
+            float high = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float v = __uint_as_float(s[16 * g + e]);
+              high = fmaxf(high, !cut || 32 * c + 16 * g + e <= seen ? v : -INFINITY);
+            }
+            top = fmaxf(top, high == -INFINITY ? high : fmaf(high, fabsf(k.x) * qe, k.y));
+          }
+        }
+        // The reference point moves only when a weight would pass 2^8.
+        const bool grows = top > m + 8.f || m == kNoMax;
+        if (__any_sync(0xffffffffu, grows && top != -INFINITY)) {
+          float fade = 1.f;
+          if (grows && top != -INFINITY) {
+            fade = m == kNoMax ? 0.f : exp2_approx(m - top);
+            m = top;
+            l *= fade;
+          }
+          if (step > 0) {
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(o_at + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
+              tmem_st32(o_at + c * 32, o);
+            }
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) {
+          uint32_t s[32], w[16];
+          tmem_ld32(s_at + c * 32, s);
+          tmem_wait_ld();
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const float4 k = cs[2 * c + g];
+            const float mul = fabsf(k.x) * qe, add = k.y - m;
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              float x = exp2_approx(fmaf(__uint_as_float(s[16 * g + e]), mul, add));
+              float y = exp2_approx(fmaf(__uint_as_float(s[16 * g + e + 1]), mul, add));
+              if (cut) {
+                if (32 * c + 16 * g + e > seen) x = 0.f;
+                if (32 * c + 16 * g + e + 1 > seen) y = 0.f;
+              }
+              sum += x + y;
+              w[8 * g + e / 2] = h2_as_u32(__floats2half2_rn(x, y));
+            }
+            l = fmaf(sum, sum == 0.f ? 1.f : k.z, l);
+          }
+          tmem_st16(s_at + c * 16, w);
+        }
+        tmem_wait_st();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(const_empty + stage);
+          mbar_arrive(p_full + t);
+        }
+      }
+      if (a.count > 0) {
+        wait(o_full, seg & 1);
+        ++seg;
+        tc_fence_after_sync();
+      }
+      const int slot = (int)blockIdx.x * 2 + (a.opens ? 1 : 0);
+      float* part = parts + (size_t)slot * kRows * (HD + 2);
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t o[32];
+        if (a.count > 0) {
+          tmem_ld32(o_at + c * 32, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0;
+        }
+        if (!live) continue;
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float num[4] = {__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
+                                __uint_as_float(o[e + 3])};
+          if (a.whole)
+            store_out(p, a.start, a.h, row, c * 32 + e, num, l);
+          else
+            *reinterpret_cast<float4*>(part + (size_t)local * HD + c * 32 + e) = make_float4(num[0], num[1], num[2], num[3]);
+        }
+      }
+      tc_fence_before_sync();  // the next segment's products overwrite the output
+      if (!a.whole) {
+        if (live) *reinterpret_cast<float2*>(part + kRows * HD + 2 * local) = make_float2(m, l);
+        const int c0 = (int)(((a.first_step + 1) * C - 1) / all), c1 = (int)(((a.first_step + a.steps) * C - 1) / all);
+        __threadfence();
+        named_barrier_sync(1, 128 * QT);
+        if (threadIdx.x == 0) *last_one = atomicAdd(counters + c0, 1) == c1 - c0;
+        named_barrier_sync(1, 128 * QT);
+        if (*last_one) {
+          __threadfence();
+          if (live) {
+            float top = kNoMax, den = 0.f;
+            for (int c = c0; c <= c1; ++c)
+              top = fmaxf(top, __ldcg(parts + ((size_t)(2 * c + (c == c0)) * kRows) * (HD + 2) + kRows * HD + 2 * local));
+            for (int c = c0; c <= c1; ++c) {
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(parts + ((size_t)(2 * c + (c == c0)) * kRows) * (HD + 2) +
+                                                                       kRows * HD + 2 * local));
+              den = fmaf(ml.y, exp2_approx(ml.x - top), den);
+            }
+            for (int d = 0; d < HD; d += 4) {
+              float num[4] = {0.f, 0.f, 0.f, 0.f};
+              for (int c = c0; c <= c1; ++c) {
+                const float* from = parts + ((size_t)(2 * c + (c == c0)) * kRows) * (HD + 2);
+                const float f = exp2_approx(__ldcg(from + kRows * HD + 2 * local) - top);
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(from + (size_t)local * HD + d));
+                num[0] = fmaf(x.x, f, num[0]);
+                num[1] = fmaf(x.y, f, num[1]);
+                num[2] = fmaf(x.z, f, num[2]);
+                num[3] = fmaf(x.w, f, num[3]);
+              }
+              store_out(p, a.start, a.h, row, d, num, den);
+            }
+          }
+          if (threadIdx.x == 0) counters[c0] = 0;
+        }
+        named_barrier_sync(1, 128 * QT);  // *last_one is read before it is written again
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+}
+
+// Counters, then partial sums of two items per CTA.
+template <int HD>
+size_t tile_workspace(int sms) {
+  return kCounterBytes + (size_t)sms * 2 * TileLayout<HD>::kRows * (HD + 2) * 4;
+}
+
 struct CacheMapKey {
   uintptr_t ptr;
   long long rows;
@@ -853,14 +1447,37 @@ int launch_stream(const AttendArgs& a, const DeviceInfo& dev, void* workspace, s
   return e == cudaSuccess ? GDSQ_OK : cuda_fail(e, "attend launch");
 }
 
+// Rows per (request, KV head) up to which the stream kernel is taken.
+constexpr int kStreamRows = 16;
+
+template <int HD, int F>
+int launch_tile(const AttendArgs& a, const DeviceInfo& dev, void* workspace, size_t bytes, cudaStream_t stream) {
+  const size_t need = tile_workspace<HD>(dev.sms);
+  if (bytes < need)
+    return fail(GDSQ_ERR_INVALID_VALUE, "attend_kv8: workspace of %zu bytes, %zu needed", bytes, need);
+  if ((size_t)dev.sms * sizeof(int) > kCounterBytes) return fail(GDSQ_ERR_UNSUPPORTED, "attend_kv8: %d SMs", dev.sms);
+  const long long rows = ((long long)a.num_blocks * a.kv_heads) << a.block_shift;
+  CUtensorMap kmap, vmap;
+  int st = cache_map(dev, a.k_cache, rows, HD, &kmap);
+  if (st == GDSQ_OK) st = cache_map(dev, a.v_cache, rows, HD, &vmap);
+  if (st != GDSQ_OK) return st;
+  auto kernel = attend_tile_kernel<HD, F>;
+  constexpr int smem = TileLayout<HD>::kTotal;
+  cudaError_t e = ensure_smem(kernel, smem, dev.ordinal);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(attend)");
+  int* counters = static_cast<int*>(workspace);
+  float* parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
+  e = launch(kernel, dim3(dev.sms), dim3(kTileThreads), smem, stream, g_pdl_enabled != 0, a, kmap, vmap, parts, counters);
+  return e == cudaSuccess ? GDSQ_OK : cuda_fail(e, "attend launch");
+}
+
 template <int HD, int F>
 int launch_attend(const AttendArgs& a, int max_query_len, const DeviceInfo& dev, void* workspace, size_t bytes,
                   cudaStream_t stream) {
   const long long rows = (long long)max_query_len * a.group;
   if (rows <= 8) return launch_stream<HD, F, 1>(a, dev, workspace, bytes, stream);
-  if constexpr (HD != 256)
-    if (rows > 16) return launch_stream<HD, F, 4>(a, dev, workspace, bytes, stream);
-  return launch_stream<HD, F, 2>(a, dev, workspace, bytes, stream);
+  if (rows <= kStreamRows) return launch_stream<HD, F, 2>(a, dev, workspace, bytes, stream);
+  return launch_tile<HD, F>(a, dev, workspace, bytes, stream);
 }
 
 }  // namespace
@@ -884,11 +1501,11 @@ extern "C" size_t gdsq_attend_kv8_workspace(int num_requests, int max_query_len,
   const DeviceInfo* dev = nullptr;
   if (device_info(&dev) != GDSQ_OK) return 0;
   const long long rows = (long long)max_query_len * (num_heads / num_kv_heads);
-  auto of = [&](size_t one, size_t two, size_t four) { return rows <= 8 ? one : rows <= 16 ? two : four; };
-  if (head_dim == 64) return of(stream_workspace<64, 1>(dev->sms), stream_workspace<64, 2>(dev->sms), stream_workspace<64, 4>(dev->sms));
+  auto of = [&](size_t one, size_t two, size_t tile) { return rows <= 8 ? one : rows <= kStreamRows ? two : tile; };
+  if (head_dim == 64) return of(stream_workspace<64, 1>(dev->sms), stream_workspace<64, 2>(dev->sms), tile_workspace<64>(dev->sms));
   if (head_dim == 128)
-    return of(stream_workspace<128, 1>(dev->sms), stream_workspace<128, 2>(dev->sms), stream_workspace<128, 4>(dev->sms));
-  return of(stream_workspace<256, 1>(dev->sms), stream_workspace<256, 2>(dev->sms), stream_workspace<256, 2>(dev->sms));
+    return of(stream_workspace<128, 1>(dev->sms), stream_workspace<128, 2>(dev->sms), tile_workspace<128>(dev->sms));
+  return of(stream_workspace<256, 1>(dev->sms), stream_workspace<256, 2>(dev->sms), tile_workspace<256>(dev->sms));
 }
 
 extern "C" int gdsq_attend_kv8(const void* q, int elem_type, long long q_token_stride, long long q_head_stride,
