@@ -32,6 +32,7 @@
 #include <algorithm>
 #include <functional>
 #include <mutex>
+#include <type_traits>
 #include <unordered_map>
 
 #include "gdsq.h"
@@ -796,7 +797,7 @@ size_t stream_workspace(int sms) {
 //               TMEM, weights back to TMEM over them, in the end the output.
 //   warps 8-11  widen the 8-bit tiles to fp16
 //   warp 12     issues the products
-//   warp 13     TMA of the 8-bit tiles, and the blocks' scales
+//   warp 13     TMA of the 8-bit tiles, and the blocks' scales (14 and 15 idle)
 //
 // K and V are widened to the same layout, [64 dims][token][128 bytes], 128-byte
 // swizzled: K major for the scores (a row of B is a token) and N major for the
@@ -819,7 +820,9 @@ struct TileLayout {
   static constexpr int kNeed = kBars + 512 + 1024;
   static constexpr int kTotal = kNeed > 116 * 1024 ? kNeed : 116 * 1024;  // one CTA (512 TMEM columns) per SM
 };
-constexpr int kTileThreads = 14 * 32;
+constexpr int kTileThreads = 16 * 32;
+// Registers per thread of the softmax, widening and other warp groups: together the launch's 4 x 128.
+constexpr int kSoftmaxRegs = 176, kWidenRegs = 80, kOtherRegs = 80;
 
 __device__ __forceinline__ void tc_mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                               uint32_t accumulate) {
@@ -847,18 +850,25 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-// Each lane stores 32 consecutive 32-bit columns of its own TMEM lane.
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
-      "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
-      "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
 }
-
+__device__ __forceinline__ float2 add2f(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 template <int HD, int F>
 __global__ void __launch_bounds__(kTileThreads, 1)
     attend_tile_kernel(const AttendArgs p, const __grid_constant__ CUtensorMap kmap,
@@ -1021,6 +1031,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   };
 
   Segment a;
+  if (warp >= 12) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == kTmaWarp) {
     uint32_t i = 0;  // steps so far
     while (next_segment(a))
@@ -1117,7 +1129,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       commit(o_full);
     }
+  }
   } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWidenRegs));
     // widen: 16 codes of one token at a time
     const int tid = threadIdx.x - 256;
     uint32_t i = 0;
@@ -1158,7 +1172,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
         }
       }
-  } else if (warp < 4 * QT) {
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    if (warp < 4 * QT) {
     const int t = warp >> 2;                       // tile
     const int local = t * 128 + (threadIdx.x & 127);  // row of the item
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;  // TMEM lane (warp % 4) * 32 in the address
@@ -1226,70 +1242,75 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const float4* cs = consts + stage * (BN / 16);
         const int seen = lim - j0;  // columns up to here count
         const bool cut = __any_sync(0xffffffffu, seen < BN - 1);
-        float top = -INFINITY;
+        uint32_t s[BN / 32][32];
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) {
-          uint32_t s[32];
-          tmem_ld32(s_at + c * 32, s);
-          tmem_wait_ld();
+        for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_at + c * 32, s[c]);
+        tmem_wait_ld();
+        auto softmax = [&](auto masked) {
+          constexpr bool kCut = decltype(masked)::value;
+          float top = -INFINITY;
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float4 k = cs[2 * c + g];
-            float high = -INFINITY;
+          for (int c = 0; c < BN / 32; ++c)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float v = __uint_as_float(s[16 * g + e]);
-              high = fmaxf(high, !cut || 32 * c + 16 * g + e <= seen ? v : -INFINITY);
-            }
-            top = fmaxf(top, high == -INFINITY ? high : fmaf(high, fabsf(k.x) * qe, k.y));
-          }
-        }
-        // The reference point moves only when a weight would pass 2^8.
-        const bool grows = top > m + 8.f || m == kNoMax;
-        if (__any_sync(0xffffffffu, grows && top != -INFINITY)) {
-          float fade = 1.f;
-          if (grows && top != -INFINITY) {
-            fade = m == kNoMax ? 0.f : exp2_approx(m - top);
-            m = top;
-            l *= fade;
-          }
-          if (step > 0) {
-#pragma unroll 1
-            for (int c = 0; c < HD / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(o_at + c * 32, o);
-              tmem_wait_ld();
+            for (int g = 0; g < 2; ++g) {
+              const float4 k = cs[2 * c + g];
+              float high = -INFINITY;
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
-              tmem_st32(o_at + c * 32, o);
-            }
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < BN / 32; ++c) {
-          uint32_t s[32], w[16];
-          tmem_ld32(s_at + c * 32, s);
-          tmem_wait_ld();
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float4 k = cs[2 * c + g];
-            const float mul = fabsf(k.x) * qe, add = k.y - m;
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              float x = exp2_approx(fmaf(__uint_as_float(s[16 * g + e]), mul, add));
-              float y = exp2_approx(fmaf(__uint_as_float(s[16 * g + e + 1]), mul, add));
-              if (cut) {
-                if (32 * c + 16 * g + e > seen) x = 0.f;
-                if (32 * c + 16 * g + e + 1 > seen) y = 0.f;
+              for (int e = 0; e < 16; ++e) {
+                const float v = __uint_as_float(s[c][16 * g + e]);
+                high = fmaxf(high, !kCut || 32 * c + 16 * g + e <= seen ? v : -INFINITY);
               }
-              sum += x + y;
-              w[8 * g + e / 2] = h2_as_u32(__floats2half2_rn(x, y));
+              const float z = fmaf(high, fabsf(k.x) * qe, k.y);
+              top = fmaxf(top, !kCut || high != -INFINITY ? z : -INFINITY);
             }
-            l = fmaf(sum, sum == 0.f ? 1.f : k.z, l);
+          // The reference point moves only when a weight would pass 2^8.
+          const bool grows = (top > m + 8.f || m == kNoMax) && top > -INFINITY;
+          if (__any_sync(0xffffffffu, grows)) {
+            float fade = 1.f;
+            if (grows) {
+              fade = m == kNoMax ? 0.f : exp2_approx(m - top);
+              m = top;
+              l *= fade;
+            }
+            if (step > 0) {
+#pragma unroll 1
+              for (int c = 0; c < HD / 16; ++c) {
+                uint32_t o[16];
+                tmem_ld16(o_at + c * 16, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
+                tmem_st16(o_at + c * 16, o);
+              }
+            }
           }
-          tmem_st16(s_at + c * 16, w);
-        }
+#pragma unroll
+          for (int c = 0; c < BN / 32; ++c) {
+            uint32_t w[16];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              const float4 k = cs[2 * c + g];
+              const float mul = fabsf(k.x) * qe, add = k.y - m;
+              const float2 mul2 = make_float2(mul, mul), add2 = make_float2(add, add);
+              float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int e = 0; e < 16; e += 2) {
+                const float2 z = fma2(make_float2(__uint_as_float(s[c][16 * g + e]), __uint_as_float(s[c][16 * g + e + 1])), mul2, add2);
+                float2 x = make_float2(exp2_approx(z.x), exp2_approx(z.y));
+                if (kCut) {
+                  if (32 * c + 16 * g + e > seen) x.x = 0.f;
+                  if (32 * c + 16 * g + e + 1 > seen) x.y = 0.f;
+                }
+                sum = add2f(sum, x);
+                w[8 * g + e / 2] = h2_as_u32(__floats2half2_rn(x.x, x.y));
+              }
+              l = fmaf(sum.x + sum.y, k.z, l);
+            }
+            tmem_st16(s_at + c * 16, w);
+          }
+        };
+        if (cut) softmax(std::true_type{});
+        else softmax(std::false_type{});
         tmem_wait_st();
         tc_fence_before_sync();
         __syncwarp();
@@ -1363,6 +1384,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         named_barrier_sync(1, 128 * QT);  // *last_one is read before it is written again
       }
+    }
     }
   }
   tc_fence_before_sync();
