@@ -803,8 +803,8 @@ size_t stream_workspace(int sms) {
 // swizzled: K major for the scores (a row of B is a token) and N major for the
 // output (a column of B is a dim).  With two tiles the order of products is
 // O0(i) S0(i+1) O1(i) S1(i+1), so that one tile's softmax runs beside the other's
-// products; the weights take the scores' place in TMEM.  The widened tiles need
-// no second buffer: scores i are done long before K i+1 is needed.
+// products; the weights take the scores' place in TMEM.  Widened K needs no second
+// buffer: scores i are done long before K i+1 is needed; V has two.
 
 template <int HD>
 struct TileLayout {
@@ -814,7 +814,7 @@ struct TileLayout {
   static constexpr int kQ = 128 * HD * 2;        // one tile of Q
   static constexpr int kWide = BN * HD * 2;      // K or V of a step in fp16
   static constexpr int kRaw = BN * HD;           // in 8 bits
-  static constexpr int kKOff = QT * kQ, kVOff = kKOff + kWide, kRawOff = kVOff + kWide;
+  static constexpr int kKOff = QT * kQ, kVOff = kKOff + kWide, kRawOff = kVOff + 2 * kWide;  // V twice
   static constexpr int kConst = kRawOff + 4 * kRaw;  // [2][BN / 16] float4
   static constexpr int kBars = kConst + 2 * (BN / 16) * 16;
   static constexpr int kNeed = kBars + 512 + 1024;
@@ -824,32 +824,64 @@ constexpr int kTileThreads = 16 * 32;
 // Registers per thread of the softmax, widening and other warp groups: together the launch's 4 x 128.
 constexpr int kSoftmaxRegs = 176, kWidenRegs = 80, kOtherRegs = 80;
 
-__device__ __forceinline__ void tc_mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                              uint32_t accumulate) {
+// The whole warp calls these and the lane with leader != 0 issues, so that the
+// code around them is not divergent and their operands stay in uniform
+// registers: issued from a branch of one lane, a product took 110 cycles to
+// issue, twice its own time.  Descriptors are given by their low word.
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t a_hi, uint32_t b_hi,
+                                       uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      "{\n\t.reg .pred e, p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 e, %0, 0;\n\tsetp.ne.b32 p, %7, 0;\n\t"
+      "mov.b64 a, {%2, %4};\n\tmov.b64 b, {%3, %5};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%1], a, b, %6, p;\n\t}" ::"r"(leader),
+      "r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(a_hi), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred e, p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 e, %0, 0;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 b, {%3, %4};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], b, %5, p;\n\t}" ::"r"(leader),
+      "r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void commit_by(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %0, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}" ::"r"(leader),
+      "r"(smem_addr(bar))
       : "memory");
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle: 8 rows of 128 bytes per
 // 1024-byte atom.  K major: `sbo` bytes between groups of 8 rows.  N major:
 // `sbo` bytes between groups of 8 K rows, `lbo` between blocks of 64 columns.
-__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-  d |= (uint64_t)((lbo >> 4) & 0x3FFFu) << 16;
-  d |= (uint64_t)((sbo >> 4) & 0x3FFFu) << 32;
-  d |= (uint64_t)1 << 46;  // descriptor version for sm_100
-  d |= (uint64_t)2 << 61;  // 128-byte swizzle
-  return d;
+// Low word (the start and `lbo`) and high word of the descriptor.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return ((saddr >> 4) & 0x3FFFu) | ((lbo >> 4) & 0x3FFFu) << 16; }
+__host__ __device__ constexpr uint32_t desc_hi(uint32_t sbo) {
+  return ((sbo >> 4) & 0x3FFFu) | 1u << 14 | 2u << 29;  // version for sm_100, 128-byte swizzle
 }
 
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {  // does not block
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
+__device__ __forceinline__ float max4(float a, float b, float c, float d) { return fmaxf(fmaxf(a, b), fmaxf(c, d)); }
+
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -883,8 +915,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
   uint64_t* raw_full = bars;        // [2][K, V]
   uint64_t* raw_empty = bars + 4;   // [2][K, V]
-  uint64_t* wide_full = bars + 8;   // [K, V]
-  uint64_t* wide_empty = bars + 10; // [K, V]
+  uint64_t* wide_full = bars + 8;   // [K, V even, V odd]
+  uint64_t* wide_empty = bars + 44; // [K, V even, V odd]
   uint64_t* s_full = bars + 12;     // [QT]
   uint64_t* p_full = bars + 14;     // [QT]
   uint64_t* o_full = bars + 16;
@@ -898,7 +930,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint64_t* const_empty = bars + 42;  // [2]
   const float4* consts = reinterpret_cast<const float4*>(smem + L::kConst);  // [2][BN / 16]
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // From one lane, so that the compiler knows the roles' branches to be uniform.
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   constexpr int kMmaWarp = 12, kTmaWarp = 13;
   if (warp == kTmaWarp && lane == 0) {
     for (int i = 0; i < 4; ++i) {
@@ -906,12 +939,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(raw_empty + i, 4);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(wide_full + i, 4);
-      mbar_init(wide_empty + i, 1);
       mbar_init(s_full + i, 1);
       mbar_init(p_full + i, 4);
       mbar_init(const_full + i, 1);
       mbar_init(const_empty + i, 4 * QT);
+    }
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(wide_full + i, 4);
+      mbar_init(wide_empty + i, 1);
     }
     mbar_init(o_full, 1);
     mbar_init(q_full, 4 * QT);
@@ -1023,7 +1058,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   };
   // Waits of one warp; once one has run out nobody waits any more.
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (*dead) return;
+    if (mbar_test_wait(bar, parity) || *dead) return;
     if (!mbar_wait(bar, parity)) {
       record_device_error(kDevErrBarrierTimeout);
       *dead = 1;
@@ -1075,50 +1110,44 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | (8u << 24);
     constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // B is N major
     uint32_t i = 0, seg = 0;
+    const uint32_t leader = lane == 0;
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint32_t q_lo = desc_lo(sbase, 16), k_lo = desc_lo(sbase + L::kKOff, 16), v_lo = desc_lo(sbase + L::kVOff, BN * 128);
+    constexpr uint32_t kHi = desc_hi(1024);
     auto scores = [&](int t) {
-      if (lane == 0) {
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-          const uint64_t qa = smem_desc_sw128(sbase + t * L::kQ + (k / 4) * (128 * 128) + (k % 4) * 32, 16, 1024);
-          const uint64_t kb = smem_desc_sw128(sbase + L::kKOff + (k / 4) * (BN * 128) + (k % 4) * 32, 16, 1024);
-          tc_mma_f16_ss(tmem + t * BN, qa, kb, kIdescS, k > 0);
-        }
-        tc_commit(s_full + t);
-      }
-      __syncwarp();
+      for (int k = 0; k < HD / 16; ++k)
+        mma_ss(leader, tm + t * BN, q_lo + ((t * L::kQ + (k / 4) * (128 * 128) + (k % 4) * 32) >> 4),
+               k_lo + (((k / 4) * (BN * 128) + (k % 4) * 32) >> 4), kHi, kHi, kIdescS, k > 0);
+      commit_by(leader, s_full + t);
     };
-    auto output = [&](int t, bool first) {
-      if (lane == 0) {
+    auto output = [&](int t, bool first, uint32_t buffer) {
 #pragma unroll
-        for (int k = 0; k < BN / 16; ++k) {
-          const uint64_t vb = smem_desc_sw128(sbase + L::kVOff + k * 2048, BN * 128, 1024);
-          tc_mma_f16_ts(tmem + kOCol + t * HD, tmem + t * BN + k * 8, vb, kIdescO, !(first && k == 0));
-        }
-      }
-      __syncwarp();
+      for (int k = 0; k < BN / 16; ++k)
+        mma_ts(leader, tm + kOCol + t * HD, tm + t * BN + k * 8, v_lo + buffer * (L::kWide >> 4) + k * (2048 >> 4), kHi, kIdescO,
+               !(first && k == 0));
     };
-    auto commit = [&](uint64_t* bar) {
-      if (lane == 0) tc_commit(bar);
-      __syncwarp();
-    };
-    while (next_segment(a)) {
-      if (a.count == 0) continue;
+    auto commit = [&](uint64_t* bar) { commit_by(leader, bar); };
+    while (__shfl_sync(0xffffffffu, (int)next_segment(a), 0)) {
+      const int count = __shfl_sync(0xffffffffu, a.count, 0);
+      if (count == 0) continue;
       wait(q_full, seg & 1);
       ++seg;
       tc_fence_after_sync();
       wait(wide_full + 0, i & 1);
       tc_fence_after_sync();
+#pragma unroll
       for (int t = 0; t < QT; ++t) scores(t);
       commit(wide_empty + 0);
-      for (int step = 0; step < a.count; ++step, ++i) {
-        const bool more = step + 1 < a.count;
-        wait(wide_full + 1, i & 1);
+      for (int step = 0; step < count; ++step, ++i) {
+        const bool more = step + 1 < count;
+        wait(wide_full + 1 + (i & 1), (i >> 1) & 1);
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
           wait(p_full + t, i & 1);
           tc_fence_after_sync();
-          output(t, step == 0);
-          if (t == QT - 1) commit(wide_empty + 1);
+          output(t, step == 0, i & 1);
+          if (t == QT - 1) commit(wide_empty + 1 + (i & 1));
           if (more) {
             if (t == 0) wait(wide_full + 0, (i + 1) & 1);
             tc_fence_after_sync();
@@ -1141,9 +1170,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           wait(raw_full + 2 * stage + kv, (i >> 1) & 1);
-          if (i >= 1) wait(wide_empty + kv, (i - 1) & 1);
+          // K has one buffer, V two
+          if (kv == 0 && i >= 1) wait(wide_empty, (i - 1) & 1);
+          if (kv == 1 && i >= 2) wait(wide_empty + 1 + (i & 1), ((i >> 1) - 1) & 1);
           const uint32_t raw = sbase + L::kRawOff + (2 * stage + kv) * L::kRaw;
-          const uint32_t wide = sbase + (kv ? L::kVOff : L::kKOff);
+          const uint32_t wide = sbase + (kv ? L::kVOff + (i & 1) * L::kWide : L::kKOff);
 #pragma unroll 4
           for (int j = 0; j < BN * (HD / 16) / 128; ++j) {
             const int unit = tid + j * 128, tok = unit % BN, c = unit / BN;  // chunk of 16 dims
@@ -1168,7 +1199,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           __syncwarp();
           if (lane == 0) {
             mbar_arrive(raw_empty + 2 * stage + kv);
-            mbar_arrive(wide_full + kv);
+            mbar_arrive(wide_full + (kv ? 1 + (i & 1) : 0));
           }
         }
       }
@@ -1254,12 +1285,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
               const float4 k = cs[2 * c + g];
-              float high = -INFINITY;
+              float v[16];
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
-                const float v = __uint_as_float(s[c][16 * g + e]);
-                high = fmaxf(high, !kCut || 32 * c + 16 * g + e <= seen ? v : -INFINITY);
+                v[e] = __uint_as_float(s[c][16 * g + e]);
+                if (kCut && 32 * c + 16 * g + e > seen) v[e] = -INFINITY;
               }
+              const float high = fmaxf(fmaxf(max4(v[0], v[1], v[2], v[3]), max4(v[4], v[5], v[6], v[7])),
+                                       fmaxf(max4(v[8], v[9], v[10], v[11]), max4(v[12], v[13], v[14], v[15])));
               const float z = fmaf(high, fabsf(k.x) * qe, k.y);
               top = fmaxf(top, !kCut || high != -INFINITY ? z : -INFINITY);
             }
