@@ -164,6 +164,20 @@ __device__ __forceinline__ void store_out(const AttendArgs& p, int start, int h,
   *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + at) = v;
 }
 
+// Eight dims of one output row.
+__device__ __forceinline__ void store_out8(const AttendArgs& p, int start, int h, int row, int d, const float (&num)[8], float inv) {
+  const long long at = (long long)(start + row / p.group) * p.out_token_stride +
+                       (long long)(h * p.group + row % p.group) * p.out_head_stride + d;
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = num[2 * i] * inv, y = num[2 * i + 1] * inv;
+    const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+    w[i] = p.bf16 ? *reinterpret_cast<const uint32_t*>(&b) : h2_as_u32(__floats2half2_rn(x, y));
+  }
+  *reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // Per-page constants of the softmax: x = kscale factor, y = lv, z = 2^-lv.
 __device__ __forceinline__ float3 page_constants(const AttendArgs& p, int page, int h, float log_factor) {
   const size_t i = (size_t)page * p.kv_heads + h;
@@ -880,8 +894,6 @@ __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
   return done != 0;
 }
 
-__device__ __forceinline__ float max4(float a, float b, float c, float d) { return fmaxf(fmaxf(a, b), fmaxf(c, d)); }
-
 // Two fp32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -1273,53 +1285,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const float4* cs = consts + stage * (BN / 16);
         const int seen = lim - j0;  // columns up to here count
         const bool cut = __any_sync(0xffffffffu, seen < BN - 1);
-        uint32_t s[BN / 32][32];
-#pragma unroll
-        for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_at + c * 32, s[c]);
-        tmem_wait_ld();
-        auto softmax = [&](auto masked) {
+        // Weights against the reference point m, in one pass; `over`: one has passed 2^8, which is not stored.
+        uint32_t w[BN / 2];
+        float more = 0.f;
+        bool over = false;
+        auto weights = [&](auto masked) {
           constexpr bool kCut = decltype(masked)::value;
-          float top = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < BN / 32; ++c)
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              const float4 k = cs[2 * c + g];
-              float v[16];
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                v[e] = __uint_as_float(s[c][16 * g + e]);
-                if (kCut && 32 * c + 16 * g + e > seen) v[e] = -INFINITY;
-              }
-              const float high = fmaxf(fmaxf(max4(v[0], v[1], v[2], v[3]), max4(v[4], v[5], v[6], v[7])),
-                                       fmaxf(max4(v[8], v[9], v[10], v[11]), max4(v[12], v[13], v[14], v[15])));
-              const float z = fmaf(high, fabsf(k.x) * qe, k.y);
-              top = fmaxf(top, !kCut || high != -INFINITY ? z : -INFINITY);
-            }
-          // The reference point moves only when a weight would pass 2^8.
-          const bool grows = (top > m + 8.f || m == kNoMax) && top > -INFINITY;
-          if (__any_sync(0xffffffffu, grows)) {
-            float fade = 1.f;
-            if (grows) {
-              fade = m == kNoMax ? 0.f : exp2_approx(m - top);
-              m = top;
-              l *= fade;
-            }
-            if (step > 0) {
-#pragma unroll 1
-              for (int c = 0; c < HD / 16; ++c) {
-                uint32_t o[16];
-                tmem_ld16(o_at + c * 16, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
-                tmem_st16(o_at + c * 16, o);
-              }
-            }
-          }
+          __half2 high = __float2half2_rn(0.f);
+          more = 0.f;
 #pragma unroll
           for (int c = 0; c < BN / 32; ++c) {
-            uint32_t w[16];
+            uint32_t s[32];
+            tmem_ld32(s_at + c * 32, s);
+            tmem_wait_ld();
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
               const float4 k = cs[2 * c + g];
@@ -1328,22 +1306,72 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
               for (int e = 0; e < 16; e += 2) {
-                const float2 z = fma2(make_float2(__uint_as_float(s[c][16 * g + e]), __uint_as_float(s[c][16 * g + e + 1])), mul2, add2);
+                const float2 z = fma2(make_float2(__uint_as_float(s[16 * g + e]), __uint_as_float(s[16 * g + e + 1])), mul2, add2);
                 float2 x = make_float2(exp2_approx(z.x), exp2_approx(z.y));
                 if (kCut) {
                   if (32 * c + 16 * g + e > seen) x.x = 0.f;
                   if (32 * c + 16 * g + e + 1 > seen) x.y = 0.f;
                 }
                 sum = add2f(sum, x);
-                w[8 * g + e / 2] = h2_as_u32(__floats2half2_rn(x.x, x.y));
+                const __half2 h = __floats2half2_rn(x.x, x.y);
+                high = __hmax2(high, h);
+                w[16 * c + 8 * g + e / 2] = h2_as_u32(h);
               }
-              l = fmaf(sum.x + sum.y, k.z, l);
+              more = fmaf(sum.x + sum.y, k.z, more);
             }
-            tmem_st16(s_at + c * 16, w);
           }
+          over = __half2float(__hmax(__low2half(high), __high2half(high))) > 256.f;
         };
-        if (cut) softmax(std::true_type{});
-        else softmax(std::false_type{});
+        auto both = [&](auto f) {
+          if (cut) f(std::true_type{});
+          else f(std::false_type{});
+        };
+        if (step > 0) both(weights);
+        // The reference point moves only then, and in a segment's first step.
+        if (step == 0 || __any_sync(0xffffffffu, over || m == kNoMax)) {
+          float top = -INFINITY;
+          both([&](auto masked) {
+            constexpr bool kCut = decltype(masked)::value;
+#pragma unroll 1
+            for (int c = 0; c < BN / 16; ++c) {
+              uint32_t s[16];
+              tmem_ld16(s_at + c * 16, s);
+              tmem_wait_ld();
+              const float4 k = cs[c];
+              float high = -INFINITY;
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (!kCut || 16 * c + e <= seen) high = fmaxf(high, __uint_as_float(s[e]));
+              if (high > -INFINITY) top = fmaxf(top, fmaf(high, fabsf(k.x) * qe, k.y));
+            }
+          });
+          float fade = 1.f;
+          if (top > -INFINITY && (top > m || m == kNoMax)) {
+            fade = m == kNoMax ? 0.f : exp2_approx(m - top);
+            m = top;
+            l *= fade;
+          }
+          if (step > 0) {
+#pragma unroll 1
+            for (int c = 0; c < HD / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(o_at + c * 16, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
+              tmem_st16(o_at + c * 16, o);
+            }
+          }
+          both(weights);
+        }
+        l += more;
+#pragma unroll
+        for (int c = 0; c < BN / 32; ++c) {
+          uint32_t out[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) out[e] = w[16 * c + e];
+          tmem_st16(s_at + c * 16, out);
+        }
         tmem_wait_st();
         tc_fence_before_sync();
         __syncwarp();
@@ -1369,15 +1397,22 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0;
         }
+        // partial sums: [4 dims][row], so that a warp writes 32 rows side by side
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         if (!live) continue;
+        if (a.whole) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float num[4] = {__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
-                                __uint_as_float(o[e + 3])};
-          if (a.whole)
-            store_out(p, a.start, a.h, row, c * 32 + e, num, l);
-          else
-            *reinterpret_cast<float4*>(part + (size_t)local * HD + c * 32 + e) = make_float4(num[0], num[1], num[2], num[3]);
+          for (int e = 0; e < 32; e += 8) {
+            float num[8];
+#pragma unroll
+            for (int y = 0; y < 8; ++y) num[y] = __uint_as_float(o[e + y]);
+            store_out8(p, a.start, a.h, row, c * 32 + e, num, inv);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<uint4*>(part + ((size_t)((c * 32 + e) / 4) * kRows + local) * 4) =
+                make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         }
       }
       tc_fence_before_sync();  // the next segment's products overwrite the output
@@ -1391,26 +1426,39 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (*last_one) {
           __threadfence();
           if (live) {
+            auto from = [&](int c) { return parts + ((size_t)(2 * c + (c == c0)) * kRows) * (HD + 2); };
             float top = kNoMax, den = 0.f;
-            for (int c = c0; c <= c1; ++c)
-              top = fmaxf(top, __ldcg(parts + ((size_t)(2 * c + (c == c0)) * kRows) * (HD + 2) + kRows * HD + 2 * local));
+            for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(from(c) + kRows * HD + 2 * local));
             for (int c = c0; c <= c1; ++c) {
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(parts + ((size_t)(2 * c + (c == c0)) * kRows) * (HD + 2) +
-                                                                       kRows * HD + 2 * local));
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(from(c) + kRows * HD + 2 * local));
               den = fmaf(ml.y, exp2_approx(ml.x - top), den);
             }
-            for (int d = 0; d < HD; d += 4) {
-              float num[4] = {0.f, 0.f, 0.f, 0.f};
+            const float inv = den == 0.f ? 0.f : 1.f / den;
+#pragma unroll 1
+            for (int d = 0; d < HD; d += 32) {
+              float num[32];
+#pragma unroll
+              for (int y = 0; y < 32; ++y) num[y] = 0.f;
               for (int c = c0; c <= c1; ++c) {
-                const float* from = parts + ((size_t)(2 * c + (c == c0)) * kRows) * (HD + 2);
-                const float f = exp2_approx(__ldcg(from + kRows * HD + 2 * local) - top);
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(from + (size_t)local * HD + d));
-                num[0] = fmaf(x.x, f, num[0]);
-                num[1] = fmaf(x.y, f, num[1]);
-                num[2] = fmaf(x.z, f, num[2]);
-                num[3] = fmaf(x.w, f, num[3]);
+                const float f = exp2_approx(__ldcg(from(c) + kRows * HD + 2 * local) - top);
+                float4 x[8];
+#pragma unroll
+                for (int y = 0; y < 8; ++y) x[y] = __ldcg(reinterpret_cast<const float4*>(from(c) + ((size_t)(d / 4 + y) * kRows + local) * 4));
+#pragma unroll
+                for (int y = 0; y < 8; ++y) {
+                  num[4 * y] = fmaf(x[y].x, f, num[4 * y]);
+                  num[4 * y + 1] = fmaf(x[y].y, f, num[4 * y + 1]);
+                  num[4 * y + 2] = fmaf(x[y].z, f, num[4 * y + 2]);
+                  num[4 * y + 3] = fmaf(x[y].w, f, num[4 * y + 3]);
+                }
               }
-              store_out(p, a.start, a.h, row, d, num, den);
+#pragma unroll
+              for (int y = 0; y < 32; y += 8) {
+                float out[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) out[e] = num[y + e];
+                store_out8(p, a.start, a.h, row, d + y, out, inv);
+              }
             }
           }
           if (threadIdx.x == 0) counters[c0] = 0;
