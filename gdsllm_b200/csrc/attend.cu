@@ -1233,14 +1233,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const long long q_at = (long long)(a.start + (live ? row : 0) / p.group) * p.q_token_stride +
                                (long long)(a.h * p.group + (live ? row : 0) % p.group) * p.q_head_stride;
         const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + q_at);
+        constexpr int kBatch = HD == 256 ? 16 : HD / 8;  // 16-byte vectors in registers (half of a row of 256)
         float most = 0.f;
-        uint4 w[8];
+        uint4 w[kBatch];
 #pragma unroll
-        for (int half = 0; half < HD / 64; ++half) {
+        for (int half = 0; half < HD / 8 / kBatch; ++half) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) w[c] = live ? __ldg(src + half * 8 + c) : make_uint4(0, 0, 0, 0);
+          for (int c = 0; c < kBatch; ++c) w[c] = live ? __ldg(src + half * kBatch + c) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
+          for (int c = 0; c < kBatch; ++c) {
             const uint32_t ww[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -1255,13 +1256,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         qe = __uint_as_float((uint32_t)(127 + ex) << 23);
         const uint32_t dst = sbase + t * L::kQ + (threadIdx.x & 127) * 128;
 #pragma unroll
-        for (int half = 0; half < HD / 64; ++half) {
-          if (HD > 64) {
+        for (int half = 0; half < HD / 8 / kBatch; ++half) {
+          if (HD == 256) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) w[c] = live ? __ldg(src + half * 8 + c) : make_uint4(0, 0, 0, 0);
+            for (int c = 0; c < kBatch; ++c) w[c] = live ? __ldg(src + half * kBatch + c) : make_uint4(0, 0, 0, 0);
           }
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
+          for (int c = 0; c < kBatch; ++c) {
             const uint32_t ww[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
             uint32_t o[4];
 #pragma unroll
@@ -1269,7 +1270,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               const float2 f = unpack_q(p.bf16, ww[e]);
               o[e] = h2_as_u32(__floats2half2_rn(f.x * down, f.y * down));
             }
-            sts128(dst + half * (128 * 128) + ((c ^ (threadIdx.x & 7)) << 4), o[0], o[1], o[2], o[3]);
+            const int v = half * kBatch + c;
+            sts128(dst + (v / 8) * (128 * 128) + (((v % 8) ^ (threadIdx.x & 7)) << 4), o[0], o[1], o[2], o[3]);
           }
         }
         fence_proxy_async_smem();
@@ -1293,11 +1295,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           constexpr bool kCut = decltype(masked)::value;
           __half2 high = __float2half2_rn(0.f);
           more = 0.f;
+          uint32_t ahead[2][32];  // the next 32 scores are on their way while these are worked on
+          tmem_ld32(s_at, ahead[0]);
 #pragma unroll
           for (int c = 0; c < BN / 32; ++c) {
-            uint32_t s[32];
-            tmem_ld32(s_at + c * 32, s);
             tmem_wait_ld();
+            if (c + 1 < BN / 32) tmem_ld32(s_at + (c + 1) * 32, ahead[(c + 1) & 1]);
+            const uint32_t(&s)[32] = ahead[c & 1];
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
               const float4 k = cs[2 * c + g];
