@@ -835,6 +835,9 @@ struct TileLayout {
   static constexpr int kTotal = kNeed > 116 * 1024 ? kNeed : 116 * 1024;  // one CTA (512 TMEM columns) per SM
 };
 constexpr int kTileThreads = 16 * 32;
+// What beginning and ending an item costs, in tokens of a step's time: with 11
+// steps of 128 prompts of 2048 tokens take 597 us, with 2 728 and with 15 611.
+constexpr int kItemTokens = 1408;
 // Registers per thread of the softmax, widening and other warp groups: together the launch's 4 x 128.
 constexpr int kSoftmaxRegs = 176, kWidenRegs = 80, kOtherRegs = 80;
 
@@ -974,12 +977,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   pdl_launch_dependents();
   pdl_wait_primary();
 
-  // The schedule, as in attend_stream_kernel.
+  // The schedule, in tokens: tile j of a request's rows counts an item's fixed cost
+  // and about the tokens that it sees, `first` + j * `rise`, whose running sum is
+  // quadratic in j.  A step belongs to the CTA whose share its first token falls in.
   const int most_len = p.table_width << p.block_shift;
+  const int rise = ceil_div(kRows, p.group);
   auto rows_of = [&](int r) { return max(min(p.starts[r + 1], p.tokens) - max(p.starts[r], 0), 0) * p.group; };
-  auto cost_of = [&](int r) {
-    return (long long)ceil_div(rows_of(r), kRows) * p.kv_heads * (max(ceil_div(min(p.seq_lens[r], most_len), BN), 1) + kItemCost);
+  auto first_of = [&](int r) {  // cost of the first row tile
+    const int n = max(min(p.starts[r + 1], p.tokens) - max(p.starts[r], 0), 0);
+    return (long long)kItemTokens + max(min(p.seq_lens[r], most_len) - n, 0) + rise + 1;
   };
+  auto upto_tile = [&](long long first, long long j) { return j * first + j * (j - 1) / 2 * rise; };
+  auto cost_of = [&](int r) { return upto_tile(first_of(r), ceil_div(rows_of(r), kRows)) * p.kv_heads; };
   long long all, s0, s1, request_at;
   const int per = ceil_div(p.requests, kTileThreads);
   const int ra = min((int)threadIdx.x * per, p.requests), rb = min(ra + per, p.requests);
@@ -1002,8 +1011,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (w < warp) before += shared_ll[w];
     all += shared_ll[w];
   }
-  const long long C = min((long long)gridDim.x, all);
-  const bool works = blockIdx.x < C;
+  const long long C = max(min((long long)gridDim.x, all / BN), 1ll);  // a share holds a step at least
+  const bool works = blockIdx.x < C && all > 0;
   s0 = works ? all * blockIdx.x / C : 0;
   s1 = works ? all * (blockIdx.x + 1) / C : 0;
   if (works && before <= s0 && s0 < before + mine) {
@@ -1024,8 +1033,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   struct Segment {
     int r, h, row0, rows, start, lim0;  // row i of the item sees positions up to lim0 + (row0 + i) / group
     int t0, t1, count;                  // first token, the end, and the steps
-    int kv_len, steps;
-    long long first_step;
+    int steps;              // of the item
+    long long first_token;  // of the item, in the schedule
     bool opens, whole;
   };
   auto next_segment = [&](Segment& a) {
@@ -1036,34 +1045,41 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const int row_tiles = ceil_div(rows, kRows);
       const int len = min(p.seq_lens[r], most_len);
       if (len < p.seq_lens[r]) record_device_error(kDevErrBadIndex);
-      const int steps = max(ceil_div(len, BN), 1), cost = steps + kItemCost;
-      const long long request_cost = (long long)row_tiles * p.kv_heads * cost;
-      if (s0 >= request_at + request_cost) {
-        request_at += request_cost;
+      const long long first = first_of(r), head_cost = upto_tile(first, row_tiles);
+      if (s0 >= request_at + head_cost * p.kv_heads) {
+        request_at += head_cost * p.kv_heads;
         ++r;
         continue;
       }
-      const int item = (int)((s0 - request_at) / cost);
-      const long long first_step = request_at + (long long)item * cost + kItemCost;
-      const int step = (int)max(s0 - first_step, 0ll);
-      s0 = first_step + step;
-      if (s0 >= s1) return false;
-      const int step_end = (int)min((long long)steps, step + (s1 - s0));
-      s0 += step_end - step;
+      const int h = (int)((s0 - request_at) / head_cost);
+      const long long in_head = s0 - request_at - h * head_cost;
+      int tile = 0;
+      for (int end = row_tiles; end - tile > 1;) {  // the last tile that begins at or before it
+        const int mid = (tile + end) >> 1;
+        if (upto_tile(first, mid) <= in_head) tile = mid;
+        else end = mid;
+      }
+      const long long item_at = request_at + h * head_cost + upto_tile(first, tile);
+      const long long item_end = item_at + first + (long long)tile * rise;
+      a.first_token = item_at + kItemTokens;
       a.r = r;
-      a.h = item / row_tiles;
-      a.row0 = (item % row_tiles) * kRows;
+      a.h = h;
+      a.row0 = tile * kRows;
       a.rows = rows;
       a.start = start;
       a.lim0 = len - n;
-      a.kv_len = max(min(len, a.lim0 + (min(rows, a.row0 + kRows) - 1) / p.group + 1), 0);
+      const int kv_len = max(min(len, a.lim0 + (min(rows, a.row0 + kRows) - 1) / p.group + 1), 0);
+      a.steps = max(ceil_div(kv_len, BN), 1);
+      // steps whose first token is at s0 or after it, and before s1
+      const int step = (int)max((s0 - a.first_token + BN - 1) / BN, 0ll);
+      const int step_end = (int)min((long long)a.steps, max((s1 - a.first_token + BN - 1) / BN, 0ll));
+      s0 = item_end;
+      if (step >= step_end) continue;
       a.t0 = step * BN;
-      a.t1 = min(a.kv_len, step_end * BN);
+      a.t1 = min(kv_len, step_end * BN);
       a.count = a.t0 < a.t1 ? (a.t1 - a.t0 + BN - 1) / BN : 0;
-      a.steps = steps;
-      a.first_step = first_step;
       a.opens = step == 0;
-      a.whole = step == 0 && step_end == steps;
+      a.whole = step == 0 && step_end == a.steps;
       return true;
     }
     return false;
@@ -1123,6 +1139,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     constexpr uint32_t kIdescO = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);  // B is N major
     uint32_t i = 0, seg = 0;
     const uint32_t leader = lane == 0;
+    uint32_t phase0 = 0, phase1 = 0;  // parity of the next p_full of each tile
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     const uint32_t q_lo = desc_lo(sbase, 16), k_lo = desc_lo(sbase + L::kKOff, 16), v_lo = desc_lo(sbase + L::kVOff, BN * 128);
     constexpr uint32_t kHi = desc_hi(1024);
@@ -1142,32 +1159,40 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     auto commit = [&](uint64_t* bar) { commit_by(leader, bar); };
     while (__shfl_sync(0xffffffffu, (int)next_segment(a), 0)) {
       const int count = __shfl_sync(0xffffffffu, a.count, 0);
+      const bool two = QT == 2 && __shfl_sync(0xffffffffu, a.rows - a.row0, 0) > 128;  // the second tile has rows
       if (count == 0) continue;
       wait(q_full, seg & 1);
       ++seg;
       tc_fence_after_sync();
       wait(wide_full + 0, i & 1);
       tc_fence_after_sync();
+      auto products = [&](auto tiles) {
+        constexpr int kTiles = decltype(tiles)::value;
 #pragma unroll
-      for (int t = 0; t < QT; ++t) scores(t);
-      commit(wide_empty + 0);
-      for (int step = 0; step < count; ++step, ++i) {
-        const bool more = step + 1 < count;
-        wait(wide_full + 1 + (i & 1), (i >> 1) & 1);
+        for (int t = 0; t < kTiles; ++t) scores(t);
+        commit(wide_empty + 0);
+        for (int step = 0; step < count; ++step, ++i) {
+          const bool more = step + 1 < count;
+          wait(wide_full + 1 + (i & 1), (i >> 1) & 1);
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-          wait(p_full + t, i & 1);
-          tc_fence_after_sync();
-          output(t, step == 0, i & 1);
-          if (t == QT - 1) commit(wide_empty + 1 + (i & 1));
-          if (more) {
-            if (t == 0) wait(wide_full + 0, (i + 1) & 1);
+          for (int t = 0; t < kTiles; ++t) {
+            wait(p_full + t, t ? phase1 : phase0);
             tc_fence_after_sync();
-            scores(t);
-            if (t == QT - 1) commit(wide_empty + 0);
+            output(t, step == 0, i & 1);
+            if (t == kTiles - 1) commit(wide_empty + 1 + (i & 1));
+            if (more) {
+              if (t == 0) wait(wide_full + 0, (i + 1) & 1);
+              tc_fence_after_sync();
+              scores(t);
+              if (t == kTiles - 1) commit(wide_empty + 0);
+            }
           }
+          phase0 ^= 1;
+          if (kTiles == 2) phase1 ^= 1;
         }
-      }
+      };
+      if (two) products(std::integral_constant<int, QT>{});
+      else products(std::integral_constant<int, 1>{});
       commit(o_full);
     }
   }
@@ -1222,56 +1247,58 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int local = t * 128 + (threadIdx.x & 127);  // row of the item
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;  // TMEM lane (warp % 4) * 32 in the address
     const uint32_t s_at = tmem + quarter + t * BN, o_at = tmem + quarter + kOCol + t * HD;
-    uint32_t i = 0, seg = 0;
+    uint32_t i = 0, seg = 0, s_phase = 0;
     while (next_segment(a)) {
       const int row = a.row0 + local;
       const bool live = row < a.rows;
       float m = kNoMax, l = 0.f, qe = 1.f;
       int lim = a.t1 - 1;
       if (a.count > 0) {
-        // the Q row: power-of-two scale, fp16
-        const long long q_at = (long long)(a.start + (live ? row : 0) / p.group) * p.q_token_stride +
-                               (long long)(a.h * p.group + (live ? row : 0) % p.group) * p.q_head_stride;
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + q_at);
-        constexpr int kBatch = HD == 256 ? 16 : HD / 8;  // 16-byte vectors in registers (half of a row of 256)
-        float most = 0.f;
-        uint4 w[kBatch];
-#pragma unroll
-        for (int half = 0; half < HD / 8 / kBatch; ++half) {
-#pragma unroll
-          for (int c = 0; c < kBatch; ++c) w[c] = live ? __ldg(src + half * kBatch + c) : make_uint4(0, 0, 0, 0);
+        // The warp's 32 Q rows, kLanes lanes to a row: power-of-two scale, fp16.
+        constexpr int kLanes = HD / 8, kAtOnce = 32 / kLanes, kBatch = 16;  // 16-byte vectors per lane at a time
+        const int sub = lane / kLanes, vec = lane % kLanes;
+        const float sign = copysignf(1.f, p.scale);
+#pragma unroll 1
+        for (int r0 = 0; r0 < 32; r0 += kAtOnce * kBatch) {
+          uint4 w[kBatch];
 #pragma unroll
           for (int c = 0; c < kBatch; ++c) {
+            const int at = r0 + c * kAtOnce + sub, rr = a.row0 + t * 128 + (warp & 3) * 32 + at;
+            w[c] = make_uint4(0, 0, 0, 0);
+            if (c * kAtOnce < 32 && rr < a.rows)
+              w[c] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) +
+                                                          (long long)(a.start + rr / p.group) * p.q_token_stride +
+                                                          (long long)(a.h * p.group + rr % p.group) * p.q_head_stride) + vec);
+          }
+#pragma unroll
+          for (int c = 0; c < kBatch; ++c) {
+            if (c * kAtOnce >= 32) break;
             const uint32_t ww[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+            float x[8], most = 0.f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float2 f = unpack_q(p.bf16, ww[e]);
+              x[2 * e] = f.x;
+              x[2 * e + 1] = f.y;
               most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
             }
-          }
-        }
-        int ex = (int)(__float_as_uint(most) >> 23) - 126;  // most < 2^ex
-        ex = isfinite(most) ? min(max(ex, -100), 100) : 0;
-        const float down = copysignf(__uint_as_float((uint32_t)(127 - ex) << 23), p.scale);
-        qe = __uint_as_float((uint32_t)(127 + ex) << 23);
-        const uint32_t dst = sbase + t * L::kQ + (threadIdx.x & 127) * 128;
 #pragma unroll
-        for (int half = 0; half < HD / 8 / kBatch; ++half) {
-          if (HD == 256) {
+            for (int d = 1; d < kLanes; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+            int ex = (int)(__float_as_uint(most) >> 23) - 126;  // most < 2^ex
+            ex = isfinite(most) ? min(max(ex, -100), 100) : 0;
+            const float down = sign * __uint_as_float((uint32_t)(127 - ex) << 23);
+            const int at = r0 + c * kAtOnce + sub;
+            // the row's own thread keeps its scale
 #pragma unroll
-            for (int c = 0; c < kBatch; ++c) w[c] = live ? __ldg(src + half * kBatch + c) : make_uint4(0, 0, 0, 0);
-          }
-#pragma unroll
-          for (int c = 0; c < kBatch; ++c) {
-            const uint32_t ww[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+            for (int s = 0; s < kAtOnce; ++s) {
+              const int theirs = __shfl_sync(0xffffffffu, ex, s * kLanes);
+              if (lane == r0 + c * kAtOnce + s) qe = __uint_as_float((uint32_t)(127 + theirs) << 23);
+            }
             uint32_t o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 f = unpack_q(p.bf16, ww[e]);
-              o[e] = h2_as_u32(__floats2half2_rn(f.x * down, f.y * down));
-            }
-            const int v = half * kBatch + c;
-            sts128(dst + (v / 8) * (128 * 128) + (((v % 8) ^ (threadIdx.x & 7)) << 4), o[0], o[1], o[2], o[3]);
+            for (int e = 0; e < 4; ++e) o[e] = h2_as_u32(__floats2half2_rn(x[2 * e] * down, x[2 * e + 1] * down));
+            sts128(sbase + t * L::kQ + (vec / 8) * (128 * 128) + ((warp & 3) * 32 + at) * 128 + (((vec % 8) ^ (at & 7)) << 4), o[0],
+                   o[1], o[2], o[3]);
           }
         }
         fence_proxy_async_smem();
@@ -1279,10 +1306,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (lane == 0) mbar_arrive(q_full);
         if (live) lim = min(a.lim0 + row / p.group, a.t1 - 1);
       }
+      const bool idle = a.row0 + t * 128 >= a.rows;  // no row of this tile: only the barriers that count both
       for (int step = 0; step < a.count; ++step, ++i) {
         const int j0 = a.t0 + step * BN, stage = i & 1;
         wait(const_full + stage, (i >> 1) & 1);
-        wait(s_full + t, i & 1);
+        if (idle) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(const_empty + stage);
+          continue;
+        }
+        wait(s_full + t, s_phase);
+        s_phase ^= 1;
         tc_fence_after_sync();
         const float4* cs = consts + stage * (BN / 16);
         const int seen = lim - j0;  // columns up to here count
@@ -1394,7 +1428,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t o[32];
-        if (a.count > 0) {
+        if (a.count > 0 && !idle) {
           tmem_ld32(o_at + c * 32, o);
           tmem_wait_ld();
         } else {
@@ -1422,7 +1456,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tc_fence_before_sync();  // the next segment's products overwrite the output
       if (!a.whole) {
         if (live) *reinterpret_cast<float2*>(part + kRows * HD + 2 * local) = make_float2(m, l);
-        const int c0 = (int)(((a.first_step + 1) * C - 1) / all), c1 = (int)(((a.first_step + a.steps) * C - 1) / all);
+        const int c0 = (int)(((a.first_token + 1) * C - 1) / all);
+        const int c1 = (int)(((a.first_token + (long long)(a.steps - 1) * BN + 1) * C - 1) / all);
         __threadfence();
         named_barrier_sync(1, 128 * QT);
         if (threadIdx.x == 0) *last_one = atomicAdd(counters + c0, 1) == c1 - c0;
@@ -1554,8 +1589,11 @@ int launch_stream(const AttendArgs& a, const DeviceInfo& dev, void* workspace, s
   return e == cudaSuccess ? GDSQ_OK : cuda_fail(e, "attend launch");
 }
 
-// Rows per (request, KV head) up to which the stream kernel is taken.
-constexpr int kStreamRows = 16;
+// Rows per (request, KV head) up to which the stream kernel is taken.  // A tile's 128 rows are a whole product however few are filled: 32 requests of
+// 2000 tokens with 20 rows take 69 us there and 113 us here, 512 rows over 30000
+// tokens 98 us here.
+template <int HD>
+constexpr int stream_rows() { return 32; }
 
 template <int HD, int F>
 int launch_tile(const AttendArgs& a, const DeviceInfo& dev, void* workspace, size_t bytes, cudaStream_t stream) {
@@ -1583,7 +1621,9 @@ int launch_attend(const AttendArgs& a, int max_query_len, const DeviceInfo& dev,
                   cudaStream_t stream) {
   const long long rows = (long long)max_query_len * a.group;
   if (rows <= 8) return launch_stream<HD, F, 1>(a, dev, workspace, bytes, stream);
-  if (rows <= kStreamRows) return launch_stream<HD, F, 2>(a, dev, workspace, bytes, stream);
+  if (rows <= 16 || (HD == 256 && rows <= stream_rows<HD>())) return launch_stream<HD, F, 2>(a, dev, workspace, bytes, stream);
+  if constexpr (HD != 256)
+    if (rows <= stream_rows<HD>()) return launch_stream<HD, F, 4>(a, dev, workspace, bytes, stream);
   return launch_tile<HD, F>(a, dev, workspace, bytes, stream);
 }
 
@@ -1608,11 +1648,16 @@ extern "C" size_t gdsq_attend_kv8_workspace(int num_requests, int max_query_len,
   const DeviceInfo* dev = nullptr;
   if (device_info(&dev) != GDSQ_OK) return 0;
   const long long rows = (long long)max_query_len * (num_heads / num_kv_heads);
-  auto of = [&](size_t one, size_t two, size_t tile) { return rows <= 8 ? one : rows <= kStreamRows ? two : tile; };
-  if (head_dim == 64) return of(stream_workspace<64, 1>(dev->sms), stream_workspace<64, 2>(dev->sms), tile_workspace<64>(dev->sms));
+  // the largest of the variants that up to this many rows can take
+  const int n = dev->sms;
+  auto most = [&](size_t one, size_t two, size_t four, size_t tile) {
+    return std::max(std::max(one, rows > 8 ? two : 0), std::max(rows > 16 ? four : 0, rows > 32 ? tile : 0));
+  };
+  if (head_dim == 64)
+    return most(stream_workspace<64, 1>(n), stream_workspace<64, 2>(n), stream_workspace<64, 4>(n), tile_workspace<64>(n));
   if (head_dim == 128)
-    return of(stream_workspace<128, 1>(dev->sms), stream_workspace<128, 2>(dev->sms), tile_workspace<128>(dev->sms));
-  return of(stream_workspace<256, 1>(dev->sms), stream_workspace<256, 2>(dev->sms), tile_workspace<256>(dev->sms));
+    return most(stream_workspace<128, 1>(n), stream_workspace<128, 2>(n), stream_workspace<128, 4>(n), tile_workspace<128>(n));
+  return most(stream_workspace<256, 1>(n), stream_workspace<256, 2>(n), 0, tile_workspace<256>(n));
 }
 
 extern "C" int gdsq_attend_kv8(const void* q, int elem_type, long long q_token_stride, long long q_head_stride,
