@@ -216,7 +216,7 @@ __device__ __forceinline__ float3 page_constants(const AttendArgs& p, int page, 
 
 constexpr int kStepTokens = kAttWarps * 32;
 constexpr int kRing = 2;      // stages per warp
-constexpr int kItemCost = 2;  // what beginning and ending an item costs, in steps
+constexpr int kItemCost = 3;  // what beginning and ending an item costs, in steps
 
 template <int HD, int NT>
 struct StreamLayout {

@@ -53,10 +53,11 @@ __global__ void __launch_bounds__(kTabThreads) build_tables_kernel(const TablesA
   int* first = starts + p.requests + 1;  // [requests] index into free_blocks
   __shared__ int wsum[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int threads = blockDim.x, warps = threads >> 5;
   pdl_launch_dependents();
   pdl_wait_primary();
   const int head = *p.free_head;
-  const int per = (p.requests + kTabThreads - 1) / kTabThreads;
+  const int per = (p.requests + threads - 1) / threads;
   const int r0 = min(tid * per, p.requests), r1 = min(r0 + per, p.requests);
   int tok = 0, blk = 0;
   bool bad = head < 0;
@@ -82,15 +83,10 @@ __global__ void __launch_bounds__(kTabThreads) build_tables_kernel(const TablesA
     wsum[1][warp] = bsum;
   }
   __syncthreads();
-  int tb = ts - tok, bb = bsum - blk, tall = 0, ball = 0;
-  for (int w = 0; w < kTabThreads / 32; ++w) {
-    if (w < warp) {
-      tb += wsum[0][w];
-      bb += wsum[1][w];
-    }
-    tall += wsum[0][w];
-    ball += wsum[1][w];
-  }
+  const int wt = lane < warps ? wsum[0][lane] : 0, wb = lane < warps ? wsum[1][lane] : 0;
+  const int tb = ts - tok + __reduce_add_sync(0xffffffffu, lane < warp ? wt : 0);
+  const int bb = bsum - blk + __reduce_add_sync(0xffffffffu, lane < warp ? wb : 0);
+  const int tall = __reduce_add_sync(0xffffffffu, wt), ball = __reduce_add_sync(0xffffffffu, wb);
   for (int r = r0; r < r1; ++r) {
     starts[r] += tb;
     first[r] += head + bb;
@@ -99,8 +95,7 @@ __global__ void __launch_bounds__(kTabThreads) build_tables_kernel(const TablesA
   __syncthreads();
 
   auto free_block = [&](int i) { return i >= 0 && i < p.num_free ? p.free_blocks[i] : -1; };
-  const int gw = blockIdx.x * (kTabThreads / 32) + warp;
-  for (int r = gw; r < p.requests; r += gridDim.x * (kTabThreads / 32)) {
+  for (int r = blockIdx.x * warps + warp; r < p.requests; r += gridDim.x * warps) {
     const int c = max(p.context[r], 0), n = starts[r + 1] - starts[r];
     const int held = (c + p.block - 1) / p.block, after = (c + n + p.block - 1) / p.block;
     for (int j = held + lane; j < min(after, p.width); j += 32) {
@@ -119,8 +114,8 @@ __global__ void __launch_bounds__(kTabThreads) build_tables_kernel(const TablesA
     }
   }
   bad |= tall > p.tokens;
-  const long long stride = (long long)gridDim.x * kTabThreads;
-  for (long long i = (long long)blockIdx.x * kTabThreads + tid; i < p.tokens; i += stride) {
+  const long long stride = (long long)gridDim.x * threads;
+  for (long long i = (long long)blockIdx.x * threads + tid; i < p.tokens; i += stride) {
     long long pos = 0, slot = -1;
     if (i < tall) {
       int lo = 0, hi = p.requests;  // the request with starts[lo] <= i < starts[lo + 1]
@@ -510,8 +505,10 @@ int gdsq_build_tables(const int32_t* context_lens, const int32_t* new_lens, int 
   const int smem = (2 * num_requests + 1) * (int)sizeof(int);
   cudaError_t e = ensure_smem(build_tables_kernel, smem, dev->ordinal);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(build_tables)");
-  const int grid = std::max(1, std::min(dev->sms, (num_tokens + kTabThreads - 1) / kTabThreads));
-  e = launch(build_tables_kernel, dim3(grid), dim3(kTabThreads), smem, static_cast<cudaStream_t>(stream_v),
+  // A step of few requests is bound by the barriers of a CTA, so it gets a small one.
+  const int threads = num_requests <= 256 && num_tokens <= 256 ? 256 : kTabThreads;
+  const int grid = std::max(1, std::min(dev->sms, (num_tokens + threads - 1) / threads));
+  e = launch(build_tables_kernel, dim3(grid), dim3(threads), smem, static_cast<cudaStream_t>(stream_v),
              g_pdl_enabled != 0, a);
   return e == cudaSuccess ? GDSQ_OK : cuda_fail(e, "build_tables launch");
 }

@@ -54,6 +54,15 @@ Tensor make(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
   return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
 }
 
+// A contiguous tensor `at` bytes into buffer's storage: several outputs of one call share one allocation.
+Tensor part(const Tensor& buffer, int64_t at, at::IntArrayRef sizes, at::ScalarType type) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(),
+                                                     c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(at / static_cast<int64_t>(c10::elementSize(type)));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
+}
+
 void on_gpu(const Tensor& t) { NEED(t.is_cuda(), "the tensors must be on a CUDA device, not ", t.device()); }
 
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
@@ -107,9 +116,15 @@ Tables build_tables(const Tensor& context, const Tensor& fresh, const Tensor& ta
   const int tokens = small(num_tokens, "num_tokens");
   on_gpu(context);
   const c10::cuda::CUDAGuard guard(context.device());
-  Tables o = out ? *out
-                 : Tables(make({r}, at::kInt, context), make({r + 1}, at::kInt, context), make({num_tokens}, at::kLong, context),
-                          make({num_tokens}, at::kLong, context), make({1}, at::kInt, context));
+  Tables o;
+  if (out) {
+    o = *out;
+  } else {
+    const Tensor b = make({16 * num_tokens + 8 * (r + 1)}, at::kByte, context);
+    const int64_t ints = 16 * num_tokens;
+    o = Tables(part(b, ints, {r}, at::kInt), part(b, ints + 4 * r, {r + 1}, at::kInt), part(b, 0, {num_tokens}, at::kLong),
+               part(b, 8 * num_tokens, {num_tokens}, at::kLong), part(b, ints + 8 * r + 4, {1}, at::kInt));
+  }
   check(gdsq_build_tables(static_cast<const int32_t*>(c), static_cast<const int32_t*>(n), small(r, "requests"),
                           static_cast<int32_t*>(t), small(table.size(1), "table width"), static_cast<const int32_t*>(f),
                           small(free_blocks.numel(), "free blocks"), static_cast<const int32_t*>(h),
@@ -228,8 +243,11 @@ std::tuple<Tensor, Tensor> sample(const Tensor& logits, const Tensor& uniforms, 
   param(logprobs, "logprobs", at::kFloat);
   on_gpu(logits);
   const c10::cuda::CUDAGuard guard(logits.device());
-  if (!tokens) tokens = make({b}, at::kLong, logits);
-  if (!logprobs) logprobs = make({b}, at::kFloat, logits);
+  if (!tokens || !logprobs) {
+    const Tensor both = make({12 * b}, at::kByte, logits);
+    if (!tokens) tokens = part(both, 0, {b}, at::kLong);
+    if (!logprobs) logprobs = part(both, 8 * b, {b}, at::kFloat);
+  }
   check(gdsq_sample(elem_type(logits), logits.const_data_ptr(), logits.stride(0), small(b, "rows"),
                     small(logits.size(1), "vocab"), static_cast<const float*>(u), static_cast<const float*>(t),
                     static_cast<const int32_t*>(k), static_cast<const float*>(p), static_cast<const float*>(m),
