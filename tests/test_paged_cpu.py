@@ -89,26 +89,26 @@ def test_python_refuses():
     slots = torch.zeros(3, dtype=torch.int64)
     i32 = lambda *n: torch.zeros(*n, dtype=torch.int32)  # noqa: E731
     bad = [
-        lambda: paged.append_kv8(x.float(), x, slots, kc, vc, ks, vs),
-        lambda: paged.append_kv8(x, x.bfloat16(), slots, kc, vc, ks, vs),
-        lambda: paged.append_kv8(x[:, :1], x, slots, kc, vc, ks, vs),
-        lambda: paged.append_kv8(x, x[:2], slots, kc, vc, ks, vs),
-        lambda: paged.append_kv8(x, x, slots.int(), kc, vc, ks, vs),
-        lambda: paged.append_kv8(x, x, slots, kc.half(), vc, ks, vs),
-        lambda: paged.append_kv8(x, x, slots, kc, vc[:2], ks, vs),
-        lambda: paged.append_kv8(x, x, slots, kc, vc, ks.half(), vs),
-        lambda: paged.append_kv8(x, x, slots, kc, vc, ks, vs, q=x),
-        lambda: paged.append_kv8(x, x, slots, kc, vc, ks, vs, freqs=torch.zeros(8, 32, 2)),
-        lambda: paged.append_kv8(x, x, slots, kc, vc, ks, vs, freqs=torch.zeros(8, 64, 2), positions=slots),
-        lambda: paged.append_kv8(x.transpose(1, 2), x, slots, kc, vc, ks, vs),
-        lambda: paged.attend_kv8(x.float(), kc, vc, ks, vs, i32(1, 4), i32(1), i32(2), 3),
-        lambda: paged.attend_kv8(x, kc, vc, ks, vs, i32(2, 4), i32(1), i32(2), 3),
-        lambda: paged.attend_kv8(x, kc, vc, ks, vs, i32(1, 4), i32(1), i32(2), 3, out=x.bfloat16()),
-        lambda: paged.build_tables(i32(2), i32(2), i32(3, 4), i32(9), i32(1), 16, 4),
-        lambda: sampling.sample(torch.zeros(5), torch.zeros(1)),
-        lambda: sampling.sample(torch.zeros(2, 5, dtype=torch.float64), torch.zeros(2)),
-        lambda: sampling.sample(torch.zeros(5, 2).t(), torch.zeros(2)),
+        ("k: fp16 or bf16", lambda: paged.append_kv8(x.float(), x, slots, kc, vc, ks, vs)),
+        ("v: fp16 or bf16", lambda: paged.append_kv8(x, x.bfloat16(), slots, kc, vc, ks, vs)),
+        ("k: expected", lambda: paged.append_kv8(x[:, :1], x, slots, kc, vc, ks, vs)),
+        ("k has 3 tokens, v 2", lambda: paged.append_kv8(x, x[:2], slots, kc, vc, ks, vs)),
+        ("slots: expected", lambda: paged.append_kv8(x, x, slots.int(), kc, vc, ks, vs)),
+        ("the cache is int8 or", lambda: paged.append_kv8(x, x, slots, kc.half(), vc, ks, vs)),
+        ("k_cache and v_cache", lambda: paged.append_kv8(x, x, slots, kc, vc[:2], ks, vs)),
+        ("the scales are", lambda: paged.append_kv8(x, x, slots, kc, vc, ks.half(), vs)),
+        ("q is only rotated", lambda: paged.append_kv8(x, x, slots, kc, vc, ks, vs, q=x)),
+        ("freqs needs positions", lambda: paged.append_kv8(x, x, slots, kc, vc, ks, vs, freqs=torch.zeros(8, 32, 2))),
+        ("freqs: contiguous", lambda: paged.append_kv8(x, x, slots, kc, vc, ks, vs, freqs=torch.zeros(8, 64, 2), positions=slots)),
+        ("k: expected", lambda: paged.append_kv8(x.transpose(1, 2), x, slots, kc, vc, ks, vs)),
+        ("q: fp16 or bf16", lambda: paged.attend_kv8(x.float(), kc, vc, ks, vs, i32(1, 4), i32(1), i32(2), 3)),
+        ("block_table", lambda: paged.attend_kv8(x, kc, vc, ks, vs, i32(2, 4), i32(1), i32(2), 3)),
+        ("out: contiguous", lambda: paged.attend_kv8(x, kc, vc, ks, vs, i32(1, 4), i32(1), i32(2), 3, out=x.bfloat16())),
+        ("block_table", lambda: paged.build_tables(i32(2), i32(2), i32(3, 4), i32(9), i32(1), 16, 4)),
+        ("logits:", lambda: sampling.sample(torch.zeros(5), torch.zeros(1))),
+        ("logits:", lambda: sampling.sample(torch.zeros(2, 5, dtype=torch.float64), torch.zeros(2))),
+        ("logits:", lambda: sampling.sample(torch.zeros(5, 2).t(), torch.zeros(2))),
     ]
-    for call in bad:
-        with pytest.raises(ValueError):
+    for text, call in bad:
+        with pytest.raises(ValueError, match=text):
             call()
