@@ -30,10 +30,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <functional>
-#include <mutex>
 #include <type_traits>
-#include <unordered_map>
 
 #include "gdsq.h"
 #include "host.h"
@@ -86,6 +83,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// 16 bytes of global memory to shared memory, or zeros.
+__device__ __forceinline__ void copy16_async(uint32_t to, const void* from, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // 8-bit codes to fp16 pairs, exactly.
 template <int F>
@@ -161,17 +164,16 @@ __device__ __forceinline__ void store_out(const AttendArgs& p, int start, int h,
 }
 
 // Eight dims of one output row.
-__device__ __forceinline__ void store_out8(const AttendArgs& p, int start, int h, int row, int d, const float (&num)[8], float inv) {
-  const long long at = (long long)(start + row / p.group) * p.out_token_stride +
-                       (long long)(h * p.group + row % p.group) * p.out_head_stride + d;
+// 8 values of an output row, from `to`.
+__device__ __forceinline__ void store_out8(void* to, bool bf16, const float (&num)[8], float inv) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float x = num[2 * i] * inv, y = num[2 * i + 1] * inv;
     const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
-    w[i] = p.bf16 ? *reinterpret_cast<const uint32_t*>(&b) : h2_as_u32(__floats2half2_rn(x, y));
+    w[i] = bf16 ? *reinterpret_cast<const uint32_t*>(&b) : h2_as_u32(__floats2half2_rn(x, y));
   }
-  *reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+  *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // Per-page constants of the softmax: x = kscale factor, y = lv, z = 2^-lv.
@@ -853,7 +855,8 @@ struct TileLayout {
 constexpr int kTileThreads = 16 * 32;
 // What beginning and ending an item costs, in tokens: the three prompts above
 // take 597 us with 11 steps of 128, 728 with 2, 631 with 6 and 611 with 15.
-constexpr int kItemTokens = 1408;
+template <int HD>
+__host__ __device__ constexpr int item_tokens() { return HD == 256 ? 448 : 1024; }
 // Registers per thread of the softmax, widening and other warp groups: together the launch's 4 x 128.
 constexpr int kSoftmaxRegs = 176, kWidenRegs = 80, kOtherRegs = 80;
 
@@ -1001,7 +1004,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   auto rows_of = [&](int r) { return max(min(p.starts[r + 1], p.tokens) - max(p.starts[r], 0), 0) * p.group; };
   auto first_of = [&](int r) {  // cost of the first row tile
     const int n = max(min(p.starts[r + 1], p.tokens) - max(p.starts[r], 0), 0);
-    return (long long)kItemTokens + max(min(p.seq_lens[r], most_len) - n, 0) + rise + 1;
+    return (long long)item_tokens<HD>() + max(min(p.seq_lens[r], most_len) - n, 0) + rise + 1;
   };
   auto upto_tile = [&](long long first, long long j) { return j * first + j * (j - 1) / 2 * rise; };
   auto cost_of = [&](int r) { return upto_tile(first_of(r), ceil_div(rows_of(r), kRows)) * p.kv_heads; };
@@ -1077,7 +1080,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       const long long item_at = request_at + h * head_cost + upto_tile(first, tile);
       const long long item_end = item_at + first + (long long)tile * rise;
-      a.first_token = item_at + kItemTokens;
+      a.first_token = item_at + item_tokens<HD>();
       a.r = r;
       a.h = h;
       a.row0 = tile * kRows;
@@ -1159,17 +1162,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     const uint32_t q_lo = desc_lo(sbase, 16), k_lo = desc_lo(sbase + L::kKOff, 16), v_lo = desc_lo(sbase + L::kVOff, BN * 128);
     constexpr uint32_t kHi = desc_hi(1024);
-    auto scores = [&](int t) {
+    auto scores = [&](int t, int tile) {
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k)
-        mma_ss(leader, tm + t * BN, q_lo + ((t * L::kQ + (k / 4) * (128 * 128) + (k % 4) * 32) >> 4),
+        mma_ss(leader, tm + t * BN, q_lo + ((tile * L::kQ + (k / 4) * (128 * 128) + (k % 4) * 32) >> 4),
                k_lo + (((k / 4) * (BN * 128) + (k % 4) * 32) >> 4), kHi, kHi, kIdescS, k > 0);
       commit_by(leader, s_full + t);
     };
-    auto output = [&](int t, bool first, uint32_t buffer) {
+    auto output = [&](int t, int tile, bool first, uint32_t buffer) {
 #pragma unroll
       for (int k = 0; k < BN / 16; ++k)
-        mma_ts(leader, tm + kOCol + t * HD, tm + t * BN + k * 8, v_lo + buffer * (L::kWide >> 4) + k * (2048 >> 4), kHi, kIdescO,
+        mma_ts(leader, tm + kOCol + tile * HD, tm + t * BN + k * 8, v_lo + buffer * (L::kWide >> 4) + k * (2048 >> 4), kHi, kIdescO,
                !(first && k == 0));
     };
     auto commit = [&](uint64_t* bar) { commit_by(leader, bar); };
@@ -1185,7 +1188,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       auto products = [&](auto tiles) {
         constexpr int kTiles = decltype(tiles)::value;
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) scores(t);
+        for (int t = 0; t < kTiles; ++t) scores(t, t);
         commit(wide_empty + 0);
         for (int step = 0; step < count; ++step, ++i) {
           const bool more = step + 1 < count;
@@ -1194,12 +1197,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           for (int t = 0; t < kTiles; ++t) {
             wait(p_full + t, t ? phase1 : phase0);
             tc_fence_after_sync();
-            output(t, step == 0, i & 1);
+            output(t, t, step == 0, i & 1);
             if (t == kTiles - 1) commit(wide_empty + 1 + (i & 1));
             if (more) {
               if (t == 0) wait(wide_full + 0, (i + 1) & 1);
               tc_fence_after_sync();
-              scores(t);
+              scores(t, t);
               if (t == kTiles - 1) commit(wide_empty + 0);
             }
           }
@@ -1207,7 +1210,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (kTiles == 2) phase1 ^= 1;
         }
       };
-      if (two) products(std::integral_constant<int, QT>{});
+      if constexpr (QT == 1) {
+        // one tile: the next scores go to another place, ahead of this step's weights
+        scores(i & 1, 0);
+        commit(wide_empty + 0);
+        for (int step = 0; step < count; ++step, ++i) {
+          if (step + 1 < count) {
+            wait(wide_full + 0, (i + 1) & 1);
+            tc_fence_after_sync();
+            scores((i + 1) & 1, 0);
+            commit(wide_empty + 0);
+          }
+          wait(wide_full + 1 + (i & 1), (i >> 1) & 1);
+          wait(p_full + (i & 1), (i >> 1) & 1);
+          tc_fence_after_sync();
+          output(i & 1, 0, step == 0, i & 1);
+          commit(wide_empty + 1 + (i & 1));
+        }
+      } else if (two) products(std::integral_constant<int, QT>{});
       else products(std::integral_constant<int, 1>{});
       commit(o_full);
     }
@@ -1258,253 +1278,307 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-    if (warp < 4 * QT) {
-    const int t = warp >> 2;                       // tile
+    const int t = QT == 1 ? 0 : warp >> 2;         // tile
+    const bool helps = QT == 1 && warp >= 4;       // with the joining of partial sums only
     const int local = t * 128 + (threadIdx.x & 127);  // row of the item
     const uint32_t quarter = (uint32_t)(warp & 3) << 21;  // TMEM lane (warp % 4) * 32 in the address
-    const uint32_t s_at = tmem + quarter + t * BN, o_at = tmem + quarter + kOCol + t * HD;
-    uint32_t i = 0, seg = 0, s_phase = 0;
+    const uint32_t s_at0 = tmem + quarter + t * BN, o_at = tmem + quarter + kOCol + t * HD;
+    uint32_t i = 0, seg = 0;
+    [[maybe_unused]] uint32_t s_phase = 0;
     while (next_segment(a)) {
       const int row = a.row0 + local;
       const bool live = row < a.rows;
-      float m = kNoMax, l = 0.f, qe = 1.f;
-      int lim = a.t1 - 1;
-      if (a.count > 0) {
-        // The warp's 32 Q rows, kLanes lanes to a row: power-of-two scale, fp16.
-        constexpr int kLanes = HD / 8, kAtOnce = 32 / kLanes, kBatch = 16;  // 16-byte vectors per lane at a time
-        const int sub = lane / kLanes, vec = lane % kLanes;
-        const float sign = copysignf(1.f, p.scale);
-#pragma unroll 1
-        for (int r0 = 0; r0 < 32; r0 += kAtOnce * kBatch) {
-          uint4 w[kBatch];
-#pragma unroll
-          for (int c = 0; c < kBatch; ++c) {
-            const int at = r0 + c * kAtOnce + sub, rr = a.row0 + t * 128 + (warp & 3) * 32 + at;
-            w[c] = make_uint4(0, 0, 0, 0);
-            if (c * kAtOnce < 32 && rr < a.rows)
-              w[c] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) +
-                                                          (long long)(a.start + rr / p.group) * p.q_token_stride +
-                                                          (long long)(a.h * p.group + rr % p.group) * p.q_head_stride) + vec);
-          }
-#pragma unroll
-          for (int c = 0; c < kBatch; ++c) {
-            if (c * kAtOnce >= 32) break;
-            const uint32_t ww[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
-            float x[8], most = 0.f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 f = unpack_q(p.bf16, ww[e]);
-              x[2 * e] = f.x;
-              x[2 * e + 1] = f.y;
-              most = fmaxf(most, fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
-#pragma unroll
-            for (int d = 1; d < kLanes; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-            int ex = (int)(__float_as_uint(most) >> 23) - 126;  // most < 2^ex
-            ex = isfinite(most) ? min(max(ex, -100), 100) : 0;
-            const float down = sign * __uint_as_float((uint32_t)(127 - ex) << 23);
-            const int at = r0 + c * kAtOnce + sub;
-            // the row's own thread keeps its scale
-#pragma unroll
-            for (int s = 0; s < kAtOnce; ++s) {
-              const int theirs = __shfl_sync(0xffffffffu, ex, s * kLanes);
-              if (lane == r0 + c * kAtOnce + s) qe = __uint_as_float((uint32_t)(127 + theirs) << 23);
-            }
-            uint32_t o[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = h2_as_u32(__floats2half2_rn(x[2 * e] * down, x[2 * e + 1] * down));
-            sts128(sbase + t * L::kQ + (vec / 8) * (128 * 128) + ((warp & 3) * 32 + at) * 128 + (((vec % 8) ^ (at & 7)) << 4), o[0],
-                   o[1], o[2], o[3]);
-          }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
-        if (live) lim = min(a.lim0 + row / p.group, a.t1 - 1);
-      }
-      const bool idle = a.row0 + t * 128 >= a.rows;  // no row of this tile: only the barriers that count both
-      for (int step = 0; step < a.count; ++step, ++i) {
-        const int j0 = a.t0 + step * BN, stage = i & 1;
-        wait(const_full + stage, (i >> 1) & 1);
-        if (idle) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(const_empty + stage);
-          continue;
-        }
-        wait(s_full + t, s_phase);
-        s_phase ^= 1;
-        tc_fence_after_sync();
-        const float4* cs = consts + stage * (BN / 16);
-        const int seen = lim - j0;  // columns up to here count
-        const bool cut = __any_sync(0xffffffffu, seen < BN - 1);
-        // Weights against the reference point m, in one pass; `over`: one has passed 2^8, which is not stored.
-        uint32_t w[BN / 2];
-        float more = 0.f;
-        bool over = false;
-        auto weights = [&](auto masked) {
-          constexpr bool kCut = decltype(masked)::value;
-          __half2 high = __float2half2_rn(0.f);
-          more = 0.f;
-          uint32_t ahead[2][32];  // the next 32 scores are on their way while these are worked on
-          tmem_ld32(s_at, ahead[0]);
-#pragma unroll
-          for (int c = 0; c < BN / 32; ++c) {
-            tmem_wait_ld();
-            if (c + 1 < BN / 32) tmem_ld32(s_at + (c + 1) * 32, ahead[(c + 1) & 1]);
-            const uint32_t(&s)[32] = ahead[c & 1];
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              const float4 k = cs[2 * c + g];
-              const float mul = fabsf(k.x) * qe, add = k.y - m;
-              const float2 mul2 = make_float2(mul, mul), add2 = make_float2(add, add);
-              float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-              for (int e = 0; e < 16; e += 2) {
-                const float2 z = fma2(make_float2(__uint_as_float(s[16 * g + e]), __uint_as_float(s[16 * g + e + 1])), mul2, add2);
-                float2 x = make_float2(exp2_approx(z.x), exp2_approx(z.y));
-                if (kCut) {
-                  if (32 * c + 16 * g + e > seen) x.x = 0.f;
-                  if (32 * c + 16 * g + e + 1 > seen) x.y = 0.f;
-                }
-                sum = add2f(sum, x);
-                const __half2 h = __floats2half2_rn(x.x, x.y);
-                high = __hmax2(high, h);
-                w[16 * c + 8 * g + e / 2] = h2_as_u32(h);
-              }
-              more = fmaf(sum.x + sum.y, k.z, more);
-            }
-          }
-          over = __half2float(__hmax(__low2half(high), __high2half(high))) > 256.f;
-        };
-        auto both = [&](auto f) {
-          if (cut) f(std::true_type{});
-          else f(std::false_type{});
-        };
-        if (step > 0) both(weights);
-        // The reference point moves only then, and in a segment's first step.
-        if (step == 0 || __any_sync(0xffffffffu, over || m == kNoMax)) {
-          float top = -INFINITY;
-          both([&](auto masked) {
-            constexpr bool kCut = decltype(masked)::value;
-#pragma unroll 1
-            for (int c = 0; c < BN / 16; ++c) {
-              uint32_t s[16];
-              tmem_ld16(s_at + c * 16, s);
-              tmem_wait_ld();
-              const float4 k = cs[c];
-              float high = -INFINITY;
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (!kCut || 16 * c + e <= seen) high = fmaxf(high, __uint_as_float(s[e]));
-              if (high > -INFINITY) top = fmaxf(top, fmaf(high, fabsf(k.x) * qe, k.y));
-            }
-          });
-          float fade = 1.f;
-          if (top > -INFINITY && (top > m || m == kNoMax)) {
-            fade = m == kNoMax ? 0.f : exp2_approx(m - top);
-            m = top;
-            l *= fade;
-          }
-          if (step > 0) {
-#pragma unroll 1
-            for (int c = 0; c < HD / 16; ++c) {
-              uint32_t o[16];
-              tmem_ld16(o_at + c * 16, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
-              tmem_st16(o_at + c * 16, o);
-            }
-          }
-          both(weights);
-        }
-        l += more;
-#pragma unroll
-        for (int c = 0; c < BN / 32; ++c) {
-          uint32_t out[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) out[e] = w[16 * c + e];
-          tmem_st16(s_at + c * 16, out);
-        }
-        tmem_wait_st();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(const_empty + stage);
-          mbar_arrive(p_full + t);
-        }
-      }
-      if (a.count > 0) {
-        wait(o_full, seg & 1);
-        ++seg;
-        tc_fence_after_sync();
-      }
+      float m = kNoMax, l = 0.f;
       const int slot = (int)blockIdx.x * 2 + (a.opens ? 1 : 0);
       float* part = parts + (size_t)slot * kRows * (HD + 2);
-#pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t o[32];
-        if (a.count > 0 && !idle) {
-          tmem_ld32(o_at + c * 32, o);
-          tmem_wait_ld();
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0;
-        }
-        // partial sums: [4 dims][row], so that a warp writes 32 rows side by side
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (!live) continue;
-        if (a.whole) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            float num[8];
-#pragma unroll
-            for (int y = 0; y < 8; ++y) num[y] = __uint_as_float(o[e + y]);
-            store_out8(p, a.start, a.h, row, c * 32 + e, num, inv);
+      __half* const out_row = static_cast<__half*>(p.out) + (long long)(a.start + row / p.group) * p.out_token_stride +
+                    (long long)(a.h * p.group + row % p.group) * p.out_head_stride;  // 16 bits of either type
+      if (!helps) {
+        float qe = 1.f;
+        int lim = a.t1 - 1;
+        if (a.count > 0) {
+          // The warp's 32 Q rows, kLanes lanes to a row: power-of-two scale, fp16.  Copied as
+          // it is, then scaled in place in a short loop: with all rows side by side in
+          // registers the fetching of the instructions took most of 20000 cycles.
+          constexpr int kLanes = HD / 8, kAtOnce = 32 / kLanes;  // 16-byte vectors
+          constexpr int kBatch = 4;                              // of a lane at a time
+          const int sub = lane / kLanes, vec = lane % kLanes;
+          const float sign = copysignf(1.f, p.scale);
+          const long long from = live ? (long long)(a.start + row / p.group) * p.q_token_stride +
+                                            (long long)(a.h * p.group + row % p.group) * p.q_head_stride
+                                      : -1;
+          auto place_of = [&](int at) {
+            return sbase + t * L::kQ + (vec / 8) * (128 * 128) + ((warp & 3) * 32 + at) * 128 + (((vec % 8) ^ (at & 7)) << 4);
+          };
+#pragma unroll 4
+          for (int r0 = 0; r0 < 32; r0 += kAtOnce) {
+            const long long at = __shfl_sync(0xffffffffu, from, r0 + sub);
+            copy16_async(place_of(r0 + sub), static_cast<const uint16_t*>(p.q) + max(at, 0ll) + vec * 8, at >= 0);
           }
-        } else {
+          copy_async_wait();
+          auto scale_rows = [&](auto bf16) {
+            constexpr bool kBf16 = decltype(bf16)::value;
+#pragma unroll 1
+            for (int r0 = 0; r0 < 32; r0 += kAtOnce * kBatch) {
+              uint4 w[kBatch];
+              float most[kBatch];
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<uint4*>(part + ((size_t)((c * 32 + e) / 4) * kRows + local) * 4) =
-                make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+              for (int c = 0; c < kBatch; ++c) w[c] = lds128(place_of(r0 + c * kAtOnce + sub));
+#pragma unroll
+              for (int c = 0; c < kBatch; ++c) {
+                const uint32_t ww[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+                most[c] = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float2 f = unpack_q(kBf16, ww[e]);
+                  most[c] = fmaxf(most[c], fmaxf(fabsf(f.x), fabsf(f.y)));
+                }
+              }
+            // level by level, so that the rows' shuffles do not wait for one another
+#pragma unroll
+              for (int d = 1; d < kLanes; d <<= 1)
+#pragma unroll
+                for (int c = 0; c < kBatch; ++c) most[c] = fmaxf(most[c], __shfl_xor_sync(0xffffffffu, most[c], d));
+#pragma unroll
+              for (int c = 0; c < kBatch; ++c) {
+                int ex = (int)(__float_as_uint(most[c]) >> 23) - 126;  // most < 2^ex
+                ex = isfinite(most[c]) ? min(max(ex, -100), 100) : 0;
+                const float down = sign * __uint_as_float((uint32_t)(127 - ex) << 23);
+                const int at = r0 + c * kAtOnce + sub;
+                // the row's own thread keeps its scale
+#pragma unroll
+                for (int s = 0; s < kAtOnce; ++s) {
+                  const int theirs = __shfl_sync(0xffffffffu, ex, s * kLanes);
+                  if (lane == r0 + c * kAtOnce + s) qe = __uint_as_float((uint32_t)(127 + theirs) << 23);
+                }
+                const uint32_t ww[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
+                uint32_t o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float2 f = unpack_q(kBf16, ww[e]);
+                  o[e] = h2_as_u32(__floats2half2_rn(f.x * down, f.y * down));
+                }
+                sts128(place_of(at), o[0], o[1], o[2], o[3]);
+              }
+            }
+          };
+          if (p.bf16) scale_rows(std::true_type{});
+          else scale_rows(std::false_type{});
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(q_full);
+          if (live) lim = min(a.lim0 + row / p.group, a.t1 - 1);
         }
+        const bool idle = a.row0 + t * 128 >= a.rows;  // no row of this tile: only the barriers that count both
+        for (int step = 0; step < a.count; ++step, ++i) {
+          const int j0 = a.t0 + step * BN, stage = i & 1;
+          wait(const_full + stage, (i >> 1) & 1);
+          if (idle) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(const_empty + stage);
+            continue;
+          }
+          const uint32_t place = QT == 1 ? i & 1 : 0;  // of the scores and the weights
+          const uint32_t s_at = s_at0 + place * BN;
+          if constexpr (QT == 1) {
+            wait(s_full + place, (i >> 1) & 1);
+          } else {
+            wait(s_full + t, s_phase);
+            s_phase ^= 1;
+          }
+          tc_fence_after_sync();
+          const float4* cs = consts + stage * (BN / 16);
+          const int seen = lim - j0;  // columns up to here count
+          const bool cut = __any_sync(0xffffffffu, seen < BN - 1);
+          // Weights against the reference point m, in one pass; `over`: one has passed 2^8, which is not stored.
+          uint32_t w[BN / 2];
+          float more = 0.f;
+          bool over = false;
+          auto weights = [&](auto masked) {
+            constexpr bool kCut = decltype(masked)::value;
+            __half2 high = __float2half2_rn(0.f);
+            more = 0.f;
+            uint32_t ahead[2][32];  // the next 32 scores are on their way while these are worked on
+            tmem_ld32(s_at, ahead[0]);
+#pragma unroll
+            for (int c = 0; c < BN / 32; ++c) {
+              tmem_wait_ld();
+              if (c + 1 < BN / 32) tmem_ld32(s_at + (c + 1) * 32, ahead[(c + 1) & 1]);
+              const uint32_t(&s)[32] = ahead[c & 1];
+#pragma unroll
+              for (int g = 0; g < 2; ++g) {
+                const float4 k = cs[2 * c + g];
+                const float mul = fabsf(k.x) * qe, add = k.y - m;
+                const float2 mul2 = make_float2(mul, mul), add2 = make_float2(add, add);
+                float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                  const float2 z = fma2(make_float2(__uint_as_float(s[16 * g + e]), __uint_as_float(s[16 * g + e + 1])), mul2, add2);
+                  float2 x = make_float2(exp2_approx(z.x), exp2_approx(z.y));
+                  if (kCut) {
+                    if (32 * c + 16 * g + e > seen) x.x = 0.f;
+                    if (32 * c + 16 * g + e + 1 > seen) x.y = 0.f;
+                  }
+                  sum = add2f(sum, x);
+                  const __half2 h = __floats2half2_rn(x.x, x.y);
+                  high = __hmax2(high, h);
+                  w[16 * c + 8 * g + e / 2] = h2_as_u32(h);
+                }
+                more = fmaf(sum.x + sum.y, k.z, more);
+              }
+            }
+            over = __half2float(__hmax(__low2half(high), __high2half(high))) > 256.f;
+          };
+          auto both = [&](auto f) {
+            if (cut) f(std::true_type{});
+            else f(std::false_type{});
+          };
+          // The reference point moves in a segment's first step and when a weight has passed the limit.
+          bool move = step == 0;
+#pragma unroll 1
+          for (;;) {
+            if (move) {
+              float top = -INFINITY;
+              both([&](auto masked) {
+                constexpr bool kCut = decltype(masked)::value;
+#pragma unroll 1
+                for (int c = 0; c < BN / 16; ++c) {
+                  uint32_t s[16];
+                  tmem_ld16(s_at + c * 16, s);
+                  tmem_wait_ld();
+                  const float4 k = cs[c];
+                  float high = -INFINITY;
+#pragma unroll
+                  for (int e = 0; e < 16; ++e)
+                    if (!kCut || 16 * c + e <= seen) high = fmaxf(high, __uint_as_float(s[e]));
+                  if (high > -INFINITY) top = fmaxf(top, fmaf(high, fabsf(k.x) * qe, k.y));
+                }
+              });
+              float fade = 1.f;
+              if (top > -INFINITY && (top > m || m == kNoMax)) {
+                fade = m == kNoMax ? 0.f : exp2_approx(m - top);
+                m = top;
+                l *= fade;
+              }
+              if (step > 0) {
+                if (QT == 1) {  // the output of the step before may still be on its way
+                  wait(wide_empty + 1 + ((i - 1) & 1), ((i - 1) >> 1) & 1);
+                  tc_fence_after_sync();
+                }
+#pragma unroll 1
+                for (int c = 0; c < HD / 16; ++c) {
+                  uint32_t o[16];
+                  tmem_ld16(o_at + c * 16, o);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
+                  tmem_st16(o_at + c * 16, o);
+                }
+              }
+            }
+            both(weights);
+            if (move || !__any_sync(0xffffffffu, over || m == kNoMax)) break;
+            move = true;
+          }
+          l += more;
+#pragma unroll
+          for (int c = 0; c < BN / 32; ++c) {
+            uint32_t out[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) out[e] = w[16 * c + e];
+            tmem_st16(s_at + c * 16, out);
+          }
+          tmem_wait_st();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(const_empty + stage);
+            mbar_arrive(p_full + (QT == 1 ? place : t));
+          }
+        }
+        if (a.count > 0) {
+          wait(o_full, seg & 1);
+          ++seg;
+          tc_fence_after_sync();
+        }
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          if (a.count > 0 && !idle) {
+            tmem_ld32(o_at + c * 32, o);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0;
+          }
+          // partial sums: [4 dims][row], so that a warp writes 32 rows side by side
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          if (!live) continue;
+          if (a.whole) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              float num[8];
+#pragma unroll
+              for (int y = 0; y < 8; ++y) num[y] = __uint_as_float(o[e + y]);
+              store_out8(out_row + c * 32 + e, p.bf16, num, inv);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4*>(part + ((size_t)((c * 32 + e) / 4) * kRows + local) * 4) =
+                  make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+        tc_fence_before_sync();  // the next segment's products overwrite the output
       }
-      tc_fence_before_sync();  // the next segment's products overwrite the output
       if (!a.whole) {
-        if (live) *reinterpret_cast<float2*>(part + kRows * HD + 2 * local) = make_float2(m, l);
+        if (live && !helps) *reinterpret_cast<float2*>(part + kRows * HD + 2 * local) = make_float2(m, l);
         const int c0 = (int)(((a.first_token + 1) * C - 1) / all);
         const int c1 = (int)(((a.first_token + (long long)(a.steps - 1) * BN + 1) * C - 1) / all);
         __threadfence();
-        named_barrier_sync(1, 128 * QT);
+        named_barrier_sync(1, 256);
         if (threadIdx.x == 0) *last_one = atomicAdd(counters + c0, 1) == c1 - c0;
-        named_barrier_sync(1, 128 * QT);
+        named_barrier_sync(1, 256);
         if (*last_one) {
           __threadfence();
           if (live) {
             auto from = [&](int c) { return parts + ((size_t)(2 * c + (c == c0)) * kRows) * (HD + 2); };
             float top = kNoMax, den = 0.f;
+#pragma unroll 4
             for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(from(c) + kRows * HD + 2 * local));
+#pragma unroll 4
             for (int c = c0; c <= c1; ++c) {
               const float2 ml = __ldcg(reinterpret_cast<const float2*>(from(c) + kRows * HD + 2 * local));
               den = fmaf(ml.y, exp2_approx(ml.x - top), den);
             }
             const float inv = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll 1
-            for (int d = 0; d < HD; d += 32) {
+            for (int d = helps ? HD / 2 : 0; d < (QT == 1 && !helps ? HD / 2 : HD); d += 32) {
               float num[32];
 #pragma unroll
               for (int y = 0; y < 32; ++y) num[y] = 0.f;
-              for (int c = c0; c <= c1; ++c) {
-                const float f = exp2_approx(__ldcg(from(c) + kRows * HD + 2 * local) - top);
-                float4 x[8];
+              // two partial sums on their way at a time
+              for (int c = c0; c <= c1; c += 2) {
+                float f[2];
+                float4 x[2][8];
 #pragma unroll
-                for (int y = 0; y < 8; ++y) x[y] = __ldcg(reinterpret_cast<const float4*>(from(c) + ((size_t)(d / 4 + y) * kRows + local) * 4));
+                for (int z = 0; z < 2; ++z) {
+                  const float* part = from(min(c + z, c1));
+                  f[z] = __ldcg(part + kRows * HD + 2 * local);
 #pragma unroll
-                for (int y = 0; y < 8; ++y) {
-                  num[4 * y] = fmaf(x[y].x, f, num[4 * y]);
-                  num[4 * y + 1] = fmaf(x[y].y, f, num[4 * y + 1]);
-                  num[4 * y + 2] = fmaf(x[y].z, f, num[4 * y + 2]);
-                  num[4 * y + 3] = fmaf(x[y].w, f, num[4 * y + 3]);
+                  for (int y = 0; y < 8; ++y) x[z][y] = __ldcg(reinterpret_cast<const float4*>(part + ((size_t)(d / 4 + y) * kRows + local) * 4));
+                }
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                  if (c + z > c1) break;
+                  const float by = exp2_approx(f[z] - top);
+#pragma unroll
+                  for (int y = 0; y < 8; ++y) {
+                    num[4 * y] = fmaf(x[z][y].x, by, num[4 * y]);
+                    num[4 * y + 1] = fmaf(x[z][y].y, by, num[4 * y + 1]);
+                    num[4 * y + 2] = fmaf(x[z][y].z, by, num[4 * y + 2]);
+                    num[4 * y + 3] = fmaf(x[z][y].w, by, num[4 * y + 3]);
+                  }
                 }
               }
 #pragma unroll
@@ -1512,15 +1586,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 float out[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) out[e] = num[y + e];
-                store_out8(p, a.start, a.h, row, d + y, out, inv);
+                store_out8(out_row + d + y, p.bf16, out, inv);
               }
             }
           }
           if (threadIdx.x == 0) counters[c0] = 0;
         }
-        named_barrier_sync(1, 128 * QT);  // *last_one is read before it is written again
+        named_barrier_sync(1, 256);  // *last_one is read before it is written again
       }
-    }
     }
   }
   tc_fence_before_sync();
@@ -1535,51 +1608,21 @@ size_t tile_workspace(int sms) {
   return kCounterBytes + (size_t)sms * 2 * TileLayout<HD>::kRows * (HD + 2) * 4;
 }
 
-struct CacheMapKey {
-  uintptr_t ptr;
-  long long rows;
-  int dim;
-  bool operator==(const CacheMapKey& o) const { return ptr == o.ptr && rows == o.rows && dim == o.dim; }
-};
-struct CacheMapHash {
-  size_t operator()(const CacheMapKey& k) const {
-    return std::hash<uintptr_t>()(k.ptr) ^ ((size_t)k.rows << 8) ^ (size_t)k.dim;
-  }
-};
-std::mutex g_cache_map_mutex;
-std::unordered_map<CacheMapKey, CUtensorMap, CacheMapHash> g_cache_maps[kMaxDevices];
-constexpr size_t kMaxCacheMaps = 4096;
-
 // The cache as a 2-D tensor of bytes [blocks * kv_heads * block_size][dim]; one
-// box is 16 tokens of one head (a 128-dim part of them), swizzled.  A map only
-// describes addresses, so it is looked up by them.
-int cache_map(const DeviceInfo& dev, const void* cache, long long rows, int dim, CUtensorMap* out) {
-  const CacheMapKey key{reinterpret_cast<uintptr_t>(cache), rows, dim};
-  {
-    std::lock_guard<std::mutex> lock(g_cache_map_mutex);
-    auto it = g_cache_maps[dev.ordinal].find(key);
-    if (it != g_cache_maps[dev.ordinal].end()) {
-      *out = it->second;
-      return GDSQ_OK;
-    }
-  }
+// box is 16 tokens of one head (a 128-dim part of them), swizzled.
+int cache_map(const void* cache, long long rows, int dim, CUtensorMap* out) {
   PFN_cuTensorMapEncodeTiled_v12000 encode;
   int st = get_encoder(&encode);
   if (st != GDSQ_OK) return st;
-  CUtensorMap map;
   const cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)dim};
   const cuuint32_t box[2] = {(cuuint32_t)std::min(dim, 128), 16};
   const cuuint32_t estr[2] = {1, 1};
-  CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(cache), dims, strides, box, estr,
+  CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(cache), dims, strides, box, estr,
                       CU_TENSOR_MAP_INTERLEAVE_NONE, dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(GDSQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for a cache of %lld x %d bytes", (int)r, rows, dim);
-  std::lock_guard<std::mutex> lock(g_cache_map_mutex);
-  if (g_cache_maps[dev.ordinal].size() >= kMaxCacheMaps) g_cache_maps[dev.ordinal].clear();
-  g_cache_maps[dev.ordinal][key] = map;
-  *out = map;
   return GDSQ_OK;
 }
 
@@ -1590,8 +1633,8 @@ int launch_stream(const AttendArgs& a, const DeviceInfo& dev, void* workspace, s
     return fail(GDSQ_ERR_INVALID_VALUE, "attend_kv8: workspace of %zu bytes, %zu needed", bytes, need);
   const long long rows = ((long long)a.num_blocks * a.kv_heads) << a.block_shift;
   CUtensorMap kmap, vmap;
-  int st = cache_map(dev, a.k_cache, rows, HD, &kmap);
-  if (st == GDSQ_OK) st = cache_map(dev, a.v_cache, rows, HD, &vmap);
+  int st = cache_map(a.k_cache, rows, HD, &kmap);
+  if (st == GDSQ_OK) st = cache_map(a.v_cache, rows, HD, &vmap);
   if (st != GDSQ_OK) return st;
   auto kernel = attend_stream_kernel<HD, F, NT>;
   constexpr int smem = StreamLayout<HD, NT>::kTotal;
@@ -1620,8 +1663,8 @@ int launch_tile(const AttendArgs& a, const DeviceInfo& dev, void* workspace, siz
   if ((size_t)dev.sms * sizeof(int) > kCounterBytes) return fail(GDSQ_ERR_UNSUPPORTED, "attend_kv8: %d SMs", dev.sms);
   const long long rows = ((long long)a.num_blocks * a.kv_heads) << a.block_shift;
   CUtensorMap kmap, vmap;
-  int st = cache_map(dev, a.k_cache, rows, HD, &kmap);
-  if (st == GDSQ_OK) st = cache_map(dev, a.v_cache, rows, HD, &vmap);
+  int st = cache_map(a.k_cache, rows, HD, &kmap);
+  if (st == GDSQ_OK) st = cache_map(a.v_cache, rows, HD, &vmap);
   if (st != GDSQ_OK) return st;
   auto kernel = attend_tile_kernel<HD, F>;
   constexpr int smem = TileLayout<HD>::kTotal;

@@ -30,7 +30,7 @@ namespace {
 // in shared memory, so that no CTA waits for another; then the CTAs share out
 // the tokens and the table rows.
 //
-// Bound by latency: 4.9 us on the GPU for 64 requests with a token each, 7.5 for
+// Bound by latency: 4.3 us on the GPU for 64 requests with a token each, 7.5 for
 // 1000 requests with up to 511 tokens each, whose 4 MB take 0.7 us of memory time.
 
 constexpr int kTabThreads = 1024;
@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(kTabThreads) build_tables_kernel(const TablesA
   int* first = starts + p.requests + 1;  // [requests] index into free_blocks
   __shared__ int wsum[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int threads = blockDim.x, warps = threads >> 5;
+  constexpr int threads = kTabThreads, warps = threads >> 5;
   pdl_launch_dependents();
   pdl_wait_primary();
   const int head = *p.free_head;
@@ -513,10 +513,8 @@ int gdsq_build_tables(const int32_t* context_lens, const int32_t* new_lens, int 
   const int smem = (2 * num_requests + 1) * (int)sizeof(int);
   cudaError_t e = ensure_smem(build_tables_kernel, smem, dev->ordinal);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(build_tables)");
-  // A step of few requests is bound by the barriers of a CTA, so it gets a small one.
-  const int threads = num_requests <= 256 && num_tokens <= 256 ? 256 : kTabThreads;
-  const int grid = std::max(1, std::min(dev->sms, (num_tokens + threads - 1) / threads));
-  e = launch(build_tables_kernel, dim3(grid), dim3(threads), smem, static_cast<cudaStream_t>(stream_v),
+  const int grid = std::max(1, std::min(dev->sms, (num_tokens + kTabThreads - 1) / kTabThreads));
+  e = launch(build_tables_kernel, dim3(grid), dim3(kTabThreads), smem, static_cast<cudaStream_t>(stream_v),
              g_pdl_enabled != 0, a);
   return e == cudaSuccess ? GDSQ_OK : cuda_fail(e, "build_tables launch");
 }
