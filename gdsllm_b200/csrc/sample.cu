@@ -55,6 +55,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBlock = 256;        // logits: 8 per lane
 constexpr int kMaxBlocks = 1024;   // per CTA
+constexpr int kMaxBinned = 511;    // with top_p: a CTA's weights in units of 2^16, at most 2^15 each, add up below 2^32
 constexpr int kBins = 2048;
 constexpr int kPerThread = kBins / kThreads;  // a 16-byte vector
 static_assert(kPerThread == 4, "bins are read by vectors");
@@ -420,10 +421,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs p,
     }
     __syncthreads();
   };
+  const bool carries = per_cta * kBlock > 65536;  // the low halves of this many weights can pass 2^32
   auto put = [&](bool weights, uint32_t bin, uint32_t w) {
     if (weights) {
-      atomicAdd(&sh.lo[bin], w & 0xffffu);
-      atomicAdd(&sh.hi[bin], w >> 16);
+      const uint32_t low = w & 0xffffu;
+      uint32_t high = w >> 16;
+      if (carries) high += atomicAdd(&sh.lo[bin], low) + low < low ? 65536u : 0u;
+      else atomicAdd(&sh.lo[bin], low);
+      atomicAdd(&sh.hi[bin], high);
     } else {
       atomicAdd(&sh.lo[bin], 1u);
     }
@@ -837,7 +842,7 @@ int launch_sample(const SampleArgs& a, int rows, cudaStream_t stream) {
   if (st != GDSQ_OK) return st;
   const int blocks = (a.vocab + 8 + kBlock - 1) / kBlock;
   int ranks = 1;
-  while (ranks < 8 && (blocks > ranks * kMaxBlocks || (ranks * rows <= dev->sms * (a.top_p ? 2 : 1) && blocks >= 32 * ranks))) ranks *= 2;
+  while (ranks < 8 && (blocks > ranks * (a.top_p ? kMaxBinned : kMaxBlocks) || (ranks * rows <= dev->sms * (a.top_p ? 2 : 1) && blocks >= 32 * ranks))) ranks *= 2;
   auto kernel = sample_kernel<T>;
   cudaError_t e = ensure_smem(kernel, (int)sizeof(SampleShared), dev->ordinal);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(sample)");

@@ -129,3 +129,18 @@ def test_frequencies(cuda):
     p = torch.softmax(row.double(), 0)
     count = torch.bincount(tokens, minlength=v).double()
     assert bool(((count - n * p).abs() <= 6 * torch.sqrt(n * p * (1 - p)) + 1).all())
+
+
+@pytest.mark.parametrize("vocab", [131072, 200000])
+def test_flat_rows_of_a_large_vocabulary(cuda, vocab):
+    """More than 2^16 logits of one value in a row that few CTAs share: sums of 2^48 and more."""
+    b = 300
+    x = torch.full((b, vocab), -3.0, dtype=torch.float16, device=cuda)
+    x[0] = 0.0
+    x[1::2, 7] = 0.0
+    u = torch.rand(b, generator=torch.Generator(device=cuda).manual_seed(5), device=cuda)
+    tokens, lp = sampling.sample(x, u, top_p=torch.full((b,), 0.5, device=cuda))
+    for i in (0, 1, 2, 3, 150, 299):
+        want, wlp = sample_ref(x[i], u[i], 1.0, 0, 0.5, 0.0)
+        assert tokens[i].item() == want
+        assert abs(lp[i].item() - wlp) <= 2.0 ** -22 * (1 + abs(wlp))
