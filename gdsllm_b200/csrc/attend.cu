@@ -827,11 +827,15 @@ size_t stream_workspace(int sms) {
 // output (a column of B is a dim).  With two tiles the order of products is
 // O0(i) S0(i+1) O1(i) S1(i+1), so that one tile's softmax runs beside the other's
 // products; the weights take the scores' place in TMEM.  Widened K needs no second
-// buffer: scores i are done long before K i+1 is needed; V has two.
+// buffer: scores i are done long before K i+1 is needed; V has two.  With one tile
+// (heads of 256) the scores alternate between two places, S(i+1) O(i), so that the
+// softmax runs beside the products all the same (44 us to 40 for the drafts below).
 //
 // Measured: three prompts of up to 2048 tokens over up to 6000 cached, 64 heads on
-// 8 of 128, e4m3: 609 us, 800 TFLOP/s counting the visible positions (half of the
-// measured matrix rate), where one tile with mma.sync took 3220.  A step of two
+// 8 of 128, e4m3: 566 us, 862 TFLOP/s counting the visible positions (53 % of the
+// measured matrix rate), where one tile with mma.sync took 3220; 33 requests with
+// five tokens each, 32 heads on 2 of 256, over up to 2047: 30 us, bound by latency
+// (the schedule 3 k cycles, Q 8 k, a step 2 k, the output 2 k, a join 10 k).  A step of two
 // tiles takes about 4600 cycles: 2048 are the exponential unit's (32768 weights,
 // 16 a cycle), 2600 the products', at 80 to 90 cycles where alone they take 64,
 // since the widening and the Q tiles use the same shared memory, and the two
@@ -854,9 +858,10 @@ struct TileLayout {
 };
 constexpr int kTileThreads = 16 * 32;
 // What beginning and ending an item costs, in tokens: the three prompts above
-// take 597 us with 11 steps of 128, 728 with 2, 631 with 6 and 611 with 15.
+// take 565 us with 896, 576 with 768 and 569 with 1024; for heads of 256 the 33
+// requests with five tokens take 30.1 us with 320, 31.0 with 448.
 template <int HD>
-__host__ __device__ constexpr int item_tokens() { return HD == 256 ? 448 : 1024; }
+__host__ __device__ constexpr int item_tokens() { return HD == 256 ? 320 : 896; }
 // Registers per thread of the softmax, widening and other warp groups: together the launch's 4 x 128.
 constexpr int kSoftmaxRegs = 176, kWidenRegs = 80, kOtherRegs = 80;
 
@@ -1650,10 +1655,12 @@ int launch_stream(const AttendArgs& a, const DeviceInfo& dev, void* workspace, s
 
 // Rows per (request, KV head) up to which the stream kernel is taken; a tile's 128
 // rows are a whole product however few are filled.  Stream against tile, heads of
-// 128: 20 rows 69 and 113 us, 24 rows 187 and 332, 32 rows 126 and 220; 64 rows
-// would take the stream kernel 78 us and take the tile kernel 60.
+// 128: 20 rows of 32 requests of 2000 tokens 70 and 84 us, 24 rows of 64 of 4000
+// 187 and 251, 32 rows of 16 of 2000 (32 KV heads) 126 and 160.  Heads of 256 leave
+// the stream kernel registers for 16 rows only: 32 rows of 16 requests of 1000
+// tokens would take it two readings of the cache, 33 us, and take the tile kernel 26.
 template <int HD>
-constexpr int stream_rows() { return 32; }
+constexpr int stream_rows() { return HD == 256 ? 16 : 32; }
 
 template <int HD, int F>
 int launch_tile(const AttendArgs& a, const DeviceInfo& dev, void* workspace, size_t bytes, cudaStream_t stream) {
@@ -1681,7 +1688,7 @@ int launch_attend(const AttendArgs& a, int max_query_len, const DeviceInfo& dev,
                   cudaStream_t stream) {
   const long long rows = (long long)max_query_len * a.group;
   if (rows <= 8) return launch_stream<HD, F, 1>(a, dev, workspace, bytes, stream);
-  if (rows <= 16 || (HD == 256 && rows <= stream_rows<HD>())) return launch_stream<HD, F, 2>(a, dev, workspace, bytes, stream);
+  if (rows <= 16) return launch_stream<HD, F, 2>(a, dev, workspace, bytes, stream);
   if constexpr (HD != 256)
     if (rows <= stream_rows<HD>()) return launch_stream<HD, F, 4>(a, dev, workspace, bytes, stream);
   return launch_tile<HD, F>(a, dev, workspace, bytes, stream);
@@ -1710,14 +1717,14 @@ extern "C" size_t gdsq_attend_kv8_workspace(int num_requests, int max_query_len,
   const long long rows = (long long)max_query_len * (num_heads / num_kv_heads);
   // the largest of the variants that up to this many rows can take
   const int n = dev->sms;
-  auto most = [&](size_t one, size_t two, size_t four, size_t tile) {
-    return std::max(std::max(one, rows > 8 ? two : 0), std::max(rows > 16 ? four : 0, rows > 32 ? tile : 0));
+  auto most = [&](size_t one, size_t two, size_t four, int upto, size_t tile) {
+    return std::max(std::max(one, rows > 8 ? two : 0), std::max(rows > 16 ? four : 0, rows > upto ? tile : 0));
   };
   if (head_dim == 64)
-    return most(stream_workspace<64, 1>(n), stream_workspace<64, 2>(n), stream_workspace<64, 4>(n), tile_workspace<64>(n));
+    return most(stream_workspace<64, 1>(n), stream_workspace<64, 2>(n), stream_workspace<64, 4>(n), stream_rows<64>(), tile_workspace<64>(n));
   if (head_dim == 128)
-    return most(stream_workspace<128, 1>(n), stream_workspace<128, 2>(n), stream_workspace<128, 4>(n), tile_workspace<128>(n));
-  return most(stream_workspace<256, 1>(n), stream_workspace<256, 2>(n), 0, tile_workspace<256>(n));
+    return most(stream_workspace<128, 1>(n), stream_workspace<128, 2>(n), stream_workspace<128, 4>(n), stream_rows<128>(), tile_workspace<128>(n));
+  return most(stream_workspace<256, 1>(n), stream_workspace<256, 2>(n), 0, stream_rows<256>(), tile_workspace<256>(n));
 }
 
 extern "C" int gdsq_attend_kv8(const void* q, int elem_type, long long q_token_stride, long long q_head_stride,
