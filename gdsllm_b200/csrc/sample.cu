@@ -46,8 +46,8 @@ namespace {
 //
 // Bound by the passes over a row where top_p stands alone (its bins are shared
 // atomics), else by latency: 256 rows of 131072 fp16 logits with all mixes of
-// filters take 105 us (10.3 for reading them once), with top_k in each row 39,
-// with top_p alone in each 154; one row of 32000 with top_k and top_p 8.9 us; 48
+// filters take 106 us (10.3 for reading them once), with top_k in each row 39,
+// with top_p alone in each 156, without filters 49; one row of 32000 with top_k and top_p 8.9 us; 48
 // rows of 50001 fp32 logits without filters 13 us (1.5 for reading).  Counting all
 // logits by bins, without lists, the 256 mixed rows took 3270 us and the one row 445.
 
