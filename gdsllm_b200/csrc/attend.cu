@@ -421,14 +421,16 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
         if (lane == 0 && i < a.count && !dead) issue(used + i, a.once, lo, hi);
       }
     }
+    // lane i finds where the warp's row i is
+    const int mine_row = a.row0 + warp + (lane % kMine) * kAttWarps;
+    const long long mine_at = (long long)(a.start + mine_row / p.group) * p.q_token_stride +
+                              (long long)(a.h * p.group + mine_row % p.group) * p.q_head_stride;
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
-      const int row = a.row0 + warp + i * kAttWarps;
+      const long long at = __shfl_sync(0xffffffffu, mine_at, i);
 #pragma unroll
       for (int e = 0; e < kPairs; ++e) raw[i][e] = 0;
-      if (row < a.rows)
-        load_q<kPairs>(p, (long long)(a.start + row / p.group) * p.q_token_stride +
-                              (long long)(a.h * p.group + row % p.group) * p.q_head_stride + lane * (HD / 32), raw[i]);
+      if (a.row0 + warp + i * kAttWarps < a.rows) load_q<kPairs>(p, at + lane * (HD / 32), raw[i]);
     }
   };
 
@@ -442,9 +444,13 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
     const int first_lim = now.lim0 + row0 / p.group;
     int2 nxt = make_int2(0, 0);
     // Q rows: power-of-two scale, fp16, in operand order.
+    if (lane < kMine) {
+      const int i = warp + lane * kAttWarps, row = row0 + i;
+      qlim[i] = row < rows ? now.lim0 + row / p.group : now.kv_len - 1;  // rows past the end are not written
+    }
 #pragma unroll
     for (int ii = 0; ii < kMine; ++ii) {
-      const int i = warp + ii * kAttWarps, row = row0 + i;
+      const int i = warp + ii * kAttWarps;
       float v[HD / 32];
       float most = 0.f;
 #pragma unroll
@@ -460,7 +466,6 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
       const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
       if (lane == 0) {
         qexp[i] = __uint_as_float((uint32_t)(127 + ex) << 23);
-        qlim[i] = row < rows ? now.lim0 + row / p.group : now.kv_len - 1;  // rows past the end are not written
       }
 #pragma unroll
       for (int e = 0; e < HD / 32; e += 2) {
