@@ -30,11 +30,12 @@ namespace {
 // in shared memory, so that no CTA waits for another; then the CTAs share out
 // the tokens and the table rows.
 //
-// Bound by latency: 4.3 us on the GPU for 64 requests with a token each, 7.5 for
+// Bound by latency: 4.5 us on the GPU for 64 requests with a token each, 8.0 for
 // 1000 requests with up to 511 tokens each, whose 4 MB take 0.7 us of memory time.
 
 constexpr int kTabThreads = 1024;
 constexpr int kTabMaxRequests = 16384;
+constexpr int kTabMaxLen = (1 << 30) - (1 << 10);  // of a request, cached or new
 
 struct TablesArgs {
   const int* context;
@@ -54,7 +55,7 @@ __global__ void __launch_bounds__(kTabThreads) build_tables_kernel(const TablesA
   extern __shared__ int sm[];
   int* starts = sm;                      // [requests + 1]
   int* first = starts + p.requests + 1;  // [requests] index into free_blocks
-  __shared__ int wsum[2][32];
+  __shared__ long long wsum[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int threads = kTabThreads, warps = threads >> 5;
   pdl_launch_dependents();
@@ -62,47 +63,80 @@ __global__ void __launch_bounds__(kTabThreads) build_tables_kernel(const TablesA
   const int head = *p.free_head;
   const int per = (p.requests + threads - 1) / threads;
   const int r0 = min(tid * per, p.requests), r1 = min(r0 + per, p.requests);
-  int tok = 0, blk = 0;
-  bool bad = head < 0;
+  bool bad = head < 0, wide = false;
+  // Lengths that no table holds are cut off, and sums stop at the largest int, so that no index wraps.
+  constexpr int kMost = 0x7fffffff;
+  auto held_of = [&](int r) { return min(max(p.context[r], 0), kTabMaxLen); };
+  auto new_of = [&](int r) { return min(max(p.fresh[r], 0), kTabMaxLen); };
   for (int r = r0; r < r1; ++r) {
-    const int c = max(p.context[r], 0), n = max(p.fresh[r], 0);
-    bad |= p.context[r] < 0 || p.fresh[r] < 0;
-    starts[r] = tok;
-    first[r] = blk;
-    tok += n;
-    blk += (c + n + p.block - 1) / p.block - (c + p.block - 1) / p.block;
+    const int n = new_of(r);
+    bad |= p.context[r] != held_of(r) || p.fresh[r] != n;
+    wide |= n > 65535;  // else 2^14 requests' sums fit in 31 bits
   }
-  int ts = tok, bsum = blk;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int a = __shfl_up_sync(0xffffffffu, ts, d), b = __shfl_up_sync(0xffffffffu, bsum, d);
-    if (lane >= d) {
-      ts += a;
-      bsum += b;
+  int tall = 0;
+  long long blocks = 0;
+  auto running_sums = [&](auto zero) {
+    using Sum = decltype(zero);
+    Sum tok = 0, blk = 0;
+    for (int r = r0; r < r1; ++r) {
+      const int c = held_of(r), n = new_of(r);
+      starts[r] = (int)min((long long)tok, (long long)kMost);
+      first[r] = (int)min((long long)blk, (long long)kMost);
+      tok += n;
+      blk += (c + n + p.block - 1) / p.block - (c + p.block - 1) / p.block;
     }
-  }
-  if (lane == 31) {
-    wsum[0][warp] = ts;
-    wsum[1][warp] = bsum;
-  }
-  __syncthreads();
-  const int wt = lane < warps ? wsum[0][lane] : 0, wb = lane < warps ? wsum[1][lane] : 0;
-  const int tb = ts - tok + __reduce_add_sync(0xffffffffu, lane < warp ? wt : 0);
-  const int bb = bsum - blk + __reduce_add_sync(0xffffffffu, lane < warp ? wb : 0);
-  const int tall = __reduce_add_sync(0xffffffffu, wt), ball = __reduce_add_sync(0xffffffffu, wb);
-  for (int r = r0; r < r1; ++r) {
-    starts[r] += tb;
-    first[r] += head + bb;
-  }
+    Sum ts = tok, bsum = blk;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const Sum a = __shfl_up_sync(0xffffffffu, ts, d), b = __shfl_up_sync(0xffffffffu, bsum, d);
+      if (lane >= d) {
+        ts += a;
+        bsum += b;
+      }
+    }
+    if (lane == 31) {
+      wsum[0][warp] = ts;
+      wsum[1][warp] = bsum;
+    }
+    __syncthreads();
+    Sum wt = (Sum)wsum[0][lane], wb = (Sum)wsum[1][lane];
+    Sum tb = lane < warp ? wt : 0, bb = lane < warp ? wb : 0;
+    if constexpr (sizeof(Sum) == 4) {
+      tb = __reduce_add_sync(0xffffffffu, tb);
+      bb = __reduce_add_sync(0xffffffffu, bb);
+      wt = __reduce_add_sync(0xffffffffu, wt);
+      wb = __reduce_add_sync(0xffffffffu, wb);
+    } else {
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) {
+        tb += __shfl_xor_sync(0xffffffffu, tb, d);
+        bb += __shfl_xor_sync(0xffffffffu, bb, d);
+        wt += __shfl_xor_sync(0xffffffffu, wt, d);
+        wb += __shfl_xor_sync(0xffffffffu, wb, d);
+      }
+    }
+    tb += ts - tok;
+    bb += bsum - blk;
+    bad |= wt > p.tokens;
+    tall = (int)min((long long)wt, (long long)kMost);
+    blocks = wb;
+    for (int r = r0; r < r1; ++r) {
+      starts[r] = (int)min((long long)starts[r] + tb, (long long)kMost);
+      first[r] = (int)min((long long)first[r] + head + bb, (long long)kMost);
+    }
+  };
+  static_assert(warps == 32, "a lane for each warp's sums");
+  if (__syncthreads_or(wide)) running_sums(0ll);
+  else running_sums(0);
   if (tid == 0) starts[p.requests] = tall;
   __syncthreads();
 
-  auto free_block = [&](int i) { return i >= 0 && i < p.num_free ? p.free_blocks[i] : -1; };
+  auto free_block = [&](long long i) { return i >= 0 && i < p.num_free ? p.free_blocks[i] : -1; };
   for (int r = blockIdx.x * warps + warp; r < p.requests; r += gridDim.x * warps) {
-    const int c = max(p.context[r], 0), n = starts[r + 1] - starts[r];
+    const int c = held_of(r), n = min(starts[r + 1] - starts[r], kTabMaxLen);
     const int held = (c + p.block - 1) / p.block, after = (c + n + p.block - 1) / p.block;
     for (int j = held + lane; j < min(after, p.width); j += 32) {
-      const int b = free_block(first[r] + j - held);
+      const int b = free_block((long long)first[r] + j - held);
       bad |= b < 0;
       p.table[(size_t)r * p.width + j] = b;
     }
@@ -112,11 +146,10 @@ __global__ void __launch_bounds__(kTabThreads) build_tables_kernel(const TablesA
       p.starts[r] = starts[r];
       if (r == 0) {
         p.starts[p.requests] = tall;
-        *p.head_out = head + ball;
+        *p.head_out = (int)min(head + blocks, (long long)kMost);
       }
     }
   }
-  bad |= tall > p.tokens;
   const long long stride = (long long)gridDim.x * threads;
   for (long long i = (long long)blockIdx.x * threads + tid; i < p.tokens; i += stride) {
     long long pos = 0, slot = -1;
@@ -127,11 +160,11 @@ __global__ void __launch_bounds__(kTabThreads) build_tables_kernel(const TablesA
         if (starts[mid] <= i) lo = mid;
         else hi = mid;
       }
-      const int c = max(p.context[lo], 0);
+      const int c = held_of(lo);
       pos = c + (i - starts[lo]);
       const int col = (int)(pos / p.block), held = (c + p.block - 1) / p.block;
       if (col < p.width) {
-        const int b = col < held ? p.table[(size_t)lo * p.width + col] : free_block(first[lo] + col - held);
+        const int b = col < held ? p.table[(size_t)lo * p.width + col] : free_block((long long)first[lo] + col - held);
         if (b >= 0) slot = (long long)b * p.block + pos % p.block;
         bad |= b < 0;
       }
@@ -492,9 +525,9 @@ int gdsq_build_tables(const int32_t* context_lens, const int32_t* new_lens, int 
                       long long* slots, int32_t* free_head_out, void* stream_v) {
   t_last_error.clear();
   if (num_requests < 1 || num_requests > kTabMaxRequests || table_width < 0 || num_free < 0 || block_size < 1 ||
-      num_tokens < 0)
+      block_size > 1024 || num_tokens < 0)
     return fail(GDSQ_ERR_INVALID_VALUE, "build_tables: requests %d (1..%d), table width %d, free blocks %d, block "
-                "size %d, tokens %d", num_requests, kTabMaxRequests, table_width, num_free, block_size, num_tokens);
+                "size %d (1..1024), tokens %d", num_requests, kTabMaxRequests, table_width, num_free, block_size, num_tokens);
   if (!context_lens || !new_lens || (!block_table && table_width) || (!free_blocks && num_free) || !free_head ||
       !seq_lens || !query_starts || (num_tokens && (!positions || !slots)) || !free_head_out)
     return fail(GDSQ_ERR_INVALID_VALUE, "build_tables: null pointer");

@@ -92,6 +92,24 @@ def test_tables_short_queue_and_row(cuda):
     assert capi.device_error(0) == 0
 
 
+def test_tables_lengths_near_the_largest_int(cuda):
+    """Lengths that no table holds: reported, the rows' own neighbours untouched, the sums stop at the largest int."""
+    big, bs = 2 ** 31 - 1, 16
+    table = torch.full((3, 4), -7, dtype=torch.int32, device=cuda)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
+    t = paged.build_tables(i32(big, 0, 3), i32(5, 2, 2), table, i32(4, 5, 6, 7), i32(0), bs, 9)
+    assert capi.device_error(0) == 4
+    assert table[0].tolist() == [-7] * 4 and table[1].tolist()[1:] == [-7] * 3 and table[2].tolist() == [-7] * 4
+    assert t.query_starts.tolist() == [0, 5, 7, 9] and t.slots[:5].tolist() == [-1] * 5
+    assert t.slots[5:7].tolist() == [table[1, 0].item() * bs, table[1, 0].item() * bs + 1]
+    t = paged.build_tables(i32(0, 0, 0), i32(big, big, big), table, i32(4, 5, 6, 7), i32(0), bs, 20)
+    assert capi.device_error(0) == 4
+    assert table[0].tolist() == [4, 5, 6, 7] and t.slots.tolist() == [4 * bs + i for i in range(16)] + [5 * bs + i for i in range(4)]
+    assert t.query_starts.tolist()[3] == big
+    assert capi.device_error(0) == 0
+
+
+
 # ---- cache write ------------------------------------------------------------------
 
 def append_ref(x, slots, cache, scale, kind):
