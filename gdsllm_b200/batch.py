@@ -149,12 +149,14 @@ class BatchLlama:
                     top_p=torch.full((n,), top_p, device=dev), min_p=torch.full((n,), min_p, device=dev))
         idle = [[]] * (self.max_requests - n)
         step, tokens, logprobs = [list(p) for p in prompts], [], []
-        for _ in range(new_tokens):
-            logits = self.step(step + idle)
-            t, lp = sampling.sample(logits[:n], torch.rand(n, generator=gen, device=dev), **rows)
-            tokens.append(t.cpu())
-            logprobs.append(lp.cpu())
-            step = [[i] for i in tokens[-1].tolist()]
-        for r in range(n):
-            self.release(r)
+        try:
+            for _ in range(new_tokens):
+                logits = self.step(step + idle)
+                t, lp = sampling.sample(logits[:n], torch.rand(n, generator=gen, device=dev), **rows)
+                tokens.append(t.cpu())
+                logprobs.append(lp.cpu())
+                step = [[i] for i in tokens[-1].tolist()]
+        finally:
+            for r in range(n):
+                self.release(r)
         return torch.stack(tokens, 1), torch.stack(logprobs, 1)
