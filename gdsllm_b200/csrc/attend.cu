@@ -839,7 +839,7 @@ size_t stream_workspace(int sms) {
 // Measured: three prompts of up to 2048 tokens over up to 6000 cached, 64 heads on
 // 8 of 128, e4m3: 566 us, 862 TFLOP/s counting the visible positions (53 % of the
 // measured matrix rate), where one tile with mma.sync took 3220; 33 requests with
-// five tokens each, 32 heads on 2 of 256, over up to 2047: 30 us, bound by latency
+// five tokens each, 32 heads on 2 of 256, over up to 2047: 31 us, bound by latency
 // (the schedule 3 k cycles, Q 8 k, a step 2 k, the output 2 k, a join 10 k).  A step of two
 // tiles takes about 4600 cycles: 2048 are the exponential unit's (32768 weights,
 // 16 a cycle), 2600 the products', at 80 to 90 cycles where alone they take 64,
