@@ -1555,11 +1555,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             auto from = [&](int c) { return parts + ((size_t)(2 * c + (c == c0)) * kRows) * (HD + 2); };
             float top = kNoMax, den = 0.f;
 #pragma unroll 4
-            for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(from(c) + kRows * HD + 2 * local));
-#pragma unroll 4
             for (int c = c0; c <= c1; ++c) {
               const float2 ml = __ldcg(reinterpret_cast<const float2*>(from(c) + kRows * HD + 2 * local));
-              den = fmaf(ml.y, exp2_approx(ml.x - top), den);
+              const float high = fmaxf(top, ml.x);
+              den = fmaf(ml.y, exp2_approx(ml.x - high), den * exp2_approx(top - high));
+              top = high;
             }
             const float inv = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll 1
