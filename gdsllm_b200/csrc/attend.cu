@@ -969,8 +969,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 20);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_at + 1);  // a wait ran out
   int* last_one = reinterpret_cast<int*>(tmem_at + 2);
-  long long* shared_ll = reinterpret_cast<long long*>(bars + 24);    // [14] and one more
-  int* shared_r = reinterpret_cast<int*>(bars + 40);
+  // The schedule: a sum from each warp, and apart from them what one thread finds while the sums are still being read.
+  constexpr int kWarps = kTileThreads / 32, kSumsAt = 24, kFoundAt = 47;
+  static_assert(kSumsAt + kWarps <= 40 && kFoundAt >= 47 && (kFoundAt + 1) * 8 <= 512, "the schedule's words overlap others");
+  long long* warp_sums = reinterpret_cast<long long*>(bars + kSumsAt);  // [kWarps]
+  int* shared_r = reinterpret_cast<int*>(bars + 40);                    // the CTA's first request ..
+  long long* shared_at = reinterpret_cast<long long*>(bars + kFoundAt);  // .. and where it begins
   uint64_t* const_empty = bars + 42;  // [2]
   const float4* consts = reinterpret_cast<const float4*>(smem + L::kConst);  // [2][BN / 16]
 
@@ -1029,16 +1033,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const long long x = __shfl_up_sync(0xffffffffu, upto, d);
     if (lane >= d) upto += x;
   }
-  if (lane == 31) shared_ll[warp] = upto;
+  if (lane == 31) warp_sums[warp] = upto;
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *tmem_at;
   long long before = upto - mine;
   all = 0;
-  for (int w = 0; w < kTileThreads / 32; ++w) {
-    if (w < warp) before += shared_ll[w];
-    all += shared_ll[w];
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += warp_sums[w];
+    all += warp_sums[w];
   }
   const long long C = max(min((long long)gridDim.x, all / BN), 1ll);  // a share holds a step at least
   const bool works = blockIdx.x < C && all > 0;
@@ -1053,11 +1057,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       at += n;
     }
     *shared_r = r;
-    shared_ll[15] = at;
+    *shared_at = at;
   }
   __syncthreads();
   int r = works ? *shared_r : 0;
-  request_at = works ? shared_ll[15] : 0;
+  request_at = works ? *shared_at : 0;
 
   struct Segment {
     int r, h, row0, rows, start, lim0;  // row i of the item sees positions up to lim0 + (row0 + i) / group
