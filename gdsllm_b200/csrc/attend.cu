@@ -415,6 +415,8 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
   auto begin = [&](const Segment& a, int2& at, uint32_t(&raw)[kMine][kPairs]) {
     if (a.count > 0) {
       at = half_row(a, 0);
+      // The warp has read the stages' last tiles (the __syncwarp that ends a step); the copies come after those reads.
+      if (lane == 0) fence_proxy_async_smem();
 #pragma unroll
       for (int i = 0; i < kRing; ++i) {
         const int lo = __shfl_sync(0xffffffffu, at.y, 2 * i), hi = __shfl_sync(0xffffffffu, at.y, 2 * i + 1);

@@ -49,6 +49,14 @@ def test_tile_schedule(cuda, requests, heads, kv_heads, dim):
     check_repeated(cuda, "e4m3", heads, kv_heads, dim, 16, [max(n, 1) for n in lens], new, 200, requests + dim)
 
 
+@pytest.mark.parametrize("requests", [2, 129, 300, 1000])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 1, 128), (10, 1, 256), (24, 1, 64)])
+def test_stream_schedule(cuda, requests, heads, kv_heads, dim):
+    rng = random.Random(requests)
+    lens = [rng.choice([1, 15, 64, 130, 300]) for _ in range(requests)]
+    check_repeated(cuda, "int8", heads, kv_heads, dim, 16, lens, [1] + [rng.choice([0, 1]) for _ in range(requests - 1)], 200, requests + dim)
+
+
 def test_prompts_beside_single_tokens(cuda):
     """One prompt chunk among decoding requests: all of them take the kernel that its rows ask for."""
     rng = random.Random(6)
