@@ -539,6 +539,30 @@ int gdsq_build_tables(const int32_t* context_lens, const int32_t* new_lens, int 
       !aligned(free_head, 4) || !aligned(seq_lens, 4) || !aligned(query_starts, 4) || !aligned(positions, 8) ||
       !aligned(slots, 8) || !aligned(free_head_out, 4))
     return fail(GDSQ_ERR_MISALIGNED, "build_tables: 4-byte (positions and slots 8-byte) alignment");
+  // Other CTAs and later loops read the inputs again after the first outputs are written, so nothing may be both.
+  struct Range {
+    const char* name;
+    const void* at;
+    unsigned long long bytes;
+    bool overlaps(const Range& o) const {
+      const auto a = reinterpret_cast<uintptr_t>(at), b = reinterpret_cast<uintptr_t>(o.at);
+      return bytes && o.bytes && a < b + o.bytes && b < a + bytes;
+    }
+  };
+  const unsigned long long r = num_requests, t = num_tokens;
+  const Range outputs[] = {{"seq_lens", seq_lens, 4 * r},       {"query_starts", query_starts, 4 * (r + 1)},
+                           {"positions", positions, 8 * t},     {"slots", slots, 8 * t},
+                           {"free_head_out", free_head_out, 4}, {"block_table", block_table, 4 * r * table_width}};
+  const Range inputs[] = {{"context_lens", context_lens, 4 * r},
+                          {"new_lens", new_lens, 4 * r},
+                          {"free_blocks", free_blocks, 4ull * num_free},
+                          {"free_head", free_head, 4}};
+  for (const Range& o : outputs) {
+    for (const Range& i : inputs)
+      if (o.overlaps(i)) return fail(GDSQ_ERR_INVALID_VALUE, "build_tables: %s overlaps %s", o.name, i.name);
+    for (const Range& i : outputs)
+      if (&i != &o && o.overlaps(i)) return fail(GDSQ_ERR_INVALID_VALUE, "build_tables: %s overlaps %s", o.name, i.name);
+  }
   const DeviceInfo* dev = nullptr;
   int st = device_info(&dev);
   if (st != GDSQ_OK) return st;

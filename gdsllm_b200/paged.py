@@ -46,7 +46,9 @@ def build_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table
     gets its new entries in place, from ``free_blocks[free_head:]`` in request
     order.  ``num_tokens`` sizes the per-token outputs; tokens past the sum of
     ``new_lens`` get slot -1.  A row or a queue that is too short sets device
-    error bit 4 (``capi.device_error``)."""
+    error bit 4 (``capi.device_error``).  ``out`` takes the results in place of
+    new tensors; none of them may share memory with an input, so a loop that
+    feeds ``seq_lens`` and ``free_head`` back takes turns between two."""
     t = ext().build_tables(context_lens, new_lens, block_table, free_blocks, free_head, block_size, num_tokens, out)
     return StepTables(*t) if out is None else out
 

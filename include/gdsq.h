@@ -378,9 +378,10 @@ GDSQ_API int gdsq_argmax_f16(const void* logits, int n, long long* token, long l
  * request order), seq_lens[r] = context + new, query_starts [requests + 1] =
  * the running sum of new_lens, and for each of the num_tokens new tokens its
  * position and slot; tokens past the last request get position 0, slot -1.
- * *free_head_out = *free_head + blocks taken (not the same address).  All
- * arrays int32 except positions and slots (int64).  At most 16384 requests,
- * block_size at most 1024.  A length that is negative or above 2^30 - 1024 (it
+ * *free_head_out = *free_head + blocks taken.  All arrays int32 except positions
+ * and slots (int64).  No output (the block table is one) may overlap an input or
+ * another output: the next step's lengths go into arrays of their own.  At most
+ * 16384 requests, block_size at most 1024.  A length that is negative or above 2^30 - 1024 (it
  * is cut off), a row or queue that is too short or more new tokens than
  * num_tokens sets device error bit 4; the entries it concerns become -1. */
 GDSQ_API int gdsq_build_tables(const int32_t* context_lens, const int32_t* new_lens, int num_requests,
