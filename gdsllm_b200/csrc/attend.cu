@@ -41,6 +41,8 @@ namespace {
 
 constexpr int kAttWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f;
+// Positions of a table row: positions, and those of the 16 tiles of 128 tokens that a lane looks up ahead, stay below 2^31.
+constexpr long long kMostPositions = (1ll << 31) - 4096;
 constexpr float kNoMax = -1e30f;       // the running maximum before any score
 constexpr float kMaxLogScale = 100.f;  // |log2| of a value scale is held to this
 
@@ -1775,6 +1777,9 @@ extern "C" int gdsq_attend_kv8(const void* q, int elem_type, long long q_token_s
   if ((((long long)num_blocks * num_kv_heads * block_size) >> 31) != 0 || num_blocks < 1)
     return fail(GDSQ_ERR_UNSUPPORTED, "attend_kv8: %d blocks of %d heads x %d tokens, not 1 to 2^31 - 1 rows", num_blocks,
                 num_kv_heads, block_size);
+  if ((long long)table_width * block_size > kMostPositions)
+    return fail(GDSQ_ERR_UNSUPPORTED, "attend_kv8: table rows of %d blocks of %d tokens, more than 2^31 - 4096 positions", table_width,
+                block_size);
   const DeviceInfo* dev = nullptr;
   int st = device_info(&dev);
   if (st != GDSQ_OK) return st;

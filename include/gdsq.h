@@ -420,7 +420,9 @@ GDSQ_API int gdsq_append_kv8(int elem_type, const void* q, long long q_token_str
  * workspace: workspace_bytes of device memory, zeroed before its first use
  * and left zeroed where it has to be by every call; calls that may overlap
  * need one each.  gdsq_attend_kv8_workspace says how much a call can use. A
- * block table entry out of range sets device error bit 4 and reads block 0. */
+ * block table entry out of range sets device error bit 4 and reads block 0; a
+ * length that the table row cannot hold is cut off and sets it too.  A row names
+ * at most 2^31 - 4096 positions (table_width * block_size). */
 GDSQ_API size_t gdsq_attend_kv8_workspace(int num_requests, int max_query_len, int num_heads, int num_kv_heads,
                                           int head_dim);
 GDSQ_API int gdsq_attend_kv8(const void* q, int elem_type, long long q_token_stride, long long q_head_stride,

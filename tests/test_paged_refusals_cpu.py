@@ -31,3 +31,14 @@ def test_tables_refuse_an_output_that_overlaps(output):
             assert tables(**{output: at}) == 1, (output, other, at)
             text = lib().gdsq_last_error()
             assert (b"overlaps" in text or b"must not be" in text) and output.encode() in text, text
+
+
+def attend(width, block, requests=1):
+    return lib().gdsq_attend_kv8(P, 0, 64, 64, P, P, 0, P, P, 4, block, P, width, P, P, requests, 1, 1, 64, 2, 1, 64, 0.1, P, P, 1 << 30, None)
+
+
+@pytest.mark.parametrize("width,block", [(1 << 27, 16), (1 << 24, 128), ((1 << 26) - 1, 32), (2 ** 31 - 1, 64)])
+def test_attend_refuses_a_table_row_past_31_bits(width, block):
+    """table_width * block_size is a position in the kernels."""
+    assert attend(width, block) == 3
+    assert b"positions" in lib().gdsq_last_error()
