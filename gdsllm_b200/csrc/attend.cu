@@ -866,6 +866,10 @@ struct TileLayout {
   static constexpr int kTotal = kNeed > 116 * 1024 ? kNeed : 116 * 1024;  // one CTA (512 TMEM columns) per SM
 };
 constexpr int kTileThreads = 16 * 32;
+// Tokens that are added up in tensor memory before the sum is taken out.  The tensor cores cut off what does not fit when they add,
+// always toward zero: over 131072 tokens of about equal weight a sum came out 1.0e-3 of itself too small, over 16384 at a time as
+// exact as fp16 shows (1.8e-4, the rounding of the output).
+constexpr int kChain = 16384;
 // What beginning and ending an item costs, in tokens: the three prompts above
 // take 565 us with 896, 576 with 768 and 569 with 1024; for heads of 256 the 33
 // requests with five tokens take 30.1 us with 320, 31.0 with 448.
@@ -1067,13 +1071,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   int r = works ? *shared_r : 0;
   request_at = works ? *shared_at : 0;
 
+  // What a CTA takes of an item is its run; a segment is up to kChain tokens of a run.
   struct Segment {
     int r, h, row0, rows, start, lim0;  // row i of the item sees positions up to lim0 + (row0 + i) / group
     int t0, t1, count;                  // first token, the end, and the steps
     int steps;              // of the item
     long long first_token;  // of the item, in the schedule
-    bool opens, whole;
+    bool opens, whole;      // the run begins the item; it is all of the item
+    bool goes_on, last;     // not the run's first segment; its last
   };
+  const long long cta_s0 = s0;
   auto next_segment = [&](Segment& a) {
     while (s0 < s1) {
       const int start = max(p.starts[r], 0);
@@ -1107,16 +1114,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       a.lim0 = len - n;
       const int kv_len = max(min(len, a.lim0 + (min(rows, a.row0 + kRows) - 1) / p.group + 1), 0);
       a.steps = max(ceil_div(kv_len, BN), 1);
-      // steps whose first token is at s0 or after it, and before s1
-      const int step = (int)max((s0 - a.first_token + BN - 1) / BN, 0ll);
-      const int step_end = (int)min((long long)a.steps, max((s1 - a.first_token + BN - 1) / BN, 0ll));
-      s0 = item_end;
+      // steps whose first token is at a share's start or after it, and before its end
+      auto step_from = [&](long long at) { return (int)min(max((at - a.first_token + BN - 1) / BN, 0ll), (long long)a.steps); };
+      const int step = step_from(s0), run_begin = step_from(cta_s0), run_end = step_from(s1);
+      const int step_end = min(run_end, step + kChain / BN);
+      a.last = step_end == run_end;
+      s0 = a.last ? item_end : a.first_token + (long long)step_end * BN;
       if (step >= step_end) continue;
       a.t0 = step * BN;
       a.t1 = min(kv_len, step_end * BN);
       a.count = a.t0 < a.t1 ? (a.t1 - a.t0 + BN - 1) / BN : 0;
-      a.opens = step == 0;
-      a.whole = step == 0 && step_end == a.steps;
+      a.opens = run_begin == 0;
+      a.whole = run_begin == 0 && run_end == a.steps;
+      a.goes_on = step > run_begin;
       return true;
     }
     return false;
@@ -1519,6 +1529,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           ++seg;
           tc_fence_after_sync();
         }
+        // The run's earlier segments, left by this thread in the CTA's place for partial sums.
+        float by = 1.f, by_before = 0.f;
+        if (a.goes_on && live) {
+          const float2 ml = *reinterpret_cast<const float2*>(part + kRows * HD + 2 * local);
+          const float top = fmaxf(m, ml.x);
+          by = exp2_approx(m - top);
+          by_before = exp2_approx(ml.x - top);
+          l = fmaf(l, by, ml.y * by_before);
+          m = top;
+        }
+        const bool writes_out = a.whole && a.last;
 #pragma unroll 1
         for (int c = 0; c < HD / 32; ++c) {
           uint32_t o[32];
@@ -1532,7 +1553,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           // partial sums: [4 dims][row], so that a warp writes 32 rows side by side
           const float inv = l == 0.f ? 0.f : 1.f / l;
           if (!live) continue;
-          if (a.whole) {
+          if (a.goes_on) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 x = *reinterpret_cast<const float4*>(part + ((size_t)((c * 32 + e) / 4) * kRows + local) * 4);
+              o[e] = __float_as_uint(fmaf(__uint_as_float(o[e]), by, x.x * by_before));
+              o[e + 1] = __float_as_uint(fmaf(__uint_as_float(o[e + 1]), by, x.y * by_before));
+              o[e + 2] = __float_as_uint(fmaf(__uint_as_float(o[e + 2]), by, x.z * by_before));
+              o[e + 3] = __float_as_uint(fmaf(__uint_as_float(o[e + 3]), by, x.w * by_before));
+            }
+          }
+          if (writes_out) {
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
               float num[8];
@@ -1549,8 +1580,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         tc_fence_before_sync();  // the next segment's products overwrite the output
       }
-      if (!a.whole) {
-        if (live && !helps) *reinterpret_cast<float2*>(part + kRows * HD + 2 * local) = make_float2(m, l);
+      if (live && !helps && !(a.whole && a.last)) *reinterpret_cast<float2*>(part + kRows * HD + 2 * local) = make_float2(m, l);
+      if (!a.whole && a.last) {
         const int c0 = (int)(((a.first_token + 1) * C - 1) / all);
         const int c1 = (int)(((a.first_token + (long long)(a.steps - 1) * BN + 1) * C - 1) / all);
         __threadfence();

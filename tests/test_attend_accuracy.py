@@ -92,6 +92,16 @@ def flat_case(kind, heads, dim, n, new, seed=0):
     return Case(kind, heads, dim, n, new, k, v, q, ks, vs, 1 / math.sqrt(dim))
 
 
+def sink_case(kind, heads, dim, n, new, bits):
+    """The first token's weight is 2^bits times each other's; its value is 0, the others' is not."""
+    k, v = torch.zeros(n, dim), torch.full((n, dim), 96.0)
+    k[0], v[0] = 64.0, 0.0
+    q = torch.full((new, heads, dim), 0.5).half()
+    blocks = -(-n // BS)
+    ks = torch.full((blocks,), 0.015625)
+    return Case(kind, heads, dim, n, new, k, v, q, ks, torch.full((blocks,), 0.01), bits * math.log(2.0) / (64 * 0.015625 * 0.5 * dim))
+
+
 SHAPES = [("int8", 2, 128, 70001, 1), ("e4m3", 8, 64, 70001, 3), ("e4m3", 2, 256, 40003, 2),   # up to 32 rows
           ("e4m3", 8, 128, 70001, 40), ("int8", 3, 64, 30007, 17), ("int8", 16, 256, 40003, 9)]  # more
 
@@ -119,3 +129,13 @@ def test_the_bound_shows_a_lost_or_doubled_tile(kind, heads, dim, n, new):
         wrong = (num.sum(1, keepdim=True) + times * num) / (den.sum(1, keepdim=True) + times * den)
         worst = ((wrong - o[:, None]).abs() / bound[:, None]).amax((0, 2))[:whole]
         assert worst.min().item() > 2, worst.min().item()
+
+
+# As many requests as keep a CTA at one of them, so that
+# its weights are added up in one place.
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [10.3])
+@pytest.mark.parametrize("kind,heads,dim,n,new", [("int8", 4, 128, 131072, 1), ("e4m3", 1, 64, 131071, 3), ("e4m3", 4, 256, 100003, 1),
+                                                  ("e4m3", 8, 128, 131072, 5), ("int8", 33, 64, 131072, 1), ("int8", 20, 256, 100003, 1)])
+def test_many_small_weights_beside_a_large_one(cuda, kind, heads, dim, n, new, bits):
+    sink_case(kind, heads, dim, n, new, bits).check(cuda, independent=False, requests=444)
