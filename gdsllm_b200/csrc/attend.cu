@@ -15,14 +15,19 @@
 //
 // Products run on 16-bit matrix instructions with fp32 sums.  Every code is
 // exact in fp16, and a query row is scaled by a power of two to at most 1
-// before it becomes fp16, so the only operand that is rounded is the softmax
-// weight (11 bits, as the output has).
+// before it becomes fp16, so what is rounded is the softmax weight, to the 11
+// bits that an fp16 output has.
 //
-// One pass with a running maximum: with lv = log2(vs[page]), a weight is
-// p_j = 2^(s_j log2(e) + lv - r), r the running maximum of s_j log2(e) + lv.
-// p_j is at most 1 whatever the scales are, sum p_j vq_j needs no scale of its
-// own, and the softmax's denominator is sum p_j 2^-lv, kept from the fp32
-// weights before they are rounded.
+// One pass with a running reference point: with lv = log2(vs[page]), a weight is
+// p_j = 2^(s_j log2(e) + lv - r).  r is set kUnder below the largest s_j log2(e)
+// + lv seen, and moved only when a weight would pass 2^kMostWeight, so the largest
+// weight is between 2^kUnder and 2^kMostWeight whatever the scales are: near
+// the top of fp16's range, so that a weight keeps its 11 bits down to 2^-21 of the
+// largest, and a smaller one is off by 2^-32 of the largest at most.  (With the largest
+// at 1, 131072 tokens at 2^-25.2 of one other token, 0.3 % of the softmax, came
+// out as nothing.)  sum p_j vq_j needs no scale of its own, and the softmax's
+// denominator is sum p_j 2^-lv, kept from the fp32 weights before they are rounded
+// (2^-kUnder of it, so that 2^100 from the smallest value scales leaves room for 2^20 tokens).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -43,7 +48,9 @@ constexpr int kAttWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 // Positions of a table row: positions, and those of the 16 tiles of 128 tokens that a lane looks up ahead, stay below 2^31.
 constexpr long long kMostPositions = (1ll << 31) - 4096;
-constexpr float kNoMax = -1e30f;       // the running maximum before any score
+constexpr float kNoMax = -1e30f;       // the reference point before any score
+constexpr float kUnder = 7.f, kMostWeight = 15.f;  // log2
+constexpr float kWeightUnit = 1.f / 128.f;         // 2^-kUnder
 constexpr float kMaxLogScale = 100.f;  // |log2| of a value scale is held to this
 
 struct AttendArgs {
@@ -150,7 +157,7 @@ __device__ __forceinline__ uint64_t l2_policy_normal() {
 // Four dims of one output row.
 __device__ __forceinline__ void store_out(const AttendArgs& p, int start, int h, int row, int d, const float (&num)[4],
                                           float den) {
-  const float inv = den == 0.f ? 0.f : 1.f / den;
+  const float inv = den == 0.f ? 0.f : kWeightUnit / den;
   const long long at = (long long)(start + row / p.group) * p.out_token_stride +
                        (long long)(h * p.group + row % p.group) * p.out_head_stride + d;
   uint2 v;
@@ -178,7 +185,7 @@ __device__ __forceinline__ void store_out8(void* to, bool bf16, const float (&nu
   *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Per-page constants of the softmax: x = kscale factor, y = lv, z = 2^-lv.
+// Per-page constants of the softmax: x = kscale factor, y = lv, z = 2^(-lv - kUnder).
 __device__ __forceinline__ float3 page_constants(const AttendArgs& p, int page, int h) {
   const size_t i = (size_t)page * p.kv_heads + h;
   const float ks = p.k_scale[i], vs = p.v_scale[i];
@@ -186,7 +193,7 @@ __device__ __forceinline__ float3 page_constants(const AttendArgs& p, int page, 
   const float lv = fminf(fmaxf(log2f(vs), -kMaxLogScale), kMaxLogScale);
   // A non-finite scale marks a block that was written with non-finite values:
   // the queries that see it come out as NaN.
-  return make_float3(ks * p.scale, fine ? lv : __int_as_float(0x7fffffff), fine ? exp2f(-lv) : 1.f);
+  return make_float3(ks * p.scale, fine ? lv : __int_as_float(0x7fffffff), fine ? exp2f(-lv - kUnder) : 1.f);
 }
 
 // ---------------------------------------------------------------------------
@@ -588,8 +595,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
               most[y] = fmaxf(most[y], z);
             }
           }
-        // The reference point moves only when a weight would pass 2^8: fp16 holds that as exactly as smaller ones.
-        if (__any_sync(0xffffffffu, fmaxf(most[0], most[1]) > 8.f)) {
+        if (__any_sync(0xffffffffu, fmaxf(most[0], most[1]) > kMostWeight)) {
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             float top = most[y];  // relative to m
@@ -609,9 +615,9 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
             float up;  // how far m rises
             if (m[nt][y] == kNoMax) {
               up = top == -INFINITY ? 0.f : INFINITY;
-              if (top != -INFINITY) m[nt][y] = top;
+              if (top != -INFINITY) m[nt][y] = top - kUnder;
             } else {
-              up = fmaxf(top, 0.f);
+              up = fmaxf(top - kUnder, 0.f);
               m[nt][y] += up;
             }
             const float fade = exp2_approx(-up);
@@ -1418,7 +1424,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           const float4* cs = consts + stage * (BN / 16);
           const int seen = lim - j0;  // columns up to here count
           const bool cut = __any_sync(0xffffffffu, seen < BN - 1);
-          // Weights against the reference point m, in one pass; `over`: one has passed 2^8, which is not stored.
+          // Weights against the reference point m, in one pass; `over`: one has passed 2^kMostWeight, which is not stored.
           uint32_t w[BN / 2];
           float more = 0.f;
           bool over = false;
@@ -1455,7 +1461,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 more = fmaf(sum.x + sum.y, k.z, more);
               }
             }
-            over = __half2float(__hmax(__low2half(high), __high2half(high))) > 256.f;
+            over = __half2float(__hmax(__low2half(high), __high2half(high))) > 32768.f;
           };
           auto both = [&](auto f) {
             if (cut) f(std::true_type{});
@@ -1483,9 +1489,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 }
               });
               float fade = 1.f;
-              if (top > -INFINITY && (top > m || m == kNoMax)) {
-                fade = m == kNoMax ? 0.f : exp2_approx(m - top);
-                m = top;
+              const float to = top - kUnder;
+              if (top > -INFINITY && (to > m || m == kNoMax)) {
+                fade = m == kNoMax ? 0.f : exp2_approx(m - to);
+                m = to;
                 l *= fade;
               }
               if (step > 0) {
@@ -1551,7 +1558,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             for (int e = 0; e < 32; ++e) o[e] = 0;
           }
           // partial sums: [4 dims][row], so that a warp writes 32 rows side by side
-          const float inv = l == 0.f ? 0.f : 1.f / l;
+          const float inv = l == 0.f ? 0.f : kWeightUnit / l;
           if (!live) continue;
           if (a.goes_on) {
 #pragma unroll
@@ -1600,7 +1607,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               den = fmaf(ml.y, exp2_approx(ml.x - high), den * exp2_approx(top - high));
               top = high;
             }
-            const float inv = den == 0.f ? 0.f : 1.f / den;
+            const float inv = den == 0.f ? 0.f : kWeightUnit / den;
 #pragma unroll 1
             for (int d = helps ? HD / 2 : 0; d < (QT == 1 && !helps ? HD / 2 : HD); d += 32) {
               float num[32];

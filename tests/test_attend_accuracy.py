@@ -131,10 +131,10 @@ def test_the_bound_shows_a_lost_or_doubled_tile(kind, heads, dim, n, new):
         assert worst.min().item() > 2, worst.min().item()
 
 
-# As many requests as keep a CTA at one of them, so that
-# its weights are added up in one place.
+# 2^-25.2 of the largest is below fp16's smallest number, 2^-24.4 a little above it.  As many requests as keep a CTA at one of them, so
+# that its weights share a reference point.
 @pytest.mark.gpu
-@pytest.mark.parametrize("bits", [10.3])
+@pytest.mark.parametrize("bits", [10.3, 20.5, 24.4, 25.2, 28.0])
 @pytest.mark.parametrize("kind,heads,dim,n,new", [("int8", 4, 128, 131072, 1), ("e4m3", 1, 64, 131071, 3), ("e4m3", 4, 256, 100003, 1),
                                                   ("e4m3", 8, 128, 131072, 5), ("int8", 33, 64, 131072, 1), ("int8", 20, 256, 100003, 1)])
 def test_many_small_weights_beside_a_large_one(cuda, kind, heads, dim, n, new, bits):
