@@ -14,9 +14,10 @@
 // one matrix product per (request, KV head).
 //
 // Products run on 16-bit matrix instructions with fp32 sums.  Every code is
-// exact in fp16, and a query row is scaled by a power of two to at most 1
-// before it becomes fp16, so what is rounded is the softmax weight, to the 11
-// bits that an fp16 output has.
+// exact in fp16.  A query row is scaled by a power of two to just under 2^15, the
+// top of fp16's range, so that all elements down to 2^-29 of its largest keep the
+// bits they came with, and a smaller one is off by 2^-40 of the largest at most.
+// So what is rounded is the softmax weight, to the 11 bits that an fp16 output has.
 //
 // One pass with a running reference point: with lv = log2(vs[page]), a weight is
 // p_j = 2^(s_j log2(e) + lv - r).  r is set kUnder below the largest s_j log2(e)
@@ -51,6 +52,7 @@ constexpr long long kMostPositions = (1ll << 31) - 4096;
 constexpr float kNoMax = -1e30f;       // the reference point before any score
 constexpr float kUnder = 7.f, kMostWeight = 15.f;  // log2
 constexpr float kWeightUnit = 1.f / 128.f;         // 2^-kUnder
+constexpr int kQTop = 15;                          // a query row's elements are below 2^kQTop as fp16
 constexpr float kMaxLogScale = 100.f;  // |log2| of a value scale is held to this
 
 struct AttendArgs {
@@ -130,6 +132,11 @@ struct Code<GDSQ_CACHE_E4M3> {
 
 __device__ __forceinline__ float2 unpack_q(bool bf16, uint32_t w) {
   return bf16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w)) : __half22float2(u32_as_h2(w));
+}
+
+// The power of two that a q row with this largest magnitude is below; a row with inf or NaN keeps its values.
+__device__ __forceinline__ int q_exponent(float most) {
+  return isfinite(most) ? max((int)(__float_as_uint(most) >> 23) - 126, -100) : kQTop;
 }
 
 // N pairs of one q row, from element i (aligned to N pairs).
@@ -472,12 +479,9 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
         most = fmaxf(most, fmaxf(fabsf(x.x), fabsf(x.y)));
       }
       most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
-      int ex = (int)(__float_as_uint(most) >> 23) - 126;  // most < 2^ex
-      ex = isfinite(most) ? min(max(ex, -100), 100) : 0;
-      const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
-      if (lane == 0) {
-        qexp[i] = __uint_as_float((uint32_t)(127 + ex) << 23);
-      }
+      const int ex = q_exponent(most);
+      const float by = __uint_as_float((uint32_t)(127 + kQTop - ex) << 23);
+      if (lane == 0) qexp[i] = __uint_as_float((uint32_t)(127 - kQTop + ex) << 23);
 #pragma unroll
       for (int e = 0; e < HD / 32; e += 2) {
         const int d = lane * (HD / 32) + e;
@@ -487,7 +491,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
         const int reg = (w & 1) * 2 + (b >> 1);
         const int ln = (i & 7) * 4 + tt;
         reinterpret_cast<uint32_t*>(qf + (((i >> 3) * kSteps + part * kWords + w) >> 1) * 32 + ln)[reg] =
-            h2_as_u32(__floats2half2_rn(v[e] * down, v[e + 1] * down));
+            h2_as_u32(__floats2half2_rn(v[e] * by, v[e + 1] * by));
       }
     }
     float3 cc = make_float3(0.f, 0.f, 0.f), nc = cc;
@@ -1375,22 +1379,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 for (int c = 0; c < kBatch; ++c) most[c] = fmaxf(most[c], __shfl_xor_sync(0xffffffffu, most[c], d));
 #pragma unroll
               for (int c = 0; c < kBatch; ++c) {
-                int ex = (int)(__float_as_uint(most[c]) >> 23) - 126;  // most < 2^ex
-                ex = isfinite(most[c]) ? min(max(ex, -100), 100) : 0;
-                const float down = sign * __uint_as_float((uint32_t)(127 - ex) << 23);
+                const int ex = q_exponent(most[c]);
+                const float by = sign * __uint_as_float((uint32_t)(127 + kQTop - ex) << 23);
                 const int at = r0 + c * kAtOnce + sub;
                 // the row's own thread keeps its scale
 #pragma unroll
                 for (int s = 0; s < kAtOnce; ++s) {
                   const int theirs = __shfl_sync(0xffffffffu, ex, s * kLanes);
-                  if (lane == r0 + c * kAtOnce + s) qe = __uint_as_float((uint32_t)(127 + theirs) << 23);
+                  if (lane == r0 + c * kAtOnce + s) qe = __uint_as_float((uint32_t)(127 - kQTop + theirs) << 23);
                 }
                 const uint32_t ww[4] = {w[c].x, w[c].y, w[c].z, w[c].w};
                 uint32_t o[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const float2 f = unpack_q(kBf16, ww[e]);
-                  o[e] = h2_as_u32(__floats2half2_rn(f.x * down, f.y * down));
+                  o[e] = h2_as_u32(__floats2half2_rn(f.x * by, f.y * by));
                 }
                 sts128(place_of(at), o[0], o[1], o[2], o[3]);
               }

@@ -139,3 +139,22 @@ def test_the_bound_shows_a_lost_or_doubled_tile(kind, heads, dim, n, new):
                                                   ("e4m3", 8, 128, 131072, 5), ("int8", 33, 64, 131072, 1), ("int8", 20, 256, 100003, 1)])
 def test_many_small_weights_beside_a_large_one(cuda, kind, heads, dim, n, new, bits):
     sink_case(kind, heads, dim, n, new, bits).check(cuda, independent=False, requests=444)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ratio", [2.0 ** -12, 2.0 ** -17, 2.0 ** -22])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("kind,heads,dim,n,new", [("int8", 4, 64, 50, 1), ("e4m3", 2, 128, 50, 8), ("int8", 2, 256, 50, 8),
+                                                  ("e4m3", 1, 64, 90, 40), ("int8", 2, 128, 90, 40), ("e4m3", 2, 256, 90, 40)])
+def test_small_query_elements_beside_a_large_one(cuda, kind, heads, dim, n, new, dtype, ratio):
+    """The query's largest element meets keys of zero: the scores come from elements far smaller."""
+    gen = torch.Generator().manual_seed(dim + new)
+    top = TOP[kind]
+    k = (torch.randn(n, dim, generator=gen) * top / 4).clamp(-top, top)
+    k = k.round() if kind == "int8" else k.to(CODE[kind]).float()
+    k[:, 5] = 0
+    q = torch.randn(new, heads, dim, generator=gen) * ratio
+    q[:, :, 5] = 1.0
+    blocks = -(-n // BS)
+    Case(kind, heads, dim, n, new, k, torch.randint(-14, 15, (n, dim), generator=gen) * 8.0, (q * 50000).to(dtype), torch.full((blocks,), 4 / top),
+         torch.full((blocks,), 0.01), 4 / (50000 * ratio * math.sqrt(dim))).check(cuda, independent=False)
