@@ -53,7 +53,8 @@ constexpr float kNoMax = -1e30f;       // the reference point before any score
 constexpr float kUnder = 7.f, kMostWeight = 15.f;  // log2
 constexpr float kWeightUnit = 1.f / 128.f;         // 2^-kUnder
 constexpr int kQTop = 15;                          // a query row's elements are below 2^kQTop as fp16
-constexpr float kMaxLogScale = 100.f;  // |log2| of a value scale is held to this
+// log2 of a value scale is held to these.  The cache write stores a scale below 2^-100 as zero, and none above 2^122.
+constexpr float kLeastLogScale = -100.f, kMostLogScale = 126.f;
 
 struct AttendArgs {
   const void* q;
@@ -197,7 +198,7 @@ __device__ __forceinline__ float3 page_constants(const AttendArgs& p, int page, 
   const size_t i = (size_t)page * p.kv_heads + h;
   const float ks = p.k_scale[i], vs = p.v_scale[i];
   const bool fine = isfinite(vs);
-  const float lv = fminf(fmaxf(log2f(vs), -kMaxLogScale), kMaxLogScale);
+  const float lv = fminf(fmaxf(log2f(vs), kLeastLogScale), kMostLogScale);
   // A non-finite scale marks a block that was written with non-finite values:
   // the queries that see it come out as NaN.
   return make_float3(ks * p.scale, fine ? lv : __int_as_float(0x7fffffff), fine ? exp2f(-lv - kUnder) : 1.f);

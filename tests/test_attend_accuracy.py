@@ -158,3 +158,30 @@ def test_small_query_elements_beside_a_large_one(cuda, kind, heads, dim, n, new,
     blocks = -(-n // BS)
     Case(kind, heads, dim, n, new, k, torch.randint(-14, 15, (n, dim), generator=gen) * 8.0, (q * 50000).to(dtype), torch.full((blocks,), 4 / top),
          torch.full((blocks,), 0.01), 4 / (50000 * ratio * math.sqrt(dim))).check(cuda, independent=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("log_scale", [-96, 60, 99, 105, 119])
+@pytest.mark.parametrize("kind,heads,dim,n,new", [("int8", 4, 128, 300, 1), ("e4m3", 8, 64, 300, 3), ("e4m3", 4, 256, 300, 9), ("int8", 8, 128, 300, 40)])
+def test_value_scales_over_bf16s_range(cuda, kind, heads, dim, n, new, log_scale):
+    """Values far outside fp16's range; the largest are 2^126."""
+    case = flat_case(kind, heads, dim, n, new)
+    case.q, case.vs = case.q.bfloat16(), case.vs * 2.0 ** (log_scale - math.log2(case.vs[0].item()))
+    case.check(cuda, independent=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("new", [1, 40])
+def test_large_bf16_values_written_and_read(cuda, kind, new):
+    """Written by the cache write, read by attention: one token's value comes back."""
+    dim, n = 64, 40
+    caches = [torch.zeros(1, 1, BS, dim, dtype=torch.uint8, device=cuda).view(CODE[kind]) for _ in range(2)]
+    scales = [torch.zeros(1, 1, device=cuda) for _ in range(2)]
+    v = torch.full((n, 1, dim), 2.0 ** 125, dtype=torch.bfloat16, device=cuda)
+    i32 = lambda *t: torch.tensor(t, dtype=torch.int32, device=cuda)  # noqa: E731
+    paged.append_kv8(torch.zeros_like(v), v, torch.arange(n, device=cuda), *caches, *scales)
+    q = torch.ones(new, 1, dim, dtype=torch.bfloat16, device=cuda)
+    got = paged.attend_kv8(q, *caches, *scales, i32(0)[None], i32(n), i32(0, new), new)
+    # the code is top itself; the scale's rounding, the weights' and bf16's
+    assert bool(((got.double() / 2.0 ** 125 - 1).abs() <= 2.0 ** -8 + 2.0 ** -10).all())
