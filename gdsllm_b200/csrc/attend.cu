@@ -180,8 +180,15 @@ __device__ __forceinline__ void store_out(const AttendArgs& p, int start, int h,
   *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + at) = v;
 }
 
-// Eight dims of one output row.
-// 8 values of an output row, from `to`.
+// Tokens behind the last request's (a step padded to a fixed size) belong to none: zeros.
+// `thread` of the `threads` in every CTA that share the work.
+__device__ __forceinline__ void zero_padding(const AttendArgs& p, int thread, int threads) {
+  const long long first = max(min(p.starts[p.requests], p.tokens), 0) * p.out_token_stride / 8, last = p.tokens * p.out_token_stride / 8;
+  for (long long i = first + (long long)blockIdx.x * threads + thread; i < last; i += (long long)gridDim.x * threads)
+    static_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
+}
+
+// Eight dims of one output row, from `to`.
 __device__ __forceinline__ void store_out8(void* to, bool bf16, const float (&num)[8], float inv) {
   uint32_t w[4];
 #pragma unroll
@@ -333,6 +340,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, (stream_per_sm<HD, NT>()))
     if (w < warp) before += shared_ll[w];
     all += shared_ll[w];
   }
+  zero_padding(p, threadIdx.x, kAttWarps * 32);
   const long long C = min((long long)gridDim.x, all);  // every CTA in use has a step
   if (blockIdx.x >= C) return;
   long long s0 = all * blockIdx.x / C;
@@ -840,7 +848,7 @@ size_t stream_workspace(int sms) {
 //               TMEM, weights back to TMEM over them, in the end the output.
 //   warps 8-11  widen the 8-bit tiles to fp16
 //   warp 12     issues the products
-//   warp 13     TMA of the 8-bit tiles, and the blocks' scales (14 and 15 idle)
+//   warp 13     TMA of the 8-bit tiles, and the blocks' scales (14 and 15: zeros for the step's padding)
 //
 // K and V are widened to the same layout, [64 dims][token][128 bytes], 128-byte
 // swizzled: K major for the scores (a row of B is a token) and N major for the
@@ -1270,6 +1278,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       else products(std::integral_constant<int, 1>{});
       commit(o_full);
     }
+  } else {
+    zero_padding(p, threadIdx.x - (kTmaWarp + 1) * 32, kTileThreads - (kTmaWarp + 1) * 32);
   }
   } else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWidenRegs));

@@ -209,6 +209,7 @@ Tensor attend_kv8(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
   on_gpu(q);
   const c10::cuda::CUDAGuard guard(q.device());
   if (!out) out = make(q.sizes(), q.scalar_type(), q);
+  if (r == 0 || max_query_len == 0) out->zero_();  // no token belongs to a request; the C call has nothing to do
   if (!workspace) workspace = attend_workspace(r, max_query_len, heads, c.heads, c.dim, q.device());
   const int width = small(table.size(1), "table width");
   check(gdsq_attend_kv8(q.const_data_ptr(), elem_type(q), q.stride(0), q.stride(1), k_cache.const_data_ptr(),

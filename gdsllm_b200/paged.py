@@ -83,7 +83,7 @@ def attend_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_
     heads in order (heads a multiple of kv_heads).  ``max_query_len`` and
     ``max_seq_len`` (default: what the block table can hold) bound the
     lengths, which the host does not see.  Returns [T, heads, dim]; a query
-    that sees nothing gives zeros.  ``workspace``: see ``attend_workspace``
+    that sees nothing gives zeros, as does a token behind the last request's.  ``workspace``: see ``attend_workspace``
     (allocated for the call when not given)."""
     return ext().attend_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_starts, max_query_len,
                             max_seq_len, softmax_scale, out, workspace)

@@ -414,7 +414,9 @@ GDSQ_API int gdsq_append_kv8(int elem_type, const void* q, long long q_token_str
  * query_starts[r] .. query_starts[r+1]-1 are the last new tokens of request
  * r's seq_lens[r], and each sees the positions up to its own.  Query heads
  * h*G..h*G+G-1 (G = num_heads / num_kv_heads) read KV head h.  out: contiguous,
- * q's type; a query that sees nothing gives zeros.  max_query_len and
+ * q's type; a query that sees nothing gives zeros, and so do tokens from
+ * query_starts[num_requests] on (with no request, no token or max_query_len 0
+ * nothing is launched and out is not written).  max_query_len and
  * max_seq_len bound the requests' new tokens and lengths (they size the
  * launch; tokens past max_query_len of a request are left unwritten).
  * workspace: workspace_bytes of device memory, zeroed before its first use
