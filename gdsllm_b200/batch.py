@@ -85,7 +85,10 @@ class BatchLlama:
     def step(self, new_tokens: list[list[int]]) -> torch.Tensor:
         """Appends ``new_tokens[r]`` (may be empty) to request r and returns
         the logits [max_requests, vocab] after its last token (a request
-        without new tokens: those of the step's last token, to be ignored)."""
+        without new tokens: those of the step's last token, to be ignored).
+        A step that raises leaves every request as it was: the host's lengths
+        and the queue of free blocks move when all its work is launched, and
+        tokens written past a request's length are written again."""
         if len(new_tokens) != self.max_requests:
             raise ValueError(f"BatchLlama: {len(new_tokens)} lists for {self.max_requests} requests")
         counts = [len(t) for t in new_tokens]
@@ -104,9 +107,6 @@ class BatchLlama:
         ids, context, new = (torch.tensor(v, dtype=t, device=self.device) for v, t in (
             ([i for t in new_tokens for i in t], torch.int64), (self.lengths, torch.int32), (counts, torch.int32)))
         t = paged.build_tables(context, new, self.table, self.free, self.free_head, bs, tokens)
-        self.free_head = t.free_head
-        self.blocks_left -= taken
-        self.lengths = after
         d = self.head_dim
         h = self._embed(ids)
         delta = None
@@ -121,7 +121,11 @@ class BatchLlama:
             delta, = self._project([lay.down], capi.silu_mul(*self._project([lay.gate, lay.up], x)))
         last = (t.query_starts[1:].long() - 1).clamp_min(0)
         x = capi.add_rmsnorm(h[last].contiguous(), self.final_norm, self.eps, delta=delta[last].contiguous())
-        return self._project([self.lm], x)[0]
+        logits, = self._project([self.lm], x)
+        self.free_head = t.free_head
+        self.blocks_left -= taken
+        self.lengths = after
+        return logits
 
     def release(self, request: int) -> None:
         """Frees a finished request's cache blocks for the requests to come."""
