@@ -147,6 +147,10 @@ class BatchLlama:
         again afterwards."""
         if not 0 < len(prompts) <= self.max_requests or any(self.lengths) or not all(prompts):
             raise ValueError(f"BatchLlama: 1 to {self.max_requests} non-empty prompts, with no request being served")
+        if new_tokens < 0:
+            raise ValueError(f"BatchLlama: {new_tokens} new tokens")
+        if new_tokens == 0:
+            return torch.empty(len(prompts), 0, dtype=torch.int64), torch.empty(len(prompts), 0)
         n, dev = len(prompts), self.device
         gen = torch.Generator(device=dev).manual_seed(seed)
         rows = dict(temperature=torch.full((n,), temperature, device=dev), top_k=torch.full((n,), top_k, dtype=torch.int32, device=dev),

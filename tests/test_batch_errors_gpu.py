@@ -50,3 +50,12 @@ def test_a_step_that_raises_can_be_tried_again(cuda, model, monkeypatch, cache, 
         bad.release(r)
     assert bad.blocks_left == 20 and sorted(bad.free.tolist()) == list(range(20))
     assert capi.device_error(0) == 0
+
+
+def test_generate_no_tokens(cuda, model):
+    b = served(model, torch.int8)
+    tokens, logprobs = b.generate([[1, 2], [3]], 0)
+    assert tokens.shape == logprobs.shape == (2, 0) and tokens.dtype == torch.int64 and logprobs.dtype == torch.float32
+    assert b.blocks_left == 20 and b.lengths == [0, 0, 0]
+    with pytest.raises(ValueError, match="-1 new tokens"):
+        b.generate([[1, 2], [3]], -1)
