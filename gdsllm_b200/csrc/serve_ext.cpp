@@ -217,7 +217,7 @@ Tensor attend_kv8(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
                         c.blocks, c.block, static_cast<const int32_t*>(tb), width, static_cast<const int32_t*>(ln),
                         static_cast<const int32_t*>(st), small(r, "requests"), small(q.size(0), "tokens"),
                         small(max_query_len, "max_query_len"),
-                        small(max_seq_len ? *max_seq_len : static_cast<int64_t>(width) * c.block, "max_seq_len"),
+                        small(max_seq_len.value_or(0), "max_seq_len"),
                         small(heads, "heads"), c.heads, c.dim,
                         static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(c.dim))), out->data_ptr(),
                         workspace->data_ptr(), workspace->nbytes(), stream_of(q)),

@@ -80,10 +80,12 @@ def attend_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_
     """Attention of the new tokens q [T, heads, dim] over the cache: request
     r's tokens are ``query_starts[r]:query_starts[r + 1]``, the last of its
     ``seq_lens[r]``, and each sees the positions up to its own.  Heads share KV
-    heads in order (heads a multiple of kv_heads).  ``max_query_len`` and
-    ``max_seq_len`` (default: what the block table can hold) bound the
-    lengths, which the host does not see.  Returns [T, heads, dim]; a query
-    that sees nothing gives zeros, as does a token behind the last request's.  ``workspace``: see ``attend_workspace``
+    heads in order (heads a multiple of kv_heads).  ``max_query_len`` is the
+    largest number of new tokens of a request, which the host does not see: it
+    chooses the kernel, and a request with more is only slower.  Nothing
+    depends on ``max_seq_len``, which callers that have it may give.  Returns
+    [T, heads, dim]; a query that sees nothing gives zeros, as does a token behind
+    the last request's.  ``workspace``: see ``attend_workspace``
     (allocated for the call when not given)."""
     return ext().attend_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_starts, max_query_len,
                             max_seq_len, softmax_scale, out, workspace)

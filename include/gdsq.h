@@ -416,9 +416,10 @@ GDSQ_API int gdsq_append_kv8(int elem_type, const void* q, long long q_token_str
  * h*G..h*G+G-1 (G = num_heads / num_kv_heads) read KV head h.  out: contiguous,
  * q's type; a query that sees nothing gives zeros, and so do tokens from
  * query_starts[num_requests] on (with no request, no token or max_query_len 0
- * nothing is launched and out is not written).  max_query_len and
- * max_seq_len bound the requests' new tokens and lengths (they size the
- * launch; tokens past max_query_len of a request are left unwritten).
+ * nothing is launched and out is not written).
+ * max_query_len, the largest number of new tokens of a request, chooses the
+ * kernel and with it the least workspace; a request with more is computed all the
+ * same, only slower.  max_seq_len must not be negative; nothing depends on it.
  * workspace: workspace_bytes of device memory, zeroed before its first use
  * and left zeroed where it has to be by every call; calls that may overlap
  * need one each.  gdsq_attend_kv8_workspace says how much a call can use. A

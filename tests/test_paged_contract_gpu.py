@@ -49,3 +49,17 @@ def test_a_step_without_requests_gives_zeros(cuda):
     out.fill_(math.nan)
     paged.attend_kv8(q, *cache, table, ints(lens, cuda), ints([0, 0], cuda), 1, out=out)
     assert not out.any()
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 64), (16, 1, 128), (12, 1, 256)])
+def test_lengths_that_the_host_was_not_told(cuda, heads, kv_heads, dim):
+    """max_query_len chooses the kernel only, max_seq_len nothing: more tokens and longer requests than they say are right."""
+    new = [1, 70, 3, 0]
+    q, cache, table, lens, starts = step(cuda, [200, 300, 3, 5], new, heads, kv_heads, dim)
+    want, bound = attend_ref(q, *cache, table, lens, starts, 1 / math.sqrt(dim), 2.0 ** -11)
+    for longest in (1, 2, 4, 70):
+        ws = paged.attend_workspace(4, longest, heads, kv_heads, dim, cuda)
+        for seq in (None, 0, 7, 300):
+            got = paged.attend_kv8(q, *cache, table, ints(lens, cuda), ints(starts, cuda), longest, seq, workspace=ws)
+            assert bool(((got.double() - want).abs() <= bound).all())
+    assert capi.device_error(0) == 0
