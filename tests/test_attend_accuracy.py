@@ -112,6 +112,13 @@ def test_long_and_flat(cuda, kind, heads, dim, n, new):
     flat_case(kind, heads, dim, n, new).check(cuda, independent=True)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,heads,dim,n,new", SHAPES[3:])
+def test_long_and_flat_for_many_requests(cuda, kind, heads, dim, n, new):
+    """More requests than two thirds of the CTAs: each takes tens of thousands of tokens of a request and leaves it to the next."""
+    flat_case(kind, heads, dim, n, new).check(cuda, independent=True, requests=101)
+
+
 @pytest.mark.parametrize("kind,heads,dim,n,new", [s[:4] + (1,) for s in SHAPES])
 def test_the_bound_shows_a_lost_or_doubled_tile(kind, heads, dim, n, new):
     """Every tile of 32 tokens, left out of the reference or counted twice, takes some output further than twice the bound."""
