@@ -224,11 +224,12 @@ __device__ __forceinline__ float3 page_constants(const AttendArgs& p, int page, 
 // first: two requests of 131072 tokens, 64 heads on 8 of 128, took 2146 us with
 // one CTA for each (request, KV head).
 //
-// Measured, on the GPU alone: those two requests 99.8 us, 5.4 TB/s (82 % of a
-// copy's rate); 64 requests of 1 to 16384 tokens, the same heads, e4m3, 46.8 us,
-// 70 %, the rest being the cut, the filling of the rings and the joins; one
-// request of 513 tokens with 32 heads 9.7 us, bound by the latency of the
-// schedule, one step and the join.
+// Measured, on the GPU alone: those two requests 100 us, 5.4 TB/s (82 % of a
+// copy's rate); 64 requests of 1 to 16384 tokens, the same heads, e4m3, 47.4 us,
+// 69 %, the rest being the cut, the filling of the rings and the joins; one
+// request of 513 tokens with 32 heads 10.2 us, bound by the latency of a chain:
+// lengths, table and scales, copies, a step, the warps' join, partial sums out, the
+// counter, partial sums back.
 //
 // In a step, warp w takes the 32 tokens from 32 w, through its own ring of
 // TMA boxes of 16 tokens (one block holds at least 16).  A lane looks up the
@@ -860,11 +861,12 @@ size_t stream_workspace(int sms) {
 // softmax runs beside the products all the same.
 //
 // Measured: three prompts of up to 2048 tokens over up to 6000 cached, 64 heads on
-// 8 of 128, e4m3: 566 us, 862 TFLOP/s counting the visible positions (53 % of the
-// measured matrix rate), where one tile with mma.sync took 3220; 33 requests with
-// five tokens each, 32 heads on 2 of 256, over up to 2047: 31 us, bound by latency
-// (the schedule 3 k cycles, Q 8 k, a step 2 k, the output 2 k, a join 10 k).  A step of two
-// tiles takes about 4600 cycles: 2048 are the exponential unit's (32768 weights,
+// 8 of 128, e4m3: 539 us, 905 TFLOP/s counting the visible positions (55 % of the
+// measured matrix rate), where one tile with mma.sync took 3220; the same with 32
+// heads on 8 of 64: 260 us, 470 TFLOP/s; 33 requests with five tokens each, 32 heads on
+// 2 of 256, over up to 2047: 30 to 33 us, bound by latency (the schedule 3 k cycles, Q 8 k,
+// a step 2 k, the output 2 k, a join 10 k).  A step of two tiles took about 4600 cycles
+// when the prompts took 566 us: 2048 are the exponential unit's (32768 weights,
 // 16 a cycle), 2600 the products', at 80 to 90 cycles where alone they take 64,
 // since the widening and the Q tiles use the same shared memory, and the two
 // overlap in part.  A polynomial for some of the exponentials was slower (936
@@ -890,8 +892,9 @@ constexpr int kTileThreads = 16 * 32;
 // exact as fp16 shows (1.8e-4, the rounding of the output).
 constexpr int kChain = 16384;
 // What beginning and ending an item costs, in tokens: the three prompts above
-// take 565 us with 896, 576 with 768 and 569 with 1024; for heads of 256 the 33
-// requests with five tokens take 30.1 us with 320, 31.0 with 448.
+// take 539 us with 896, 555 with 768 and 543 with 1024, and with heads of 64 260 with
+// 896, 279 with 448 and 268 with 1792 (33 requests of ten tokens on them 36, 30 and 44);
+// for heads of 256 the 33 requests with five tokens take 33.0 us with 320, 33.5 with 448.
 template <int HD>
 __host__ __device__ constexpr int item_tokens() { return HD == 256 ? 320 : 896; }
 // Registers per thread of the softmax, widening and other warp groups: together the launch's 4 x 128.
@@ -979,7 +982,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   using L = TileLayout<HD>;
   constexpr int QT = L::QT, BN = L::BN, kRows = L::kRows;
   constexpr int kParts = HD >= 128 ? HD / 128 : 1, kPart = HD >= 128 ? 128 : 64;
-  constexpr uint32_t kOCol = 2 * BN;  // scores of the tiles first (one tile: the second place is unused)
+  constexpr uint32_t kOCol = 2 * BN;  // after the scores: of two tiles, or of one tile in two places
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   const uint32_t sbase = smem_addr(smem);
@@ -1721,7 +1724,10 @@ int launch_stream(const AttendArgs& a, const DeviceInfo& dev, void* workspace, s
 // Rows per (request, KV head) up to which the stream kernel is taken; a tile's 128
 // rows are a whole product however few are filled.  Stream against tile, heads of
 // 128: 20 rows of 32 requests of 2000 tokens 70 and 84 us, 24 rows of 64 of 4000
-// 187 and 251, 32 rows of 16 of 2000 (32 KV heads) 126 and 160.  Heads of 256 leave
+// 187 and 251, 32 rows of 16 of 2000 (32 KV heads) 126 and 160.  From 33 rows on the stream
+// kernel reads the cache twice: 40 rows of those requests 127 and 89, 367 and 260, 222
+// and 164; 64 rows 136 and 88, 381 and 262, 239 and 176; with heads of 64 (32 requests
+// of 2000 tokens, 8 KV heads) 72 and 73 with 40 rows, 77 and 73 with 64.  Heads of 256 leave
 // the stream kernel registers for 16 rows only: 32 rows of 16 requests of 1000
 // tokens would take it two readings of the cache, 33 us, and take the tile kernel 26.
 template <int HD>
